@@ -28,6 +28,8 @@ OP_EXPORTS = (
     "dagnet_op_bn_moments", "dagnet_op_bn_merge", "dagnet_op_bn_apply", "dagnet_op_bn_bwd_sums", "dagnet_op_bn_bwd_apply",
     "dagnet_op_gat_attn_fwd", "dagnet_op_gat_attn_bwd", "dagnet_op_adj_matmul", "dagnet_op_disposition", "dagnet_op_sumsq",
     "dagnet_op_adam",
+    "dagnet_op_attn_fwd", "dagnet_op_attn_bwd_workspace", "dagnet_op_attn_bwd", "dagnet_op_attn_step_workspace", "dagnet_op_attn_step",
+    "dagnet_op_rotary",
 )
 
 _bound = False
@@ -93,6 +95,15 @@ def _lib():
         lib.dagnet_op_disposition.argtypes = [vp, i32, vp, vp, i64, vp]
         lib.dagnet_op_sumsq.argtypes = [i64, vp, vp, vp]
         lib.dagnet_op_adam.argtypes = [i64, vp, vp, vp, vp, vp, f32, f32, f32, f32, f32, i32, vp]
+        lib.dagnet_op_attn_fwd.argtypes = [vp, vp, vp, vp, vp, vp, vp]
+        lib.dagnet_op_attn_bwd_workspace.argtypes = [vp]
+        lib.dagnet_op_attn_bwd_workspace.restype = i64
+        lib.dagnet_op_attn_bwd.argtypes = [vp, vp, vp, vp, vp, vp, i64, i64, vp, vp, vp, vp, vp, vp, vp, vp]
+        lib.dagnet_op_attn_step_workspace.argtypes = [vp, i32, i32, i32]
+        lib.dagnet_op_attn_step_workspace.restype = i64
+        lib.dagnet_op_attn_step.argtypes = [vp, vp, vp, i32, i32, i32, i64, i64, vp, vp, vp]
+        lib.dagnet_op_rotary.argtypes = [i64, i32, i32, i32, i32, vp, i64, i64, vp, i64, i64, vp, i32, i32, vp, vp, i32, i32, i32, vp, i64, i64,
+                                         vp, i64, i64, vp]
         _bound = True
     return lib
 
@@ -1646,3 +1657,128 @@ class ClipAdam:
 
     def total_norm(self) -> torch.Tensor:
         return self.sumsq.sqrt().float()
+
+
+# ---------------------------------------------------------------------------------------------
+# attention over the rows of a scene, rotary positions (public names and argument checks: dagnet_amd.attention)
+# ---------------------------------------------------------------------------------------------
+class _Attn(C.Structure):                       # dagnet_attn
+    _fields_ = [(n, C.c_void_p) for n in ("q", "k", "v", "slopes", "q_pos", "k_pos")] + \
+               [(n, C.c_int64) for n in ("q_row", "q_head", "k_row", "k_head", "v_row", "v_head")] + \
+               [(n, C.c_int32) for n in ("nq", "nk", "n_heads", "n_kv_heads", "head_dim", "axes", "dtype")] + \
+               [("scale", C.c_float), ("softcap", C.c_float)]
+
+
+def _addr(t):
+    return None if t is None else t.data_ptr()
+
+
+def _attn_struct(q, k, v, slopes, pos, k_pos, nk, scale, softcap):
+    """q [nq, H, D], k and v [..., KV, D] (their row and head strides are those of the last three dimensions)."""
+    axes = 0 if slopes is None else pos.shape[-1]
+    qs, ks, vs = q.stride(), k.stride(), v.stride()
+    return _Attn(q.data_ptr(), k.data_ptr(), v.data_ptr(), _addr(slopes), _addr(pos), _addr(k_pos), qs[0], qs[1], ks[-3], ks[-2], vs[-3], vs[-2],
+                 q.shape[0], nk, q.shape[1], k.shape[-2], q.shape[2], axes, int(q.dtype == torch.bfloat16), scale, softcap)
+
+
+def _on(device):
+    """The calls launch on the CURRENT device; tensors of another one make it current for the call."""
+    return contextlib.nullcontext() if device.index == torch.cuda.current_device() else torch.cuda.device(device)
+
+
+def _heads(t: torch.Tensor) -> torch.Tensor:
+    """A gradient as autograd hands it over -> unit column stride."""
+    return t if t.stride(-1) == 1 or t.shape[-1] == 1 else t.contiguous()
+
+
+class SceneAttnFn(torch.autograd.Function):
+    """Attention over the rows of a scene (include/dagnet_hip.h, dagnet_op_attn_fwd / _bwd).  ``tables``: layout.tables(device)."""
+
+    @staticmethod
+    def forward(ctx, q, k, v, slopes, tables, scale, softcap, pos, k_pos):
+        row_lo, row_hi = tables[:2]
+        grad = any(ctx.needs_input_grad[:4])
+        out = torch.empty(q.shape, dtype=q.dtype, device=q.device)
+        lse = torch.empty(q.shape[0] * q.shape[1], dtype=torch.float32, device=q.device) if grad else None
+        o32 = torch.empty(q.shape, dtype=torch.float32, device=q.device) if grad and q.dtype != torch.float32 else None
+        a = _attn_struct(q, k, v, slopes, pos, k_pos, k.shape[0], scale, softcap)
+        with _on(q.device):
+            _check(_lib().dagnet_op_attn_fwd(C.byref(a), row_lo, row_hi, out.data_ptr(), _addr(lse), _addr(o32), _stream(q.device)))
+        if grad:
+            ctx.save_for_backward(q, k, v, slopes, pos, k_pos, lse, out if o32 is None else o32)
+            ctx.meta = (tables, scale, softcap)
+        return out
+
+    @staticmethod
+    @torch.autograd.function.once_differentiable
+    def backward(ctx, dout):
+        q, k, v, slopes, pos, k_pos, lse, o = ctx.saved_tensors
+        tables, scale, softcap = ctx.meta
+        row_lo, row_hi, key_lo, key_hi = tables[:4]
+        need_q, need_k, need_v, need_s = ctx.needs_input_grad[:4]
+        dout = _heads(dout)
+        dev = q.device
+        a = _attn_struct(q, k, v, slopes, pos, k_pos, k.shape[0], scale, softcap)
+        dq = torch.empty(q.shape, dtype=q.dtype, device=dev) if need_q or need_s else None
+        dk = torch.empty(k.shape, dtype=k.dtype, device=dev) if need_k or need_v else None
+        dv = torch.empty(v.shape, dtype=v.dtype, device=dev) if need_k or need_v else None
+        ds = torch.zeros(slopes.shape, dtype=torch.float32, device=dev) if need_s else None
+        with _on(dev):
+            ws = torch.empty(_lib().dagnet_op_attn_bwd_workspace(C.byref(a)), dtype=torch.float32, device=dev)
+            _check(_lib().dagnet_op_attn_bwd(C.byref(a), row_lo, row_hi, key_lo, key_hi, dout.data_ptr(), dout.stride(0), dout.stride(1),
+                                             lse.data_ptr(), o.data_ptr(), ws.data_ptr(), _addr(dq), _addr(dk), _addr(dv), _addr(ds),
+                                             _stream(dev)))
+        return dq if need_q else None, dk if need_k else None, dv if need_v else None, ds, None, None, None, None, None
+
+
+def scene_attn_step(q, k, v, k_len, q_ptr, max_rows, slopes, pos, k_pos, scale, softcap):
+    """dagnet_op_attn_step: k, v [S, room, KV, D]; q_ptr, k_len int32 device tensors."""
+    S, room = k.shape[:2]
+    out = torch.empty(q.shape, dtype=q.dtype, device=q.device)
+    a = _attn_struct(q, k, v, slopes, pos, k_pos, 0, scale, softcap)
+    with _on(q.device):
+        n = _lib().dagnet_op_attn_step_workspace(C.byref(a), S, room, max_rows)
+        ws = torch.empty(n, dtype=torch.float32, device=q.device) if n else None
+        _check(_lib().dagnet_op_attn_step(C.byref(a), q_ptr, k_len.data_ptr(), S, room, max_rows, k.stride(0), v.stride(0), out.data_ptr(),
+                                          _addr(ws), _stream(q.device)))
+    return out
+
+
+_POS_TYPES = {torch.float32: 0, torch.int32: 1, torch.int64: 2}
+
+
+def rotary_apply(q, k, pos, tables, pairs, interleaved, inverse, qo, ko):
+    """dagnet_op_rotary: writes qo (and ko); k and ko may be None."""
+    hk = 0 if k is None else k.shape[1]
+    ks, kos = (k.stride(), ko.stride()) if hk else ((0, 0), (0, 0))
+    qs, qos = q.stride(), qo.stride()
+    with _on(q.device):
+        _check(_lib().dagnet_op_rotary(q.shape[0], q.shape[1], hk, q.shape[2], int(q.dtype == torch.bfloat16), q.data_ptr(), qs[0], qs[1],
+                                       _addr(k), ks[0], ks[1], pos.data_ptr(), _POS_TYPES[pos.dtype], pos.shape[1], tables[0], tables[1], pairs,
+                                       int(interleaved), int(inverse), qo.data_ptr(), qos[0], qos[1], _addr(ko), kos[0], kos[1],
+                                       _stream(q.device)))
+
+
+class RotaryFn(torch.autograd.Function):
+    """(q, k or None) turned by their positions; the gradient is the same turn backwards."""
+
+    @staticmethod
+    def forward(ctx, q, k, pos, tables, pairs, interleaved):
+        qo = torch.empty(q.shape, dtype=q.dtype, device=q.device)
+        ko = None if k is None else torch.empty(k.shape, dtype=k.dtype, device=k.device)
+        rotary_apply(q, k, pos, tables, pairs, interleaved, False, qo, ko)
+        ctx.save_for_backward(pos)
+        ctx.meta = (tables, pairs, interleaved, k is not None)
+        return qo, ko
+
+    @staticmethod
+    @torch.autograd.function.once_differentiable
+    def backward(ctx, gq, gk):
+        pos, = ctx.saved_tensors
+        tables, pairs, interleaved, has_k = ctx.meta
+        gq = _heads(gq)
+        gk = _heads(gk) if has_k else None
+        dq = torch.empty(gq.shape, dtype=gq.dtype, device=gq.device)
+        dk = torch.empty(gk.shape, dtype=gk.dtype, device=gk.device) if has_k else None
+        rotary_apply(gq, gk, pos, tables, pairs, interleaved, True, dq, dk)
+        return dq, dk, None, None, None, None

@@ -19,6 +19,8 @@
 #include "params.h"
 #include "params_v2.h"
 #include "params_wide.h"
+#include "rotary.h"
+#include "scene_attn_step.h"
 
 extern "C" hipError_t dn_launch_rollout(int mode, const void *d_static, const DnRun *run, size_t lds_bytes, hipStream_t stream);
 extern "C" hipError_t dn_launch_adjacency(int type, double sigma, int top_k, const int32_t *scene_ptr, const int32_t *row_scene,
@@ -2154,5 +2156,137 @@ extern "C" int dagnet_op_adam(int64_t n, float *p, float *g, float *m, float *v,
     OP_NEED(n >= 0 && step >= 1 && (n == 0 || (p && g && m && v)) && (clip <= 0.f || sumsq), "bad argument");
     const float bc1 = (float)(1.0 - pow((double)beta1, (double)step)), bc2 = (float)(1.0 - pow((double)beta2, (double)step));
     HIP_TRY(dn_t_adam(n, p, g, m, v, sumsq, clip, lr, beta1, beta2, eps, bc1, bc2, OP_ST));
+    return DAGNET_OK;
+}
+
+// ---------------------------------------------------------------------------------------------
+// attention over the rows of a scene, rotary positions (scene_attn*.hip, rotary.hip)
+// ---------------------------------------------------------------------------------------------
+extern "C" hipError_t dn_scene_attn_fwd(const SceneAttnArgs *, int, hipStream_t);
+extern "C" hipError_t dn_scene_attn_bwd(const SceneAttnArgs *, int, float *, hipStream_t);
+extern "C" hipError_t dn_scene_attn_step(const SceneStepArgs *, int, hipStream_t);
+extern "C" int dn_scene_attn_step_splits(int64_t groups, int room);
+extern "C" hipError_t dn_rotary(const RotaryArgs *, int, int, hipStream_t);
+
+// bytes per load that a matrix of rows allows
+static int attn_vec(const void *p, int64_t rs, int64_t hs, int D, int size) {
+    for (int b = 16; b > size && b >= 8; b /= 2)
+        if (reinterpret_cast<uintptr_t>(p) % b == 0 && rs * size % b == 0 && hs * size % b == 0 && (int64_t)D * size % b == 0) return b;
+    return size;
+}
+
+static int attn_args(const dagnet_attn *a, SceneAttnArgs *A) {
+    OP_NEED(a, "null argument");
+    OP_NEED(a->dtype == 0 || a->dtype == 1, "dtype must be 0 (fp32) or 1 (bf16)");
+    OP_NEED(a->head_dim >= 1 && a->head_dim <= 128, "head_dim must be 1 .. 128");
+    OP_NEED(a->n_kv_heads >= 1 && a->n_heads >= 1 && a->n_heads % a->n_kv_heads == 0, "n_heads must be a multiple of n_kv_heads");
+    OP_NEED(a->nq >= 0 && a->nk >= 0 && a->nq <= 0x7fff0000 && a->nk <= 0x7fff0000, "row counts must be 0 .. 2^31 - 65536");
+    OP_NEED(a->axes >= 0 && a->axes <= 3, "axes must be 0 .. 3");
+    OP_NEED(a->softcap >= 0.f && a->softcap < INFINITY && a->scale == a->scale && fabsf(a->scale) < INFINITY, "scale and softcap must be finite, softcap not negative");
+    OP_NEED(a->nq == 0 || a->q, "null q");
+    OP_NEED(a->nq == 0 || !a->axes || (a->slopes && a->q_pos), "axes > 0 needs slopes and positions");
+    *A = SceneAttnArgs{};
+    A->q = a->q; A->k = a->k; A->v = a->v;
+    A->slopes = a->slopes; A->qpos = a->q_pos; A->kpos = a->k_pos;
+    A->q_rs = a->q_row; A->q_hs = a->q_head; A->k_rs = a->k_row; A->k_hs = a->k_head; A->v_rs = a->v_row; A->v_hs = a->v_head;
+    A->nq = a->nq; A->nk = a->nk; A->H = a->n_heads; A->KV = a->n_kv_heads; A->G = a->n_heads / a->n_kv_heads; A->D = a->head_dim;
+    A->axes = a->axes; A->scale = a->scale; A->cap = a->softcap;
+    const int size = a->dtype ? 2 : 4;
+    A->q_vec = attn_vec(a->q, a->q_row, a->q_head, a->head_dim, size);
+    A->k_vec = attn_vec(a->k, a->k_row, a->k_head, a->head_dim, size);
+    A->v_vec = attn_vec(a->v, a->v_row, a->v_head, a->head_dim, size);
+    A->o_vec = a->head_dim % 4 == 0;
+    const int64_t tiles = ((int64_t)a->nq * A->G + 63) / 64;
+    OP_NEED(tiles * A->KV <= 0x7fffffffLL && ((int64_t)a->nk + 63) / 64 * A->KV <= 0x7fffffffLL && ((int64_t)a->nq * A->H + 3) / 4 <= 0x7fffffffLL,
+            "too many rows for one launch");
+    return DAGNET_OK;
+}
+// 4 values at once need a base of that alignment
+static bool attn_base(const void *p, int size) { return reinterpret_cast<uintptr_t>(p) % (4 * size) == 0; }
+
+extern "C" int dagnet_op_attn_fwd(const dagnet_attn *a, const int32_t *row_lo, const int32_t *row_hi, void *out, float *lse, float *o32,
+                                  void *stream) {
+    SceneAttnArgs A;
+    if (int rc = attn_args(a, &A)) return rc;
+    if (a->nq == 0) return DAGNET_OK;
+    OP_NEED(row_lo && row_hi && out && (a->nk == 0 || (a->k && a->v && (!a->axes || a->k_pos))), "null argument");
+    A.row_lo = row_lo; A.row_hi = row_hi; A.out = out; A.lse = lse; A.o32 = o32;
+    if (!attn_base(out, a->dtype ? 2 : 4) || !attn_base(o32, 4)) A.o_vec = 0;
+    HIP_TRY(dn_scene_attn_fwd(&A, a->dtype, OP_ST));
+    return DAGNET_OK;
+}
+
+extern "C" int64_t dagnet_op_attn_bwd_workspace(const dagnet_attn *a) { return a ? 2 * (int64_t)a->nq * a->n_heads : 0; }
+
+extern "C" int dagnet_op_attn_bwd(const dagnet_attn *a, const int32_t *row_lo, const int32_t *row_hi, const int32_t *key_lo,
+                                  const int32_t *key_hi, const void *dout, int64_t do_row, int64_t do_head, const float *lse, const float *o,
+                                  float *workspace, void *dq, void *dk, void *dv, float *dslopes, void *stream) {
+    SceneAttnArgs A;
+    if (int rc = attn_args(a, &A)) return rc;
+    OP_NEED((dk == nullptr) == (dv == nullptr), "dk and dv go together");
+    OP_NEED(!dslopes || (dq && a->axes), "dslopes needs dq and a distance term");
+    const int size = a->dtype ? 2 : 4;
+    OP_NEED(a->nq == 0 || (row_lo && row_hi && dout && lse && o && workspace), "null argument");
+    OP_NEED(a->nk == 0 || (a->k && a->v && (!dk || (key_lo && key_hi)) && (!a->axes || a->k_pos)), "null argument");
+    A.row_lo = row_lo; A.row_hi = row_hi; A.key_lo = key_lo; A.key_hi = key_hi;
+    A.dout = dout; A.do_rs = do_row; A.do_hs = do_head; A.do_vec = attn_vec(dout, do_row, do_head, a->head_dim, size);
+    A.lse = const_cast<float *>(lse); A.o32 = const_cast<float *>(o);
+    A.delta = workspace; A.dsl = dslopes ? workspace + (int64_t)a->nq * a->n_heads : nullptr;
+    A.dq = dq; A.dk = dk; A.dv = dv;
+    if (!attn_base(dq, size) || !attn_base(dk, size) || !attn_base(dv, size)) A.o_vec = 0;
+    HIP_TRY(dn_scene_attn_bwd(&A, a->dtype, dslopes, OP_ST));
+    return DAGNET_OK;
+}
+
+static int step_shape(const dagnet_attn *a, int32_t scenes, int32_t room, int32_t max_rows, int *cblocks, int *splits) {
+    *cblocks = (int)(((int64_t)max_rows * (a->n_heads / a->n_kv_heads) + 15) / 16);
+    *splits = dn_scene_attn_step_splits((int64_t)scenes * a->n_kv_heads * (*cblocks), room);
+    return DAGNET_OK;
+}
+
+extern "C" int64_t dagnet_op_attn_step_workspace(const dagnet_attn *a, int32_t scenes, int32_t room, int32_t max_rows) {
+    if (!a || scenes < 1 || room < 1 || max_rows < 1 || a->n_kv_heads < 1 || a->n_heads < a->n_kv_heads) return 0;
+    int cb, sp;
+    step_shape(a, scenes, room, max_rows, &cb, &sp);
+    return sp == 1 ? 0 : (int64_t)a->nq * a->n_heads * sp * (a->head_dim + 2);
+}
+
+extern "C" int dagnet_op_attn_step(const dagnet_attn *a, const int32_t *q_ptr, const int32_t *k_len, int32_t scenes, int32_t room,
+                                   int32_t max_rows, int64_t k_scene, int64_t v_scene, void *out, float *workspace, void *stream) {
+    SceneStepArgs A;
+    if (int rc = attn_args(a, &A.a)) return rc;
+    OP_NEED(scenes >= 0 && room >= 0 && room <= 0x7fff0000 && max_rows >= 0, "bad argument");
+    if (a->nq == 0 || scenes == 0) return DAGNET_OK;
+    OP_NEED(max_rows >= 1 && q_ptr && k_len && out && (room == 0 || (a->k && a->v && (!a->axes || a->k_pos))), "bad argument");
+    A.q_ptr = q_ptr; A.k_len = k_len; A.scenes = scenes; A.room = room; A.k_ss = k_scene; A.v_ss = v_scene;
+    step_shape(a, scenes, room, max_rows, &A.cblocks, &A.splits);
+    OP_NEED((int64_t)scenes * a->n_kv_heads * A.cblocks * A.splits <= 0x7fffffffLL, "too many rows for one launch");
+    OP_NEED(A.splits == 1 || workspace, "workspace is NULL");
+    const int size = a->dtype ? 2 : 4;
+    A.a.out = out;
+    A.a.k_vec = std::min(A.a.k_vec, attn_vec(a->k, k_scene, a->k_head, a->head_dim, size));
+    A.a.v_vec = std::min(A.a.v_vec, attn_vec(a->v, v_scene, a->v_head, a->head_dim, size));
+    if (!attn_base(out, size)) A.a.o_vec = 0;
+    A.part = workspace;
+    A.stat = workspace ? workspace + (int64_t)a->nq * a->n_heads * A.splits * a->head_dim : nullptr;
+    HIP_TRY(dn_scene_attn_step(&A, a->dtype, OP_ST));
+    return DAGNET_OK;
+}
+
+extern "C" int dagnet_op_rotary(int64_t n, int32_t hq, int32_t hk, int32_t head_dim, int32_t dtype, const void *q, int64_t q_row, int64_t q_head,
+                                const void *k, int64_t k_row, int64_t k_head, const void *pos, int32_t pos_type, int32_t axes,
+                                const double *turns, const int32_t *axis, int32_t pairs, int32_t interleaved, int32_t inverse, void *qo,
+                                int64_t qo_row, int64_t qo_head, void *ko, int64_t ko_row, int64_t ko_head, void *stream) {
+    OP_NEED(n >= 0 && hq >= 1 && hk >= 0 && (int64_t)hq + hk <= 65536 && head_dim >= 2 && head_dim <= 1024, "bad shape");
+    OP_NEED(dtype == 0 || dtype == 1, "dtype must be 0 (fp32) or 1 (bf16)");
+    OP_NEED(pos_type >= 0 && pos_type <= 2 && axes >= 1, "bad positions");
+    OP_NEED(pairs >= 1 && 2 * pairs <= head_dim, "pairs must be 1 .. head_dim / 2");
+    if (n == 0) return DAGNET_OK;
+    OP_NEED(q && qo && (hk == 0 || (k && ko)) && pos && turns && axis, "null argument");
+    RotaryArgs A = {};
+    A.q = q; A.k = k; A.pos = pos; A.qo = qo; A.ko = ko; A.turns = turns; A.axis = axis;
+    A.n = n; A.q_rs = q_row; A.q_hs = q_head; A.k_rs = k_row; A.k_hs = k_head; A.qo_rs = qo_row; A.qo_hs = qo_head; A.ko_rs = ko_row; A.ko_hs = ko_head;
+    A.hq = hq; A.hk = hk; A.D = head_dim; A.pairs = pairs; A.axes = axes; A.interleaved = interleaved != 0; A.sign = inverse ? -1.f : 1.f;
+    HIP_TRY(dn_rotary(&A, dtype, pos_type, OP_ST));
     return DAGNET_OK;
 }

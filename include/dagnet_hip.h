@@ -401,6 +401,49 @@ int dagnet_op_sumsq(int64_t n, const float *g, double *acc, void *stream);
 int dagnet_op_adam(int64_t n, float *p, float *g, float *m, float *v, const double *sumsq, float clip, float lr, float beta1,
                    float beta2, float eps, int32_t step, void *stream);
 
+/* ---- attention over the rows of a scene, and rotary positions ---------------------------------------------------------------
+ * No counterpart in the reference (its graph layers are the additive attention of gat_layers.py:25-40 and gcn_layers.py:20-26): dot-product
+ * attention over the rows of a scene - its agents, or its agents by time steps - for models that replace or follow those layers.
+ *
+ * x_ij = cap tanh(scale q_i.k_j / cap) - slope_h |q_pos_i - k_pos_j|,  o_i = sum_j softmax_j(x_ij) v_j over row_lo[i] <= j < row_hi[i].
+ * softcap 0: no cap; axes 0: no distance term (slopes, q_pos, k_pos unused), else 1 - 3 coordinates.  Query head h reads kv head
+ * h / (n_heads / n_kv_heads).  A row that sees nothing gives 0 and has no gradient; what stands in keys that a row does not see never
+ * reaches it, infinities and NaN included.  dtype: 0 fp32, 1 bf16 (q, k, v, out and their gradients; everything else fp32); statistics
+ * and sums are fp32.  head_dim 1 - 128.  Strides are in elements, columns have stride 1; out, dq, dk, dv are contiguous. */
+typedef struct {
+    const void *q, *k, *v;               /* [nq][n_heads][head_dim], [nk][n_kv_heads][head_dim] twice */
+    const float *slopes, *q_pos, *k_pos; /* [n_heads], [nq][axes], [nk][axes] */
+    int64_t q_row, q_head, k_row, k_head, v_row, v_head;
+    int32_t nq, nk, n_heads, n_kv_heads, head_dim, axes, dtype;
+    float scale, softcap;
+} dagnet_attn;
+/* row_lo, row_hi [nq]: int32, neither decreasing.  For a later backward pass (NULL: none wanted): lse [nq * n_heads] receives the rows'
+ * statistics, o32 [nq][n_heads][head_dim] the unrounded output (bf16 only; fp32 passes NULL and keeps out). */
+int dagnet_op_attn_fwd(const dagnet_attn *a, const int32_t *row_lo, const int32_t *row_hi, void *out, float *lse, float *o32, void *stream);
+/* key_lo, key_hi [nk]: the rows that see a key lie in key_lo[j] <= i < key_hi[j], neither decreasing.  o: o32, or out for fp32.
+ * dq (with dslopes) or dk and dv may be NULL: not wanted; dslopes [n_heads] is NULL or has axes > 0.  Deterministic: no atomics.
+ * workspace: dagnet_op_attn_bwd_workspace(a) floats. */
+int64_t dagnet_op_attn_bwd_workspace(const dagnet_attn *a);
+int dagnet_op_attn_bwd(const dagnet_attn *a, const int32_t *row_lo, const int32_t *row_hi, const int32_t *key_lo, const int32_t *key_hi,
+                       const void *dout, int64_t do_row, int64_t do_head, const float *lse, const float *o, float *workspace, void *dq,
+                       void *dk, void *dv, float *dslopes, void *stream);
+/* The same attention for the new rows of a step over kept keys: scene s has the query rows q_ptr[s] .. q_ptr[s + 1] - 1 (at most max_rows
+ * of them), which all see the first k_len[s] of its `room` cache rows (k_len is clamped to 0 .. room).  k, v: [scenes][room][n_kv_heads]
+ * [head_dim], k_scene / v_scene elements between scenes; k_pos [scenes][room][axes] contiguous; nk of `a` is not read.  q_ptr and
+ * k_len are DEVICE arrays, so a captured call follows a growing cache.  workspace: dagnet_op_attn_step_workspace() floats (0: may be
+ * NULL), private to the call until it has run. */
+int64_t dagnet_op_attn_step_workspace(const dagnet_attn *a, int32_t scenes, int32_t room, int32_t max_rows);
+int dagnet_op_attn_step(const dagnet_attn *a, const int32_t *q_ptr, const int32_t *k_len, int32_t scenes, int32_t room, int32_t max_rows,
+                        int64_t k_scene, int64_t v_scene, void *out, float *workspace, void *stream);
+/* Rotary positions with several axes: pair i of every head of q [n][hq][head_dim] and k [n][hk][head_dim] (hk 0: q alone) is turned by
+ * pos[row][axis[i]] * turns[i] full turns (computed in fp64), backwards with inverse != 0 (which is also its gradient).  turns [pairs] fp64,
+ * axis [pairs] int32 in 0 .. axes - 1.  interleaved: pair i = columns 2 i, 2 i + 1, else i, pairs + i; columns from 2 * pairs on pass
+ * through.  pos [n][axes] contiguous, pos_type 0 fp32, 1 int32, 2 int64.  dtype as above.  qo / ko may be q / k with their strides. */
+int dagnet_op_rotary(int64_t n, int32_t hq, int32_t hk, int32_t head_dim, int32_t dtype, const void *q, int64_t q_row, int64_t q_head,
+                     const void *k, int64_t k_row, int64_t k_head, const void *pos, int32_t pos_type, int32_t axes, const double *turns,
+                     const int32_t *axis, int32_t pairs, int32_t interleaved, int32_t inverse, void *qo, int64_t qo_row, int64_t qo_head,
+                     void *ko, int64_t ko_row, int64_t ko_head, void *stream);
+
 #ifdef __cplusplus
 }
 #endif
