@@ -2162,8 +2162,11 @@ extern "C" int dagnet_op_adam(int64_t n, float *p, float *g, float *m, float *v,
 // ---------------------------------------------------------------------------------------------
 // attention over the rows of a scene, rotary positions (scene_attn*.hip, rotary.hip)
 // ---------------------------------------------------------------------------------------------
-extern "C" hipError_t dn_scene_attn_fwd(const SceneAttnArgs *, int, hipStream_t);
-extern "C" hipError_t dn_scene_attn_bwd(const SceneAttnArgs *, int, float *, hipStream_t);
+extern "C" hipError_t dn_scene_attn_fwd_f32(const SceneAttnArgs *, hipStream_t);
+extern "C" hipError_t dn_scene_attn_fwd_bf16(const SceneAttnArgs *, hipStream_t);
+extern "C" hipError_t dn_scene_attn_bwd_f32(const SceneAttnArgs *, float *, hipStream_t);
+extern "C" hipError_t dn_scene_attn_bwd_bf16(const SceneAttnArgs *, float *, hipStream_t);
+extern "C" int dn_scene_attn_bwd_parts(int64_t, int64_t, int, int);
 extern "C" hipError_t dn_scene_attn_step(const SceneStepArgs *, int, hipStream_t);
 extern "C" int dn_scene_attn_step_splits(int64_t groups, int room);
 extern "C" hipError_t dn_rotary(const RotaryArgs *, int, int, hipStream_t);
@@ -2212,11 +2215,16 @@ extern "C" int dagnet_op_attn_fwd(const dagnet_attn *a, const int32_t *row_lo, c
     OP_NEED(row_lo && row_hi && out && (a->nk == 0 || (a->k && a->v && (!a->axes || a->k_pos))), "null argument");
     A.row_lo = row_lo; A.row_hi = row_hi; A.out = out; A.lse = lse; A.o32 = o32;
     if (!attn_base(out, a->dtype ? 2 : 4) || !attn_base(o32, 4)) A.o_vec = 0;
-    HIP_TRY(dn_scene_attn_fwd(&A, a->dtype, OP_ST));
+    HIP_TRY(a->dtype ? dn_scene_attn_fwd_bf16(&A, OP_ST) : dn_scene_attn_fwd_f32(&A, OP_ST));
     return DAGNET_OK;
 }
 
-extern "C" int64_t dagnet_op_attn_bwd_workspace(const dagnet_attn *a) { return a ? 2 * (int64_t)a->nq * a->n_heads : 0; }
+static int attn_parts(const dagnet_attn *a) { return dn_scene_attn_bwd_parts(a->nq, a->nk, a->n_kv_heads, a->n_heads / a->n_kv_heads); }
+extern "C" int64_t dagnet_op_attn_bwd_workspace(const dagnet_attn *a) {
+    if (!a || a->nq < 0 || a->nk < 0 || a->n_kv_heads < 1 || a->n_heads < a->n_kv_heads || a->head_dim < 1) return 0;
+    const int parts = attn_parts(a);
+    return 2 * (int64_t)a->nq * a->n_heads + 3 + (parts > 1 ? 2 * (int64_t)parts * a->nk * a->n_kv_heads * a->head_dim : 0);
+}
 
 extern "C" int dagnet_op_attn_bwd(const dagnet_attn *a, const int32_t *row_lo, const int32_t *row_hi, const int32_t *key_lo,
                                   const int32_t *key_hi, const void *dout, int64_t do_row, int64_t do_head, const float *lse, const float *o,
@@ -2233,8 +2241,13 @@ extern "C" int dagnet_op_attn_bwd(const dagnet_attn *a, const int32_t *row_lo, c
     A.lse = const_cast<float *>(lse); A.o32 = const_cast<float *>(o);
     A.delta = workspace; A.dsl = dslopes ? workspace + (int64_t)a->nq * a->n_heads : nullptr;
     A.dq = dq; A.dk = dk; A.dv = dv;
+    A.parts = attn_parts(a);
+    OP_NEED(((int64_t)a->nk + 63) / 64 * A.KV * A.parts <= 0x7fffffffLL && ((int64_t)a->nk * A.KV + 3) / 4 <= 0x7fffffffLL, "too many keys for one launch");
+    // behind delta and dsl, at a multiple of 16 bytes of the workspace
+    if (A.parts > 1) A.part = workspace + (2 * (int64_t)a->nq * a->n_heads + 3) / 4 * 4;
     if (!attn_base(dq, size) || !attn_base(dk, size) || !attn_base(dv, size)) A.o_vec = 0;
-    HIP_TRY(dn_scene_attn_bwd(&A, a->dtype, dslopes, OP_ST));
+    OP_NEED(A.parts == 1 || attn_base(workspace, 4), "workspace must be 16-byte aligned");
+    HIP_TRY(a->dtype ? dn_scene_attn_bwd_bf16(&A, dslopes, OP_ST) : dn_scene_attn_bwd_f32(&A, dslopes, OP_ST));
     return DAGNET_OK;
 }
 

@@ -28,6 +28,8 @@ struct SceneAttnArgs {
     int64_t q_rs, q_hs, k_rs, k_hs, v_rs, v_hs, do_rs, do_hs;      // element strides of rows and heads (out, dq, dk, dv: contiguous)
     int32_t nq, nk, H, KV, G, D, axes;
     float scale, cap;
+    int32_t parts;                             // of the rows in the dk / dv kernel; part: [parts][dk, dv][nk][KV][D]
+    float *part;
     int32_t q_vec, k_vec, v_vec, do_vec, o_vec;     // bytes per load that strides, base and width allow: 16, 8 or the element
 };
 
@@ -67,14 +69,6 @@ __device__ __forceinline__ float exp2_(float x) { return __builtin_amdgcn_exp2f(
 __device__ __forceinline__ float log2_(float x) { return __builtin_amdgcn_logf(x); }
 __device__ __forceinline__ float rcp_(float x) { return __builtin_amdgcn_rcpf(x); }
 
-// Rows of a tile in LDS: NCH chunks each, chunk c of row r at slot c ^ swz(r), so that 16 lanes reading one chunk column of 16 rows
-// spread over the banks (rows of less than 128 bytes share a bank line: those rows keep one swizzle).
-template <typename T, int DP> struct Tile {
-    static constexpr int NCH = DP / Tr<T>::CH;
-    static __device__ __forceinline__ int swz(int r) { return NCH >= 8 ? (r & 7) : ((r / (8 / NCH)) & (NCH - 1)); }
-    static __device__ __forceinline__ int slot(int r, int c) { return r * NCH + (c ^ swz(r)); }
-};
-
 // elements [d, d + CH) of a row of D elements; zeros behind D.  vec: bytes per load (16: the whole chunk, then D % CH == 0)
 template <typename T> __device__ __forceinline__ u32x4 load_chunk(const T *p, int d, int D, int vec) {
     u32x4 r = {0u, 0u, 0u, 0u};
@@ -103,6 +97,45 @@ template <typename T> __device__ __forceinline__ typename Tr<T>::frag as_frag(u3
     x.v = v;
     return x.f;
 }
+
+// Rows of a tile in LDS: NCH chunks each, chunk c of row r at slot c ^ swz(r), so that 16 lanes reading one chunk column of 16 rows
+// spread over the banks (rows of less than 128 bytes share a bank line: those rows keep one swizzle).
+template <typename T, int DP> struct Tile {
+    static constexpr int NCH = DP / Tr<T>::CH;
+    static __device__ __forceinline__ int swz(int r) { return NCH % 8 == 0 ? (r & 7) : NCH > 8 ? (r & 3) : ((r / (8 / NCH)) & (NCH - 1)); }
+    static __device__ __forceinline__ int slot(int r, int c) { return r * NCH + (c ^ swz(r)); }
+};
+
+// Fills a tile of ROWS rows with the rows row(r) points to (columns behind D: anything finite that the row holds - the other operand is 0
+// there, or the result is not stored).  vec 16: straight into LDS, 64 lanes x 16 bytes an instruction, the swizzle applied to the
+// source; nothing waits until landed().  Else through registers, done on return.
+template <typename T, int DP, int ROWS, int NT, typename Row> __device__ __forceinline__ void stage(u32x4 *tile, Row row, int D, int vec) {
+    using L = Tile<T, DP>;
+    constexpr int NC = ROWS * L::NCH, PER = (NC + NT - 1) / NT;
+    static_assert(NC % 64 == 0, "whole waves");
+    typedef __attribute__((address_space(3))) void *lp;
+    typedef const __attribute__((address_space(1))) void *gp;
+    const int lane = threadIdx.x & 63, w0 = __builtin_amdgcn_readfirstlane(threadIdx.x & ~63);
+    if (vec == 16) {
+        const int last = (D - 1) / Tr<T>::CH;
+#pragma unroll
+        for (int i = 0; i < PER; ++i) {
+            const int s0 = i * NT + w0;
+            if (NC % NT == 0 || s0 < NC) {
+                const int s = s0 + lane, r = s / L::NCH, c = (s % L::NCH) ^ L::swz(r);
+                __builtin_amdgcn_global_load_lds((gp)(row(r) + min(c, last) * Tr<T>::CH), (lp)(tile + s0), 16, 0, 0);
+            }
+        }
+    } else {
+#pragma unroll 1
+        for (int s = threadIdx.x; s < NC; s += NT) {
+            const int r = s / L::NCH, c = (s % L::NCH) ^ L::swz(r);
+            tile[s] = load_chunk<T>(row(r), c * Tr<T>::CH, D, vec);
+        }
+    }
+}
+// this wave's part of every stage() so far is in LDS (a barrier then says so of the workgroup's)
+__device__ __forceinline__ void landed() { __builtin_amdgcn_s_waitcnt(0x0f70); }      // vmcnt(0)
 
 // A operand of the first product: row r0 + c of a tile, columns kk KD + ..
 template <typename T, int DP> __device__ __forceinline__ typename Tr<T>::frag frag_rows(const u32x4 *t, int r0, int kk, int lane) {
@@ -140,6 +173,15 @@ __device__ __forceinline__ bf16x8 pack_p(const f32x4 *p, bf16) {
     for (int i = 0; i < 4; ++i) { r[i] = (bf16)p[0][i]; r[4 + i] = (bf16)p[1][i]; }
     return r;
 }
+
+// what that rounding left over, rounded in turn: p to 16 bits through two products
+__device__ __forceinline__ bf16x8 pack_rest(const f32x4 *p, bf16x8 hi) {
+    bf16x8 r;
+#pragma unroll
+    for (int i = 0; i < 4; ++i) { r[i] = (bf16)(p[0][i] - (float)hi[i]); r[4 + i] = (bf16)(p[1][i] - (float)hi[4 + i]); }
+    return r;
+}
+__device__ __forceinline__ f32x4 pack_rest(const f32x4 *, f32x4 hi) { return hi; }      // fp32 rounds nothing: never used
 
 // tanh to about 1 ulp of fp32: near zero the odd rational [7/6] from the continued fraction x / (1 + x^2 / (3 + x^2 / (5 + ...)))
 // (its next term is below 2^-27 for |x| <= 1), else 1 - 2 / (1 + e^2x), which loses nothing there.
@@ -200,11 +242,63 @@ __device__ __forceinline__ RowState row_state(const SceneAttnArgs &A, int kvh, i
     s.hi = min(A.row_hi[s.row], A.nk);
     s.slope = A.axes ? A.slopes[s.head] * LOG2E : 0.f;
     s.pos[0] = s.pos[1] = s.pos[2] = 0.f;
-    for (int a = 0; a < A.axes; ++a) s.pos[a] = A.qpos[(int64_t)s.row * A.axes + a];
+    const float *p = A.qpos + (int64_t)s.row * A.axes;
+    if (A.axes > 0) s.pos[0] = p[0];
+    if (A.axes > 1) s.pos[1] = p[1];
+    if (A.axes > 2) s.pos[2] = p[2];
     return s;
 }
 
-// One score in base 2 from the raw product: capped and biased.
+__device__ __forceinline__ int uniform(int v) { return __builtin_amdgcn_readfirstlane(v); }
+
+// Coordinate a of a tile's keys, loaded by the first lanes; missing axes are 0.
+template <int AX, int N> struct KeyPos {
+    float r[AX ? AX : 1];
+    __device__ __forceinline__ void fetch(const SceneAttnArgs &A, const float *kpos, int key) {
+        if constexpr (AX > 0)
+            if (threadIdx.x < N) {
+#pragma unroll
+                for (int a = 0; a < AX; ++a) r[a] = a < A.axes ? kpos[(int64_t)key * A.axes + a] : 0.f;
+            }
+    }
+    __device__ __forceinline__ void put(float (*s)[N]) const {
+        if constexpr (AX > 0)
+            if (threadIdx.x < N) {
+#pragma unroll
+                for (int a = 0; a < AX; ++a) s[a][threadIdx.x] = r[a];
+            }
+    }
+};
+
+// Scores in base 2 from raw products, the constants of one launch folded together.  CAP and AX (0, 1, or 3 for two and three
+// coordinates) are compiled in: the kernels are bound by vector instructions per score, not by the products.
+//   cap: t = tanh(raw scale / cap) = 1 - 2 r with r = 1 / (1 + e^2z); x = cap t.  In fp32 near zero through tanh_() (1 - 2 r is off by 2^-24 there
+//   whatever t is); for bf16 that is far below what the operands' type can tell.
+template <typename T, bool CAP, int AX> struct Score {
+    float k, cap2, arg;
+    __device__ __forceinline__ Score(const SceneAttnArgs &A) {
+        k = A.scale * LOG2E;
+        cap2 = A.cap * LOG2E;
+        arg = CAP ? (sizeof(T) == 4 ? A.scale / A.cap : 2.f * LOG2E * A.scale / A.cap) : 0.f;
+    }
+    // x in base 2; t: the tanh (for its derivative)
+    __device__ __forceinline__ float value(float raw, float &t) const {
+        if constexpr (!CAP) return raw * k;
+        else {
+            if constexpr (sizeof(T) == 4) t = tanh_(raw * arg);
+            else t = 1.f - 2.f * rcp_(1.f + exp2_(raw * arg));
+            return cap2 * t;
+        }
+    }
+    static __device__ __forceinline__ float dist(const float *a, float bx, float by, float bz) {
+        const float x = a[0] - bx;
+        if constexpr (AX == 1) return fabsf(x);
+        const float y = a[1] - by, z = a[2] - bz;
+        return __builtin_amdgcn_sqrtf(x * x + y * y + z * z);
+    }
+};
+
+// the same with everything read at run time (the slow forms and the step kernel's launch-time choices)
 __device__ __forceinline__ float score2(const SceneAttnArgs &A, float raw, float inv_cap, float slope2, const float *qpos, const float *kpos) {
     float x = raw * A.scale;
     if (A.cap > 0.f) x = A.cap * tanh_(x * inv_cap);

@@ -33,7 +33,7 @@ template <typename T> __global__ __launch_bounds__(256) void scene_attn_delta_ke
 }
 
 // dslopes[h] = sum over the rows of what the dq kernel left per packed row; one workgroup per head, fp64, fixed order
-__global__ __launch_bounds__(256) void scene_attn_dslope_kernel(int nq, int G, const float *__restrict__ part, float *__restrict__ out) {
+static __global__ __launch_bounds__(256) void scene_attn_dslope_kernel(int nq, int G, const float *__restrict__ part, float *__restrict__ out) {
     __shared__ double sh[256];
     const int h = blockIdx.x, kvh = h / G, g = h - kvh * G;
     const float *p = part + (int64_t)kvh * nq * G + g;
@@ -73,14 +73,24 @@ __device__ __forceinline__ Grad pair_grad(const SceneAttnArgs &A, float raw, flo
 
 // a row's part of dslope: sums of ds, ds dist and p dist, the delta's error taken back (above)
 struct Slope {
-    float ds = 0.f, dsd = 0.f, pd = 0.f;
-    __device__ __forceinline__ void add(const Grad &g, bool seen) {
-        const float d = seen ? g.ds : 0.f, p = seen ? g.p : 0.f;
-        ds += d;
-        dsd += d * g.dist;
-        pd += p * g.dist;
+    double ds = 0.0, dsd = 0.0, pd = 0.0;
+    __device__ __forceinline__ void add(const Grad &g) {
+        ds += g.ds;
+        dsd += g.ds * g.dist;
+        pd += g.p * g.dist;
     }
-    __device__ __forceinline__ float row() const { return ds * pd - dsd; }
+    __device__ __forceinline__ void add(f32x4 p, f32x4 d, f32x4 dist) {          // four scores in fp32, then fp64: long rows lose nothing
+        ds += (d[0] + d[1]) + (d[2] + d[3]);
+        dsd += (d[0] * dist[0] + d[1] * dist[1]) + (d[2] * dist[2] + d[3] * dist[3]);
+        pd += (p[0] * dist[0] + p[1] * dist[1]) + (p[2] * dist[2] + p[3] * dist[3]);
+    }
+    __device__ __forceinline__ float row() const { return (float)(ds * pd - dsd); }
+    __device__ __forceinline__ float row_of_groups() {                            // the four lane groups of a row together
+        ds += __shfl_xor(ds, 16);   ds += __shfl_xor(ds, 32);
+        dsd += __shfl_xor(dsd, 16); dsd += __shfl_xor(dsd, 32);
+        pd += __shfl_xor(pd, 16);   pd += __shfl_xor(pd, 32);
+        return row();
+    }
 };
 
 __device__ __forceinline__ float dot_rows(float a0, float a1, float b0, float b1, bool h0, bool h1) {
@@ -106,7 +116,7 @@ template <typename T> __device__ void dq_slow(const SceneAttnArgs &A, int kvh, c
         const Grad e = pair_grad(A, raw, dp, inv_cap, s.slope, s.pos, A.kpos + j * A.axes, lse, delta);
         a0 += e.dz * k0;
         a1 += e.dz * k1;
-        sl.add(e, true);
+        sl.add(e);
     }
     T *out = reinterpret_cast<T *>(A.dq) + ((int64_t)s.row * A.H + s.head) * A.D;
     if (h0) out[lane] = (T)(a0 * A.scale);
@@ -143,259 +153,414 @@ template <typename T> __device__ void dkv_slow(const SceneAttnArgs &A, int kvh, 
 }
 
 // ---------------------------------------------------------------------------------------------------------------------
-// dq and dslope: 64 packed rows a workgroup, 16 a wave (columns); K and V tiles in LDS
+// dq and dslope: 64 MB packed rows a workgroup, 16 MB a wave (columns); K and V tiles in LDS
 // ---------------------------------------------------------------------------------------------------------------------
-template <typename T, int DP, int BN>
+template <typename T, int DP, int BN, int MB, bool CAP, int AX>
 __global__ __launch_bounds__(256) void scene_attn_dq_kernel(const SceneAttnArgs A) {
     using X = Tr<T>;
     using L = Tile<T, DP>;
-    constexpr int NF = DP / X::KD, DB = DP / 16, PB = X::KB / 16, NC = BN * L::NCH, PER = NC / 256;
-    static_assert(NC % 256 == 0 && BN % X::KB == 0, "tile");
-    __shared__ u32x4 sk[NC], sv[NC];
+    constexpr int NF = DP / X::KD, DB = DP / 16, PB = X::KB / 16, NC = BN * L::NCH, ROWS = 64 * MB;
+    static_assert(BN % X::KB == 0, "tile");
+    __shared__ u32x4 sk[2][NC], sv[2][NC];
+    __shared__ __attribute__((aligned(16))) float sp[2][AX ? AX : 1][BN];
     const int tid = threadIdx.x, lane = tid & 63, w = tid >> 6, g = lane >> 4, c = lane & 15;
     const int kvh = (int)(blockIdx.x % A.KV);
-    const int64_t R = (int64_t)A.nq * A.G, r0 = (int64_t)(gridDim.x / A.KV - 1 - blockIdx.x / A.KV) * 64, r = r0 + w * 16 + c;
-    const RowState s = row_state(A, kvh, r, R);
-    const float lse = A.lse[kvh * R + min(r, R - 1)], delta = A.delta[kvh * R + min(r, R - 1)];
-    const T *Q = reinterpret_cast<const T *>(A.q) + s.row * A.q_rs + s.head * A.q_hs;
-    const T *G = reinterpret_cast<const T *>(A.dout) + s.row * A.do_rs + s.head * A.do_hs;
-    typename X::frag qf[NF], gf[NF];
+    const int64_t R = (int64_t)A.nq * A.G, r0 = (int64_t)(gridDim.x / A.KV - 1 - blockIdx.x / A.KV) * ROWS;
+    const Score<T, CAP, AX> S(A);
+    RowState s[MB];
+    float lse[MB], delta[MB];
+    typename X::frag qf[MB][NF], gf[MB][NF];
 #pragma unroll
-    for (int f = 0; f < NF; ++f) {
-        qf[f] = as_frag<T>(load_chunk<T>(Q, f * X::KD + g * X::CH, A.D, A.q_vec));
-        gf[f] = as_frag<T>(load_chunk<T>(G, f * X::KD + g * X::CH, A.D, A.do_vec));
+    for (int b = 0; b < MB; ++b) {
+        const int64_t r = r0 + (w * MB + b) * 16 + c;
+        s[b] = row_state(A, kvh, r, R);
+        lse[b] = A.lse[kvh * R + min(r, R - 1)];
+        delta[b] = A.delta[kvh * R + min(r, R - 1)];
+        const T *Q = reinterpret_cast<const T *>(A.q) + s[b].row * A.q_rs + s[b].head * A.q_hs;
+        const T *G = reinterpret_cast<const T *>(A.dout) + s[b].row * A.do_rs + s[b].head * A.do_hs;
+#pragma unroll
+        for (int f = 0; f < NF; ++f) {
+            qf[b][f] = as_frag<T>(load_chunk<T>(Q, f * X::KD + g * X::CH, A.D, A.q_vec));
+            gf[b][f] = as_frag<T>(load_chunk<T>(G, f * X::KD + g * X::CH, A.D, A.do_vec));
+        }
     }
-    const int qa = (int)(r0 / A.G), qb = (int)((min(r0 + 64, R) - 1) / A.G);
-    const int tlo = max(A.row_lo[qa], 0), thi = min(A.row_hi[qb], A.nk);
-    const int wlo = __builtin_amdgcn_readfirstlane(__shfl(s.lo, 0)), whi = __builtin_amdgcn_readfirstlane(__shfl(s.hi, 15));
+    const int qa = (int)(r0 / A.G), qb = (int)((min(r0 + ROWS, R) - 1) / A.G);
+    const int tlo = uniform(max(A.row_lo[qa], 0)), thi = uniform(min(A.row_hi[qb], A.nk));
+    const int wlo = uniform(__shfl(s[0].lo, 0)), whi = uniform(__shfl(s[MB - 1].hi, 15));
+    int lo_last[MB], hi_first[MB];
+#pragma unroll
+    for (int b = 0; b < MB; ++b) {
+        lo_last[b] = uniform(__shfl(s[b].lo, 15));
+        hi_first[b] = uniform(__shfl(s[b].hi, 0));
+    }
     const T *K = reinterpret_cast<const T *>(A.k) + kvh * A.k_hs, *V = reinterpret_cast<const T *>(A.v) + kvh * A.v_hs;
-    const float inv_cap = A.cap > 0.f ? 1.f / A.cap : 0.f;
-
-    u32x4 rk[PER], rv[PER];
-    auto fetch = [&](int kb) {
-#pragma unroll
-        for (int i = 0; i < PER; ++i) {
-            const int e = tid + i * 256, key = kb + e / L::NCH, ch = e % L::NCH;
-            const u32x4 z = {0u, 0u, 0u, 0u};
-            const bool in = key < thi;
-            rk[i] = in ? load_chunk<T>(K + (int64_t)key * A.k_rs, ch * X::CH, A.D, A.k_vec) : z;
-            rv[i] = in ? load_chunk<T>(V + (int64_t)key * A.v_rs, ch * X::CH, A.D, A.v_vec) : z;
-        }
+    KeyPos<AX, BN> kp;
+    auto issue = [&](int kb, int buf) {
+        stage<T, DP, BN, 256>(sk[buf], [&](int r) { return K + (int64_t)min(kb + r, thi - 1) * A.k_rs; }, A.D, A.k_vec);
+        stage<T, DP, BN, 256>(sv[buf], [&](int r) { return V + (int64_t)min(kb + r, thi - 1) * A.v_rs; }, A.D, A.v_vec);
+        kp.fetch(A, A.kpos, min(kb + tid, thi - 1));
     };
-    f32x4 acc[DB];
+    f32x4 acc[MB][DB];
+    Slope sl[MB];
 #pragma unroll
-    for (int d = 0; d < DB; ++d) acc[d] = f32x4{0.f, 0.f, 0.f, 0.f};
-    Slope sl;
-    if (tlo < thi) fetch(tlo);
-    for (int kb = tlo; kb < thi; kb += BN) {
-        __syncthreads();
+    for (int b = 0; b < MB; ++b)
 #pragma unroll
-        for (int i = 0; i < PER; ++i) {
-            const int e = tid + i * 256;
-            sk[L::slot(e / L::NCH, e % L::NCH)] = rk[i];
-            sv[L::slot(e / L::NCH, e % L::NCH)] = rv[i];
-        }
+        for (int d = 0; d < DB; ++d) acc[b][d] = f32x4{0.f, 0.f, 0.f, 0.f};
+    if (tlo < thi) issue(tlo, 0);
+    int buf = 0;
+    for (int kb = tlo; kb < thi; kb += BN, buf ^= 1) {
+        kp.put(sp[buf]);
+        landed();
         __syncthreads();
-        if (kb + BN < thi) fetch(kb + BN);
+        if (kb + BN < thi) issue(kb + BN, buf ^ 1);
 #pragma unroll
         for (int j = 0; j < BN / X::KB; ++j) {
             const int k0 = kb + j * X::KB;
             if (k0 >= whi || k0 + X::KB <= wlo) continue;
-            f32x4 dz[PB];
+            f32x4 x[MB][PB], e[MB][PB];
 #pragma unroll
-            for (int b = 0; b < PB; ++b) {
-                f32x4 a = {0.f, 0.f, 0.f, 0.f}, e = {0.f, 0.f, 0.f, 0.f};
+            for (int n = 0; n < PB; ++n) {
+#pragma unroll
+                for (int b = 0; b < MB; ++b) x[b][n] = e[b][n] = f32x4{0.f, 0.f, 0.f, 0.f};
 #pragma unroll
                 for (int f = 0; f < NF; ++f) {
-                    a = mma(frag_rows<T, DP>(sk, j * X::KB + b * 16, f, lane), qf[f], a);
-                    e = mma(frag_rows<T, DP>(sv, j * X::KB + b * 16, f, lane), gf[f], e);
+                    const typename X::frag ka = frag_rows<T, DP>(sk[buf], j * X::KB + n * 16, f, lane);
+                    const typename X::frag va = frag_rows<T, DP>(sv[buf], j * X::KB + n * 16, f, lane);
+#pragma unroll
+                    for (int b = 0; b < MB; ++b) {
+                        x[b][n] = mma(ka, qf[b][f], x[b][n]);
+                        e[b][n] = mma(va, gf[b][f], e[b][n]);
+                    }
+                }
+                f32x4 px, py, pz;
+                const int at = j * X::KB + n * 16 + 4 * g;
+                if constexpr (AX > 0) px = *reinterpret_cast<const f32x4 *>(&sp[buf][0][at]);
+                if constexpr (AX > 1) {
+                    py = *reinterpret_cast<const f32x4 *>(&sp[buf][1][at]);
+                    pz = *reinterpret_cast<const f32x4 *>(&sp[buf][2][at]);
                 }
 #pragma unroll
-                for (int i = 0; i < 4; ++i) {
-                    const int key = k0 + b * 16 + 4 * g + i;
-                    const bool seen = key >= s.lo && key < s.hi;
-                    const Grad q = pair_grad(A, a[i], e[i], inv_cap, s.slope, s.pos, A.kpos + (int64_t)min(key, A.nk - 1) * A.axes, lse, delta);
-                    dz[b][i] = seen ? q.dz : 0.f;
-                    if (A.dsl) sl.add(q, seen);
+                for (int b = 0; b < MB; ++b) {
+                    const bool masked = k0 + n * 16 < lo_last[b] || k0 + n * 16 + 16 > hi_first[b];
+                    f32x4 p, ds, dist;
+#pragma unroll
+                    for (int i = 0; i < 4; ++i) {
+                        float t = 0.f, v;
+                        if constexpr (!CAP && AX == 0) v = x[b][n][i] * S.k - lse[b];
+                        else v = S.value(x[b][n][i], t) - lse[b];
+                        if constexpr (AX > 0) {
+                            dist[i] = S.dist(s[b].pos, px[i], AX > 1 ? py[i] : 0.f, AX > 1 ? pz[i] : 0.f);
+                            v -= s[b].slope * dist[i];
+                        }
+                        p[i] = exp2_(v);
+                        x[b][n][i] = t;
+                    }
+                    if (masked) {
+#pragma unroll
+                        for (int i = 0; i < 4; ++i) {
+                            const int key = kb + at + i;
+                            p[i] = key >= s[b].lo && key < s[b].hi ? p[i] : 0.f;
+                            e[b][n][i] = key >= s[b].lo && key < s[b].hi ? e[b][n][i] : 0.f;        // 0 * inf
+                            if constexpr (CAP) x[b][n][i] = key >= s[b].lo && key < s[b].hi ? x[b][n][i] : 0.f;
+                        }
+                    }
+#pragma unroll
+                    for (int i = 0; i < 4; ++i) ds[i] = p[i] * (e[b][n][i] - delta[b]);
+                    if constexpr (AX > 0)
+                        if (A.dsl) sl[b].add(p, ds, dist);
+#pragma unroll
+                    for (int i = 0; i < 4; ++i) e[b][n][i] = CAP ? ds[i] * (1.f - x[b][n][i] * x[b][n][i]) : ds[i];
                 }
             }
-            const typename X::frag p = pack_p(dz, T());
+            typename X::frag z[MB];
 #pragma unroll
-            for (int d = 0; d < DB; ++d) acc[d] = mma(frag_cols<DP>(sk, j * X::KB, d, lane, T()), p, acc[d]);
+            for (int b = 0; b < MB; ++b) z[b] = pack_p(e[b], T());
+#pragma unroll
+            for (int d = 0; d < DB; ++d) {
+                const typename X::frag a = frag_cols<DP>(sk[buf], j * X::KB, d, lane, T());
+#pragma unroll
+                for (int b = 0; b < MB; ++b) acc[b][d] = mma(a, z[b], acc[b][d]);
+            }
         }
     }
-    sl.ds = group_sum(sl.ds);
-    sl.dsd = group_sum(sl.dsd);
-    sl.pd = group_sum(sl.pd);
-    const float dslope = sl.row();
-    bool fine = finite_(dslope);
 #pragma unroll
-    for (int d = 0; d < DB; ++d)
+    for (int b = 0; b < MB; ++b) {
+        const int64_t r = r0 + (w * MB + b) * 16 + c;
+        const float dslope = AX > 0 ? sl[b].row_of_groups() : 0.f;
+        bool fine = finite_(dslope);
 #pragma unroll
-        for (int i = 0; i < 4; ++i) {
-            acc[d][i] *= A.scale;
-            fine = fine && finite_(acc[d][i]);
+        for (int d = 0; d < DB; ++d)
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+                acc[b][d][i] *= A.scale;
+                fine = fine && finite_(acc[b][d][i]);
+            }
+        if (r < R) {
+            T *out = reinterpret_cast<T *>(A.dq) + ((int64_t)s[b].row * A.H + s[b].head) * A.D;
+#pragma unroll
+            for (int d = 0; d < DB; ++d) store4(out, acc[b][d], d * 16 + g * 4, A.D, A.o_vec != 0);
+            if (AX > 0 && A.dsl && g == 0) A.dsl[kvh * R + r] = dslope;
         }
-    if (r < R) {
-        T *out = reinterpret_cast<T *>(A.dq) + ((int64_t)s.row * A.H + s.head) * A.D;
-#pragma unroll
-        for (int d = 0; d < DB; ++d) store4(out, acc[d], d * 16 + g * 4, A.D, A.o_vec != 0);
-        if (A.dsl && g == 0) A.dsl[kvh * R + r] = dslope;
-    }
-    uint64_t bad = __ballot(!fine && r < R);
-    while (bad) {
-        const int src = __builtin_ctzll(bad) & 15;
-        bad &= ~(0x0001000100010001ull << src);
-        const RowState t = row_state(A, kvh, r0 + w * 16 + src, R);
-        dq_slow<T>(A, kvh, t, r0 + w * 16 + src, R);
+        uint64_t bad = __ballot(!fine && r < R);
+        while (bad) {
+            const int src = __builtin_ctzll(bad) & 15;
+            bad &= ~(0x0001000100010001ull << src);
+            const int64_t rr = r - c + src;
+            dq_slow<T>(A, kvh, row_state(A, kvh, rr, R), rr, R);
+        }
     }
 }
 
 // ---------------------------------------------------------------------------------------------------------------------
-// dk and dv: 64 keys a workgroup, 16 a wave (columns); tiles of BM packed rows (q, do and what belongs to a row) in LDS
+// dk and dv: 64 MB keys a workgroup, 16 MB a wave (columns); tiles of BM packed rows (q, do and what belongs to a row) in LDS.
+// parts > 1: a workgroup takes one part of the rows that see its keys and leaves fp32 sums; scene_attn_dkv_join_kernel adds them.
 // ---------------------------------------------------------------------------------------------------------------------
-template <typename T, int DP, int BM>
+template <typename T, int DP, int BM, int MB, bool CAP, int AX>
 __global__ __launch_bounds__(256) void scene_attn_dkv_kernel(const SceneAttnArgs A) {
     using X = Tr<T>;
     using L = Tile<T, DP>;
-    constexpr int NF = DP / X::KD, DB = DP / 16, PB = X::KB / 16, NC = BM * L::NCH, PER = NC / 256;
-    static_assert(NC % 256 == 0 && BM % X::KB == 0 && BM <= 64, "tile");
-    __shared__ u32x4 sq[NC], sg[NC];
-    __shared__ float srow[BM][8];                // lse, delta, slope, lo, hi, position
+    constexpr int NF = DP / X::KD, DB = DP / 16, PB = X::KB / 16, NC = BM * L::NCH, KEYS = 64 * MB, NV = 5 + AX;
+    static_assert(BM % X::KB == 0 && BM <= 64, "tile");
+    __shared__ u32x4 sq[2][NC], sg[2][NC];
+    __shared__ __attribute__((aligned(16))) float srow[2][NV][BM];      // lse, delta, slope, lo, hi, position
     const int tid = threadIdx.x, lane = tid & 63, w = tid >> 6, g = lane >> 4, c = lane & 15;
-    const int kvh = (int)(blockIdx.x % A.KV);
+    const int kvh = (int)(blockIdx.x % A.KV), part = (int)(blockIdx.x / A.KV % A.parts);
     const int64_t R = (int64_t)A.nq * A.G;
-    const int k0 = (int)(blockIdx.x / A.KV) * 64, key = k0 + w * 16 + c, kk = min(key, A.nk - 1);
-    const T *K = reinterpret_cast<const T *>(A.k) + (int64_t)kk * A.k_rs + kvh * A.k_hs, *V = reinterpret_cast<const T *>(A.v) + (int64_t)kk * A.v_rs + kvh * A.v_hs;
-    typename X::frag kf[NF], vf[NF];
+    const int k0 = (int)(blockIdx.x / A.KV / A.parts) * KEYS, kw = k0 + w * 16 * MB;
+    const Score<T, CAP, AX> S(A);
+    typename X::frag kf[MB][NF], vf[MB][NF];
+    float kpos[MB][3];
 #pragma unroll
-    for (int f = 0; f < NF; ++f) {
-        kf[f] = as_frag<T>(load_chunk<T>(K, f * X::KD + g * X::CH, A.D, A.k_vec));
-        vf[f] = as_frag<T>(load_chunk<T>(V, f * X::KD + g * X::CH, A.D, A.v_vec));
-    }
-    float kpos[3] = {0.f, 0.f, 0.f};
-    for (int a = 0; a < A.axes; ++a) kpos[a] = A.kpos[(int64_t)kk * A.axes + a];
-    const int64_t ra = (int64_t)max(A.key_lo[k0], 0) * A.G, rb = (int64_t)min(A.key_hi[min(k0 + 63, A.nk - 1)], A.nq) * A.G;
-    const int64_t wa = (int64_t)max(A.key_lo[min(k0 + w * 16, A.nk - 1)], 0) * A.G;
-    const int64_t wb = (int64_t)min(A.key_hi[min(k0 + w * 16 + 15, A.nk - 1)], A.nq) * A.G;
-    const float inv_cap = A.cap > 0.f ? 1.f / A.cap : 0.f;
-
-    u32x4 rq[PER], rg[PER];
-    float extra[8];
-    auto fetch = [&](int64_t rbase) {
+    for (int b = 0; b < MB; ++b) {
+        const int kk = min(kw + b * 16 + c, A.nk - 1);
+        const T *K = reinterpret_cast<const T *>(A.k) + (int64_t)kk * A.k_rs + kvh * A.k_hs, *V = reinterpret_cast<const T *>(A.v) + (int64_t)kk * A.v_rs + kvh * A.v_hs;
 #pragma unroll
-        for (int i = 0; i < PER; ++i) {
-            const int e = tid + i * 256, ch = e % L::NCH;
-            const int64_t rr = rbase + e / L::NCH;
-            const u32x4 z = {0u, 0u, 0u, 0u};
-            rq[i] = rg[i] = z;
-            if (rr < rb) {
-                const int64_t row = rr / A.G, head = kvh * A.G + (rr - row * A.G);
-                rq[i] = load_chunk<T>(reinterpret_cast<const T *>(A.q) + row * A.q_rs + head * A.q_hs, ch * X::CH, A.D, A.q_vec);
-                rg[i] = load_chunk<T>(reinterpret_cast<const T *>(A.dout) + row * A.do_rs + head * A.do_hs, ch * X::CH, A.D, A.do_vec);
-            }
+        for (int f = 0; f < NF; ++f) {
+            kf[b][f] = as_frag<T>(load_chunk<T>(K, f * X::KD + g * X::CH, A.D, A.k_vec));
+            vf[b][f] = as_frag<T>(load_chunk<T>(V, f * X::KD + g * X::CH, A.D, A.v_vec));
         }
+#pragma unroll
+        for (int a = 0; a < 3; ++a) kpos[b][a] = a < AX && a < A.axes ? A.kpos[(int64_t)kk * A.axes + a] : 0.f;
+    }
+    // the packed rows that see the workgroup's keys (this part of them), and this wave's
+    int64_t ra = (int64_t)max(A.key_lo[k0], 0) * A.G, rb = (int64_t)min(A.key_hi[min(k0 + KEYS - 1, A.nk - 1)], A.nq) * A.G;
+    const int64_t wa = (int64_t)max(A.key_lo[min(kw, A.nk - 1)], 0) * A.G, wb = (int64_t)min(A.key_hi[min(kw + 16 * MB - 1, A.nk - 1)], A.nq) * A.G;
+    if (A.parts > 1) {
+        const int64_t per = ((rb - ra + A.parts - 1) / A.parts + BM - 1) / BM * BM;
+        ra += per * part;
+        rb = min(rb, ra + per);
+    }
+    float extra[NV];
+    auto issue = [&](int64_t rbase, int buf) {
+        auto at = [&](int r, int64_t rs, int64_t hs) {
+            const int64_t rr = min(rbase + r, rb - 1), row = A.G == 1 ? rr : rr / A.G;
+            return row * rs + (kvh * A.G + (rr - row * A.G)) * hs;
+        };
+        stage<T, DP, BM, 256>(sq[buf], [&](int r) { return reinterpret_cast<const T *>(A.q) + at(r, A.q_rs, A.q_hs); }, A.D, A.q_vec);
+        stage<T, DP, BM, 256>(sg[buf], [&](int r) { return reinterpret_cast<const T *>(A.dout) + at(r, A.do_rs, A.do_hs); }, A.D, A.do_vec);
         if (tid < BM) {
             const int64_t rr = rbase + tid;
-            const RowState s = row_state(A, kvh, rr, R);
             const bool in = rr < rb;
-            extra[0] = in ? A.lse[kvh * R + rr] : 0.f;
-            extra[1] = in ? A.delta[kvh * R + rr] : 0.f;
+            const RowState s = row_state(A, kvh, rr, R);
+            extra[0] = A.lse[kvh * R + min(rr, rb - 1)];
+            extra[1] = A.delta[kvh * R + min(rr, rb - 1)];
             extra[2] = s.slope;
-            extra[3] = __int_as_float(in ? s.lo : 0);
+            extra[3] = __int_as_float(in ? s.lo : 0x7fffffff);           // rows behind the last one see nothing
             extra[4] = __int_as_float(in ? s.hi : 0);
-            extra[5] = s.pos[0]; extra[6] = s.pos[1]; extra[7] = s.pos[2];
+#pragma unroll
+            for (int a = 0; a < AX; ++a) extra[5 + a] = s.pos[a];
         }
     };
-    f32x4 dk[DB], dv[DB];
+    f32x4 dk[MB][DB], dv[MB][DB];
 #pragma unroll
-    for (int d = 0; d < DB; ++d) dk[d] = dv[d] = f32x4{0.f, 0.f, 0.f, 0.f};
-    if (ra < rb) fetch(ra);
-    for (int64_t rbase = ra; rbase < rb; rbase += BM) {
-        __syncthreads();
+    for (int b = 0; b < MB; ++b)
 #pragma unroll
-        for (int i = 0; i < PER; ++i) {
-            const int e = tid + i * 256;
-            sq[L::slot(e / L::NCH, e % L::NCH)] = rq[i];
-            sg[L::slot(e / L::NCH, e % L::NCH)] = rg[i];
-        }
+        for (int d = 0; d < DB; ++d) dk[b][d] = dv[b][d] = f32x4{0.f, 0.f, 0.f, 0.f};
+    if (ra < rb) issue(ra, 0);
+    int buf = 0;
+    for (int64_t rbase = ra; rbase < rb; rbase += BM, buf ^= 1) {
         if (tid < BM) {
 #pragma unroll
-            for (int i = 0; i < 8; ++i) srow[tid][i] = extra[i];
+            for (int i = 0; i < NV; ++i) srow[buf][i][tid] = extra[i];
         }
+        landed();
         __syncthreads();
-        if (rbase + BM < rb) fetch(rbase + BM);
+        if (rbase + BM < rb) issue(rbase + BM, buf ^ 1);
 #pragma unroll
         for (int j = 0; j < BM / X::KB; ++j) {
             const int64_t r0 = rbase + j * X::KB;
             if (r0 >= wb || r0 + X::KB <= wa) continue;
-            f32x4 p[PB], dz[PB];
+            f32x4 p[MB][PB], z[MB][PB];
 #pragma unroll
-            for (int b = 0; b < PB; ++b) {
-                f32x4 a = {0.f, 0.f, 0.f, 0.f}, e = {0.f, 0.f, 0.f, 0.f};
+            for (int n = 0; n < PB; ++n) {
+                const int at = j * X::KB + n * 16;
+#pragma unroll
+                for (int b = 0; b < MB; ++b) p[b][n] = z[b][n] = f32x4{0.f, 0.f, 0.f, 0.f};
 #pragma unroll
                 for (int f = 0; f < NF; ++f) {
-                    a = mma(frag_rows<T, DP>(sq, j * X::KB + b * 16, f, lane), kf[f], a);
-                    e = mma(frag_rows<T, DP>(sg, j * X::KB + b * 16, f, lane), vf[f], e);
-                }
+                    const typename X::frag qa = frag_rows<T, DP>(sq[buf], at, f, lane);
+                    const typename X::frag ga = frag_rows<T, DP>(sg[buf], at, f, lane);
 #pragma unroll
-                for (int i = 0; i < 4; ++i) {
-                    const float *s = srow[j * X::KB + b * 16 + 4 * g + i];
-                    const bool seen = key >= __float_as_int(s[3]) && key < __float_as_int(s[4]);
-                    const Grad q = pair_grad(A, a[i], e[i], inv_cap, s[2], s + 5, kpos, s[0], s[1]);
-                    p[b][i] = seen ? q.p : 0.f;
-                    dz[b][i] = seen ? q.dz : 0.f;
+                    for (int b = 0; b < MB; ++b) {
+                        p[b][n] = mma(qa, kf[b][f], p[b][n]);
+                        z[b][n] = mma(ga, vf[b][f], z[b][n]);
+                    }
+                }
+                auto col = [&](int v) { return *reinterpret_cast<const f32x4 *>(&srow[buf][v][at + 4 * g]); };
+                const f32x4 lse = col(0), delta = col(1);
+                f32x4 slope, px, py, pz;
+                if constexpr (AX > 0) { slope = col(2); px = col(5); }
+                if constexpr (AX > 1) { py = col(6); pz = col(7); }
+                // do all 16 rows see all of the block's keys?
+                const int lo_last = uniform(__float_as_int(srow[buf][3][at + 15])), hi_first = uniform(__float_as_int(srow[buf][4][at]));
+#pragma unroll
+                for (int b = 0; b < MB; ++b) {
+                    const bool masked = kw + b * 16 < lo_last || kw + b * 16 + 16 > hi_first;
+                    f32x4 t;
+#pragma unroll
+                    for (int i = 0; i < 4; ++i) {
+                        float v;
+                        t[i] = 0.f;
+                        if constexpr (!CAP && AX == 0) v = p[b][n][i] * S.k - lse[i];
+                        else {
+                            float tt;
+                            v = S.value(p[b][n][i], tt) - lse[i];
+                            if constexpr (CAP) t[i] = tt;
+                        }
+                        if constexpr (AX > 0) v -= slope[i] * S.dist(kpos[b], px[i], AX > 1 ? py[i] : 0.f, AX > 1 ? pz[i] : 0.f);
+                        p[b][n][i] = exp2_(v);
+                    }
+                    if (masked) {
+                        const f32x4 lo = col(3), hi = col(4);
+                        const int key = kw + b * 16 + c;
+#pragma unroll
+                        for (int i = 0; i < 4; ++i) {
+                            const bool seen = key >= __float_as_int(lo[i]) && key < __float_as_int(hi[i]);
+                            p[b][n][i] = seen ? p[b][n][i] : 0.f;
+                            z[b][n][i] = seen ? z[b][n][i] - delta[i] : 0.f;             // 0 * inf
+                            if constexpr (CAP) t[i] = seen ? t[i] : 0.f;
+                        }
+                    } else {
+#pragma unroll
+                        for (int i = 0; i < 4; ++i) z[b][n][i] -= delta[i];
+                    }
+#pragma unroll
+                    for (int i = 0; i < 4; ++i) z[b][n][i] *= CAP ? p[b][n][i] * (1.f - t[i] * t[i]) : p[b][n][i];
                 }
             }
-            const typename X::frag pf = pack_p(p, T()), zf = pack_p(dz, T());
+            typename X::frag pf[MB], zf[MB];
+#pragma unroll
+            for (int b = 0; b < MB; ++b) {
+                pf[b] = pack_p(p[b], T());
+                zf[b] = pack_p(z[b], T());
+            }
 #pragma unroll
             for (int d = 0; d < DB; ++d) {
-                dv[d] = mma(frag_cols<DP>(sg, j * X::KB, d, lane, T()), pf, dv[d]);
-                dk[d] = mma(frag_cols<DP>(sq, j * X::KB, d, lane, T()), zf, dk[d]);
+                const typename X::frag ga = frag_cols<DP>(sg[buf], j * X::KB, d, lane, T());
+                const typename X::frag qa = frag_cols<DP>(sq[buf], j * X::KB, d, lane, T());
+#pragma unroll
+                for (int b = 0; b < MB; ++b) {
+                    dv[b][d] = mma(ga, pf[b], dv[b][d]);
+                    dk[b][d] = mma(qa, zf[b], dk[b][d]);
+                }
             }
         }
     }
-    bool fine = true;
 #pragma unroll
-    for (int d = 0; d < DB; ++d)
-#pragma unroll
-        for (int i = 0; i < 4; ++i) {
-            dk[d][i] *= A.scale;
-            fine = fine && finite_(dk[d][i]) && finite_(dv[d][i]);
-        }
-    if (key < A.nk) {
+    for (int b = 0; b < MB; ++b) {
+        const int key = kw + b * 16 + c;
         const int64_t at = ((int64_t)key * A.KV + kvh) * A.D;
+        bool fine = true;
 #pragma unroll
-        for (int d = 0; d < DB; ++d) {
-            store4(reinterpret_cast<T *>(A.dk) + at, dk[d], d * 16 + g * 4, A.D, A.o_vec != 0);
-            store4(reinterpret_cast<T *>(A.dv) + at, dv[d], d * 16 + g * 4, A.D, A.o_vec != 0);
+        for (int d = 0; d < DB; ++d)
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+                dk[b][d][i] *= A.scale;
+                fine = fine && finite_(dk[b][d][i]) && finite_(dv[b][d][i]);
+            }
+        if (A.parts > 1) {
+            const int64_t n = (int64_t)A.nk * A.KV * A.D;
+            if (key < A.nk) {
+#pragma unroll
+                for (int d = 0; d < DB; ++d) {
+                    store4(A.part + 2 * part * n + at, dk[b][d], d * 16 + g * 4, A.D, A.D % 4 == 0);
+                    store4(A.part + (2 * part + 1) * n + at, dv[b][d], d * 16 + g * 4, A.D, A.D % 4 == 0);
+                }
+            }
+            continue;
         }
-    }
-    uint64_t bad = __ballot(!fine && key < A.nk);
-    while (bad) {
-        const int src = __builtin_ctzll(bad) & 15;
-        bad &= ~(0x0001000100010001ull << src);
-        dkv_slow<T>(A, kvh, k0 + w * 16 + src, R);
+        if (key < A.nk) {
+#pragma unroll
+            for (int d = 0; d < DB; ++d) {
+                store4(reinterpret_cast<T *>(A.dk) + at, dk[b][d], d * 16 + g * 4, A.D, A.o_vec != 0);
+                store4(reinterpret_cast<T *>(A.dv) + at, dv[b][d], d * 16 + g * 4, A.D, A.o_vec != 0);
+            }
+        }
+        uint64_t bad = __ballot(!fine && key < A.nk);
+        while (bad) {
+            const int src = __builtin_ctzll(bad) & 15;
+            bad &= ~(0x0001000100010001ull << src);
+            dkv_slow<T>(A, kvh, key - c + src, R);
+        }
     }
 }
 
-template <typename T, int DP, int BN> hipError_t launch_bwd(const SceneAttnArgs &A, float *dslopes, hipStream_t st) {
-    const int64_t n = (int64_t)A.nq * A.H, tiles = ((int64_t)A.nq * A.G + 63) / 64;
-    if (n > 0) {
-        hipLaunchKernelGGL((scene_attn_delta_kernel<T>), dim3((unsigned)((n + 63) / 64)), dim3(256), 0, st, A);
-        if (A.dq) hipLaunchKernelGGL((scene_attn_dq_kernel<T, DP, BN>), dim3((unsigned)(tiles * A.KV)), dim3(256), 0, st, A);
+// dk and dv from the parts' sums, in order; a wave per (key, kv head)
+template <typename T> __global__ __launch_bounds__(256) void scene_attn_dkv_join_kernel(const SceneAttnArgs A) {
+    const int lane = threadIdx.x & 63;
+    const int64_t item = (int64_t)blockIdx.x * 4 + (threadIdx.x >> 6), n = (int64_t)A.nk * A.KV * A.D;
+    if (item >= (int64_t)A.nk * A.KV) return;
+    bool fine = true;
+    for (int d = lane; d < A.D; d += 64) {
+        const float *p = A.part + item * A.D + d;
+        float a = 0.f, b = 0.f;
+        for (int i = 0; i < A.parts; ++i) {
+            a += p[2 * i * n];
+            b += p[(2 * i + 1) * n];
+        }
+        reinterpret_cast<T *>(A.dk)[item * A.D + d] = (T)a;
+        reinterpret_cast<T *>(A.dv)[item * A.D + d] = (T)b;
+        fine = fine && finite_(a) && finite_(b);
     }
-    if (A.nk > 0 && A.dk) hipLaunchKernelGGL((scene_attn_dkv_kernel<T, DP, BN>), dim3((unsigned)(((int64_t)A.nk + 63) / 64 * A.KV)), dim3(256), 0, st, A);
+    if (__any(!fine)) dkv_slow<T>(A, (int)(item % A.KV), item / A.KV, (int64_t)A.nq * A.G);
+}
+
+template <typename T, int DP, int BN, bool CAP, int AX> hipError_t launch_bwd(const SceneAttnArgs &A, hipStream_t st) {
+    const int64_t tiles = ((int64_t)A.nq * A.G + 63) / 64;
+    if (tiles > 0 && A.dq) hipLaunchKernelGGL((scene_attn_dq_kernel<T, DP, BN, 1, CAP, AX>), dim3((unsigned)(tiles * A.KV)), dim3(256), 0, st, A);
+    if (A.nk > 0 && A.dk) {
+        hipLaunchKernelGGL((scene_attn_dkv_kernel<T, DP, BN, 1, CAP, AX>), dim3((unsigned)(((int64_t)A.nk + 63) / 64 * A.KV * A.parts)), dim3(256), 0, st, A);
+        if (A.parts > 1) hipLaunchKernelGGL((scene_attn_dkv_join_kernel<T>), dim3((unsigned)(((int64_t)A.nk * A.KV + 3) / 4)), dim3(256), 0, st, A);
+    }
+    return hipGetLastError();
+}
+template <typename T, int DP, int BN> hipError_t pick_bwd(const SceneAttnArgs &A, hipStream_t st) {
+    if (A.cap > 0.f) return A.axes == 0 ? launch_bwd<T, DP, BN, true, 0>(A, st) : A.axes == 1 ? launch_bwd<T, DP, BN, true, 1>(A, st) : launch_bwd<T, DP, BN, true, 3>(A, st);
+    return A.axes == 0 ? launch_bwd<T, DP, BN, false, 0>(A, st) : A.axes == 1 ? launch_bwd<T, DP, BN, false, 1>(A, st) : launch_bwd<T, DP, BN, false, 3>(A, st);
+}
+template <typename T> hipError_t run_bwd(const SceneAttnArgs &A, float *dslopes, hipStream_t st) {
+    const int64_t n = (int64_t)A.nq * A.H;
+    if (n > 0) hipLaunchKernelGGL((scene_attn_delta_kernel<T>), dim3((unsigned)((n + 63) / 64)), dim3(256), 0, st, A);
+    const int D = A.D;
+    hipError_t e;
+    if constexpr (sizeof(T) == 2) e = D <= 32 ? pick_bwd<T, 32, 64>(A, st) : D <= 64 ? pick_bwd<T, 64, 64>(A, st) : D <= 96 ? pick_bwd<T, 96, 32>(A, st) : pick_bwd<T, 128, 32>(A, st);
+    else e = D <= 16 ? pick_bwd<T, 16, 64>(A, st) : D <= 32 ? pick_bwd<T, 32, 32>(A, st) : D <= 48 ? pick_bwd<T, 48, 32>(A, st) : D <= 64 ? pick_bwd<T, 64, 32>(A, st)
+           : D <= 96 ? pick_bwd<T, 96, 32>(A, st) : pick_bwd<T, 128, 32>(A, st);
+    if (e != hipSuccess) return e;
     if (dslopes) hipLaunchKernelGGL(scene_attn_dslope_kernel, dim3(A.H), dim3(256), 0, st, A.nq, A.G, A.dsl, dslopes);
     return hipGetLastError();
 }
 
 }  // namespace sattn
 
-extern "C" hipError_t dn_scene_attn_bwd(const SceneAttnArgs *A, int bf, float *dslopes, hipStream_t st) {
-    using namespace sattn;
-    const int D = A->D;
-    if (bf) return D <= 32 ? launch_bwd<bf16, 32, 64>(*A, dslopes, st) : D <= 64 ? launch_bwd<bf16, 64, 64>(*A, dslopes, st) : launch_bwd<bf16, 128, 32>(*A, dslopes, st);
-    return D <= 16 ? launch_bwd<float, 16, 64>(*A, dslopes, st) : D <= 32 ? launch_bwd<float, 32, 64>(*A, dslopes, st)
-         : D <= 64 ? launch_bwd<float, 64, 32>(*A, dslopes, st) : launch_bwd<float, 128, 32>(*A, dslopes, st);
+// one object file per type (the Makefile compiles this source twice)
+#ifdef SCENE_ATTN_BF16
+extern "C" hipError_t dn_scene_attn_bwd_bf16(const SceneAttnArgs *A, float *dslopes, hipStream_t st) { return sattn::run_bwd<sattn::bf16>(*A, dslopes, st); }
+#else
+extern "C" hipError_t dn_scene_attn_bwd_f32(const SceneAttnArgs *A, float *dslopes, hipStream_t st) { return sattn::run_bwd<float>(*A, dslopes, st); }
+// Parts of the rows in the dk / dv kernel: as many as give the chip four workgroups a CU, but none below 512 packed rows.
+extern "C" int dn_scene_attn_bwd_parts(int64_t nq, int64_t nk, int KV, int G) {
+    const int64_t groups = (nk + 63) / 64 * KV, want = groups ? 1024 / groups : 1, most = nq * G / 512;
+    return (int)(want < 1 || most < 1 ? 1 : want < most ? (want < 16 ? want : 16) : (most < 16 ? most : 16));
 }
+#endif

@@ -1,7 +1,7 @@
 // Forward of the scene attention (scene_attn.h has the mathematics and the layout).
 //
-// One workgroup: 64 packed rows of one kv head, 16 per wave; K and V tiles of BN keys staged in LDS, the next tile's loads in flight in
-// registers while the current one is worked on.  A wave skips 16-key blocks that none of its rows sees, so a tile that holds
+// One workgroup: 64 packed rows of one kv head, 16 per wave (or 128, 32 per wave); K and V tiles of BN keys in LDS twice over, the next
+// tile's loads going straight into the other copy while the current one is worked on.  A wave skips 16-key blocks that none of its rows sees, so a tile that holds
 // several small scenes costs each wave its own scenes only.
 #include "scene_attn.h"
 
@@ -40,138 +40,224 @@ template <typename T> __device__ void row_slow(const SceneAttnArgs &A, int kvh, 
     if (A.lse && lane == 0) A.lse[kvh * R + r] = l == 0.f ? 0.f : m + log2_(l);
 }
 
-template <typename T, int DP, int BN>
+// MB: 16-row blocks per wave.  One (64 rows a workgroup) where the rows would not fill the chip otherwise, two (128 rows) where they do: every K and
+// V fragment read from LDS then serves two products.
+template <typename T, int DP, int BN, int MB, bool CAP, int AX>
 __global__ __launch_bounds__(256) void scene_attn_fwd_kernel(const SceneAttnArgs A) {
     using X = Tr<T>;
     using L = Tile<T, DP>;
-    constexpr int NF = DP / X::KD, NB = BN / 16, DB = DP / 16, PB = X::KB / 16, NC = BN * L::NCH, PER = NC / 256;
-    static_assert(NC % 256 == 0 && NB % PB == 0, "tile");
-    __shared__ u32x4 sk[NC], sv[NC];
+    constexpr int NF = DP / X::KD, NB = BN / 16, DB = DP / 16, PB = X::KB / 16, NC = BN * L::NCH, ROWS = 64 * MB;
+    static_assert(BN % X::KB == 0, "tile");
+    __shared__ u32x4 sk[2][NC], sv[2][NC];
+    __shared__ __attribute__((aligned(16))) float sp[2][AX ? AX : 1][BN];
     const int tid = threadIdx.x, lane = tid & 63, w = tid >> 6, g = lane >> 4, c = lane & 15;
     const int kvh = (int)(blockIdx.x % A.KV);
-    const int64_t R = (int64_t)A.nq * A.G, r0 = (int64_t)(gridDim.x / A.KV - 1 - blockIdx.x / A.KV) * 64, r = r0 + w * 16 + c;
-    const RowState s = row_state(A, kvh, r, R);
-    const T *Q = reinterpret_cast<const T *>(A.q) + s.row * A.q_rs + s.head * A.q_hs;
-    typename X::frag qf[NF];
-#pragma unroll
-    for (int f = 0; f < NF; ++f) qf[f] = as_frag<T>(load_chunk<T>(Q, f * X::KD + g * X::CH, A.D, A.q_vec));
-    // the keys of the workgroup's rows, and of this wave's
-    const int qa = (int)(r0 / A.G), qb = (int)((min(r0 + 64, R) - 1) / A.G);
-    const int tlo = max(A.row_lo[qa], 0), thi = min(A.row_hi[qb], A.nk);
-    const int wlo = __builtin_amdgcn_readfirstlane(__shfl(s.lo, 0)), whi = __builtin_amdgcn_readfirstlane(__shfl(s.hi, 15));
-    const int lo_last = __builtin_amdgcn_readfirstlane(__shfl(s.lo, 15)), hi_first = __builtin_amdgcn_readfirstlane(__shfl(s.hi, 0));
-    const T *K = reinterpret_cast<const T *>(A.k) + kvh * A.k_hs, *V = reinterpret_cast<const T *>(A.v) + kvh * A.v_hs;
-    const float inv_cap = A.cap > 0.f ? 1.f / A.cap : 0.f;
+    const int64_t R = (int64_t)A.nq * A.G, r0 = (int64_t)(gridDim.x / A.KV - 1 - blockIdx.x / A.KV) * ROWS;
+    const Score<T, CAP, AX> S(A);
+    constexpr bool PLAIN = !CAP && AX == 0;                 // scores stay raw until the exponent: 2^(raw k - base) in one fma
+    const bool flip = PLAIN && A.scale < 0.f;               // their maximum then needs k >= 0: the sign goes to q
+    const float k = flip ? -S.k : S.k;
 
-    u32x4 rk[PER], rv[PER];
-    auto fetch = [&](int kb) {
+    RowState s[MB];
+    typename X::frag qf[MB][NF];
 #pragma unroll
-        for (int i = 0; i < PER; ++i) {
-            const int e = tid + i * 256, key = kb + e / L::NCH, ch = e % L::NCH;
-            const u32x4 z = {0u, 0u, 0u, 0u};
-            const bool in = key < thi;
-            rk[i] = in ? load_chunk<T>(K + (int64_t)key * A.k_rs, ch * X::CH, A.D, A.k_vec) : z;
-            rv[i] = in ? load_chunk<T>(V + (int64_t)key * A.v_rs, ch * X::CH, A.D, A.v_vec) : z;
+    for (int b = 0; b < MB; ++b) {
+        s[b] = row_state(A, kvh, r0 + (w * MB + b) * 16 + c, R);
+        const T *Q = reinterpret_cast<const T *>(A.q) + s[b].row * A.q_rs + s[b].head * A.q_hs;
+#pragma unroll
+        for (int f = 0; f < NF; ++f) {
+            u32x4 v = load_chunk<T>(Q, f * X::KD + g * X::CH, A.D, A.q_vec);
+            if (flip) v ^= sizeof(T) == 4 ? 0x80000000u : 0x80008000u;
+            qf[b][f] = as_frag<T>(v);
         }
+    }
+    // the keys of the workgroup's rows, of this wave's, and those that all rows of a block see
+    const int qa = (int)(r0 / A.G), qb = (int)((min(r0 + ROWS, R) - 1) / A.G);
+    const int tlo = uniform(max(A.row_lo[qa], 0)), thi = uniform(min(A.row_hi[qb], A.nk));
+    const int wlo = uniform(__shfl(s[0].lo, 0)), whi = uniform(__shfl(s[MB - 1].hi, 15));
+    int lo_last[MB], hi_first[MB];
+#pragma unroll
+    for (int b = 0; b < MB; ++b) {
+        lo_last[b] = uniform(__shfl(s[b].lo, 15));
+        hi_first[b] = uniform(__shfl(s[b].hi, 0));
+    }
+    const T *K = reinterpret_cast<const T *>(A.k) + kvh * A.k_hs, *V = reinterpret_cast<const T *>(A.v) + kvh * A.v_hs;
+
+    KeyPos<AX, BN> kp;
+    auto issue = [&](int kb, int buf) {                     // keys behind the last one: the last one again, masked below
+        stage<T, DP, BN, 256>(sk[buf], [&](int r) { return K + (int64_t)min(kb + r, thi - 1) * A.k_rs; }, A.D, A.k_vec);
+        stage<T, DP, BN, 256>(sv[buf], [&](int r) { return V + (int64_t)min(kb + r, thi - 1) * A.v_rs; }, A.D, A.v_vec);
+        kp.fetch(A, A.kpos, min(kb + tid, thi - 1));
     };
-    f32x4 o[DB];
+    f32x4 o[MB][DB];
+    float m[MB], l[MB];
 #pragma unroll
-    for (int d = 0; d < DB; ++d) o[d] = f32x4{0.f, 0.f, 0.f, 0.f};
-    float m = NEG_INF, l = 0.f;
-    if (tlo < thi) fetch(tlo);
-    for (int kb = tlo; kb < thi; kb += BN) {
-        __syncthreads();
+    for (int b = 0; b < MB; ++b) {
+        m[b] = NEG_INF;
+        l[b] = 0.f;
 #pragma unroll
-        for (int i = 0; i < PER; ++i) {
-            const int e = tid + i * 256;
-            sk[L::slot(e / L::NCH, e % L::NCH)] = rk[i];
-            sv[L::slot(e / L::NCH, e % L::NCH)] = rv[i];
-        }
-        __syncthreads();
-        if (kb + BN < thi) fetch(kb + BN);
-        if (kb >= whi || kb + BN <= wlo) continue;          // the barriers above are met by every wave of the next round
-        f32x4 x[NB];
-        float top = NEG_INF;
+        for (int d = 0; d < DB; ++d) o[b][d] = f32x4{0.f, 0.f, 0.f, 0.f};
+    }
+    if (tlo < thi) issue(tlo, 0);
+    int buf = 0;
+    for (int kb = tlo; kb < thi; kb += BN, buf ^= 1) {
+        kp.put(sp[buf]);
+        landed();
+        __syncthreads();                                    // this tile is in LDS, and nobody reads the other one any more
+        if (kb + BN < thi) issue(kb + BN, buf ^ 1);
+        if (kb >= whi || kb + BN <= wlo) continue;
+        f32x4 x[MB][NB];
+        float top[MB];
 #pragma unroll
-        for (int b = 0; b < NB; ++b) {
-            const int k0 = kb + b * 16;
-            x[b] = f32x4{NEG_INF, NEG_INF, NEG_INF, NEG_INF};
-            if (k0 >= whi || k0 + 16 <= wlo) continue;
-            f32x4 a = {0.f, 0.f, 0.f, 0.f};
+        for (int b = 0; b < MB; ++b) top[b] = NEG_INF;
 #pragma unroll
-            for (int f = 0; f < NF; ++f) a = mma(frag_rows<T, DP>(sk, b * 16, f, lane), qf[f], a);
-            const bool masked = k0 < lo_last || k0 + 16 > hi_first;
+        for (int n = 0; n < NB; ++n) {
+            const int k0 = kb + n * 16;
+            if (k0 >= whi || k0 + 16 <= wlo) {
 #pragma unroll
-            for (int i = 0; i < 4; ++i) {
-                const int key = k0 + 4 * g + i;
-                const float y = score2(A, a[i], inv_cap, s.slope, s.pos, A.kpos + (int64_t)min(key, A.nk - 1) * A.axes);
-                x[b][i] = masked && (key < s.lo || key >= s.hi) ? NEG_INF : y;
-                top = fmaxf(top, x[b][i]);
+                for (int b = 0; b < MB; ++b) x[b][n] = f32x4{NEG_INF, NEG_INF, NEG_INF, NEG_INF};
+                continue;
+            }
+#pragma unroll
+            for (int b = 0; b < MB; ++b) x[b][n] = f32x4{0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+            for (int f = 0; f < NF; ++f) {
+                const typename X::frag a = frag_rows<T, DP>(sk[buf], n * 16, f, lane);
+#pragma unroll
+                for (int b = 0; b < MB; ++b) x[b][n] = mma(a, qf[b][f], x[b][n]);
+            }
+            f32x4 px, py, pz;
+            if constexpr (AX > 0) px = *reinterpret_cast<const f32x4 *>(&sp[buf][0][n * 16 + 4 * g]);
+            if constexpr (AX > 1) {
+                py = *reinterpret_cast<const f32x4 *>(&sp[buf][1][n * 16 + 4 * g]);
+                pz = *reinterpret_cast<const f32x4 *>(&sp[buf][2][n * 16 + 4 * g]);
+            }
+#pragma unroll
+            for (int b = 0; b < MB; ++b) {
+                if constexpr (!PLAIN) {
+#pragma unroll
+                    for (int i = 0; i < 4; ++i) {
+                        float t;
+                        float v = S.value(x[b][n][i], t);
+                        if constexpr (AX > 0) v -= s[b].slope * S.dist(s[b].pos, px[i], AX > 1 ? py[i] : 0.f, AX > 1 ? pz[i] : 0.f);
+                        x[b][n][i] = v;
+                    }
+                }
+                if (k0 < lo_last[b] || k0 + 16 > hi_first[b]) {
+#pragma unroll
+                    for (int i = 0; i < 4; ++i) {
+                        const int key = k0 + 4 * g + i;
+                        x[b][n][i] = key >= s[b].lo && key < s[b].hi ? x[b][n][i] : NEG_INF;
+                    }
+                }
+#pragma unroll
+                for (int i = 0; i < 4; ++i) top[b] = fmaxf(top[b], x[b][n][i]);
             }
         }
-        top = fmaxf(group_max(top), m);
-        const float base = top == NEG_INF ? 0.f : top, corr = exp2_(m - base);
-        m = top;
-        float sum = 0.f;
 #pragma unroll
-        for (int b = 0; b < NB; ++b)
+        for (int b = 0; b < MB; ++b) {
+            top[b] = group_max(top[b]);
+            if constexpr (PLAIN) top[b] = top[b] == NEG_INF ? NEG_INF : top[b] * k;
+            if (__any(top[b] > m[b])) {                     // a new maximum somewhere in the block: later tiles rarely bring one
+                const float nm = fmaxf(top[b], m[b]), corr = exp2_(m[b] - (nm == NEG_INF ? 0.f : nm));
+                m[b] = nm;
+                l[b] *= corr;
 #pragma unroll
-            for (int i = 0; i < 4; ++i) {
-                x[b][i] = exp2_(x[b][i] - base);
-                sum += x[b][i];
+                for (int d = 0; d < DB; ++d) o[b][d] *= corr;
             }
-        l = l * corr + sum;
+            const float base = m[b] == NEG_INF ? 0.f : m[b];
+            float sum = 0.f;
 #pragma unroll
-        for (int d = 0; d < DB; ++d) o[d] *= corr;
+            for (int n = 0; n < NB; ++n)
+#pragma unroll
+                for (int i = 0; i < 4; ++i) {
+                    x[b][n][i] = exp2_(PLAIN ? x[b][n][i] * k - base : x[b][n][i] - base);
+                    sum += x[b][n][i];
+                }
+            l[b] += sum;
+        }
 #pragma unroll
         for (int j = 0; j < NB / PB; ++j) {
             const int k0 = kb + j * X::KB;
             if (k0 >= whi || k0 + X::KB <= wlo) continue;
-            const typename X::frag p = pack_p(x + j * PB, T());
+            typename X::frag p[MB], rest[MB];
 #pragma unroll
-            for (int d = 0; d < DB; ++d) o[d] = mma(frag_cols<DP>(sv, j * X::KB, d, lane, T()), p, o[d]);
+            for (int b = 0; b < MB; ++b) p[b] = pack_p(&x[b][j * PB], T());
+            const bool exact = sizeof(T) == 2 && A.o32;     // training: what rounding p left over goes through the product too
+            if (exact) {
+#pragma unroll
+                for (int b = 0; b < MB; ++b) rest[b] = pack_rest(&x[b][j * PB], p[b]);
+            }
+#pragma unroll
+            for (int d = 0; d < DB; ++d) {
+                const typename X::frag a = frag_cols<DP>(sv[buf], j * X::KB, d, lane, T());
+#pragma unroll
+                for (int b = 0; b < MB; ++b) {
+                    o[b][d] = mma(a, p[b], o[b][d]);
+                    if (exact) o[b][d] = mma(a, rest[b], o[b][d]);
+                }
+            }
         }
     }
-    l = group_sum(l);
-    const float inv = l == 0.f ? 0.f : 1.f / l;
-    bool fine = finite_(l);
 #pragma unroll
-    for (int d = 0; d < DB; ++d)
+    for (int b = 0; b < MB; ++b) {
+        const int64_t r = r0 + (w * MB + b) * 16 + c;
+        const float sum = group_sum(l[b]), inv = sum == 0.f ? 0.f : 1.f / sum;
+        bool fine = finite_(sum);
 #pragma unroll
-        for (int i = 0; i < 4; ++i) {
-            o[d][i] *= inv;
-            fine = fine && finite_(o[d][i]);
+        for (int d = 0; d < DB; ++d)
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+                o[b][d][i] *= inv;
+                fine = fine && finite_(o[b][d][i]);
+            }
+        if (r < R) {
+            const int64_t at = ((int64_t)s[b].row * A.H + s[b].head) * A.D;
+#pragma unroll
+            for (int d = 0; d < DB; ++d) {
+                store4(reinterpret_cast<T *>(A.out) + at, o[b][d], d * 16 + g * 4, A.D, A.o_vec != 0);
+                if (A.o32) store4(A.o32 + at, o[b][d], d * 16 + g * 4, A.D, A.o_vec != 0);
+            }
+            if (A.lse && g == 0) A.lse[kvh * R + r] = sum == 0.f ? 0.f : m[b] + log2_(sum);
         }
-    if (r < R) {
-        const int64_t at = ((int64_t)s.row * A.H + s.head) * A.D;
-#pragma unroll
-        for (int d = 0; d < DB; ++d) {
-            store4(reinterpret_cast<T *>(A.out) + at, o[d], d * 16 + g * 4, A.D, A.o_vec != 0);
-            if (A.o32) store4(A.o32 + at, o[d], d * 16 + g * 4, A.D, A.o_vec != 0);
+        uint64_t bad = __ballot(!fine && r < R);
+        while (bad) {                                       // wave-uniform; the same row may be named by several lane groups
+            const int src = __builtin_ctzll(bad) & 15;
+            bad &= ~(0x0001000100010001ull << src);
+            const int64_t rr = r - c + src;
+            row_slow<T>(A, kvh, row_state(A, kvh, rr, R), rr, R);
         }
-        if (A.lse && g == 0) A.lse[kvh * R + r] = l == 0.f ? 0.f : m + log2_(l);
-    }
-    uint64_t bad = __ballot(!fine && r < R);
-    while (bad) {                                           // wave-uniform; the same row may be named by several lane groups
-        const int src = __builtin_ctzll(bad) & 15;
-        bad &= ~(0x0001000100010001ull << src);
-        RowState t = row_state(A, kvh, r0 + w * 16 + src, R);
-        row_slow<T>(A, kvh, t, r0 + w * 16 + src, R);
     }
 }
 
-template <typename T, int DP, int BN> hipError_t launch_fwd(const SceneAttnArgs &A, hipStream_t st) {
-    const int64_t tiles = ((int64_t)A.nq * A.G + 63) / 64;
-    hipLaunchKernelGGL((scene_attn_fwd_kernel<T, DP, BN>), dim3((unsigned)(tiles * A.KV)), dim3(256), 0, st, A);
+template <typename T, int DP, int BN, int MB, bool CAP, int AX> hipError_t launch_fwd(const SceneAttnArgs &A, hipStream_t st) {
+    const int64_t tiles = ((int64_t)A.nq * A.G + 64 * MB - 1) / (64 * MB);
+    hipLaunchKernelGGL((scene_attn_fwd_kernel<T, DP, BN, MB, CAP, AX>), dim3((unsigned)(tiles * A.KV)), dim3(256), 0, st, A);
     return hipGetLastError();
+}
+template <typename T, int DP, int BN, int MB> hipError_t pick_fwd(const SceneAttnArgs &A, hipStream_t st) {
+    if (A.cap > 0.f) return A.axes == 0 ? launch_fwd<T, DP, BN, MB, true, 0>(A, st) : A.axes == 1 ? launch_fwd<T, DP, BN, MB, true, 1>(A, st) : launch_fwd<T, DP, BN, MB, true, 3>(A, st);
+    return A.axes == 0 ? launch_fwd<T, DP, BN, MB, false, 0>(A, st) : A.axes == 1 ? launch_fwd<T, DP, BN, MB, false, 1>(A, st) : launch_fwd<T, DP, BN, MB, false, 3>(A, st);
 }
 
 }  // namespace sattn
 
-extern "C" hipError_t dn_scene_attn_fwd(const SceneAttnArgs *A, int bf, hipStream_t st) {
+// one object file per type (the Makefile compiles this source twice)
+#ifdef SCENE_ATTN_BF16
+template <int DP, int BN> static hipError_t fwd_rows(const SceneAttnArgs &A, hipStream_t st) {
+    using namespace sattn;
+    const int64_t tiles = ((int64_t)A.nq * A.G + 127) / 128;
+    return tiles * A.KV >= 512 ? pick_fwd<bf16, DP, BN, 2>(A, st) : pick_fwd<bf16, DP, BN, 1>(A, st);
+}
+extern "C" hipError_t dn_scene_attn_fwd_bf16(const SceneAttnArgs *A, hipStream_t st) {
+    const int D = A->D;
+    return D <= 32 ? fwd_rows<32, 64>(*A, st) : D <= 64 ? fwd_rows<64, 64>(*A, st) : D <= 96 ? fwd_rows<96, 64>(*A, st) : fwd_rows<128, 64>(*A, st);
+}
+#else
+extern "C" hipError_t dn_scene_attn_fwd_f32(const SceneAttnArgs *A, hipStream_t st) {
     using namespace sattn;
     const int D = A->D;
-    if (bf) return D <= 32 ? launch_fwd<bf16, 32, 64>(*A, st) : D <= 64 ? launch_fwd<bf16, 64, 64>(*A, st) : launch_fwd<bf16, 128, 64>(*A, st);
-    return D <= 16 ? launch_fwd<float, 16, 64>(*A, st) : D <= 32 ? launch_fwd<float, 32, 64>(*A, st) : D <= 64 ? launch_fwd<float, 64, 64>(*A, st)
-                                                                                              : launch_fwd<float, 128, 32>(*A, st);
+    return D <= 16 ? pick_fwd<float, 16, 64, 1>(*A, st) : D <= 32 ? pick_fwd<float, 32, 64, 1>(*A, st) : D <= 48 ? pick_fwd<float, 48, 32, 1>(*A, st)
+         : D <= 64 ? pick_fwd<float, 64, 32, 1>(*A, st) : D <= 96 ? pick_fwd<float, 96, 32, 1>(*A, st) : pick_fwd<float, 128, 32, 1>(*A, st);
 }
+#endif

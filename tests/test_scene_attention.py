@@ -135,7 +135,7 @@ def test_c_entries_refuse_before_any_launch():
     a = _ops._Attn(**ok)
     assert lib.dagnet_op_attn_bwd(C.byref(a), *[None] * 5, 0, 0, *[None] * 3, 64, 64, None, None, None) == -1 and b"dk and dv" in lib.dagnet_last_error()
     assert lib.dagnet_op_attn_bwd(C.byref(a), *[None] * 5, 0, 0, *[None] * 3, 64, None, None, 64, None) == -1 and b"dslopes" in lib.dagnet_last_error()
-    assert lib.dagnet_op_attn_bwd_workspace(C.byref(a)) == 16
+    assert lib.dagnet_op_attn_bwd_workspace(C.byref(a)) >= 16
     assert lib.dagnet_op_attn_step(C.byref(a), None, None, 1, 8, 1, 0, 0, None, None, None) == -1
     assert lib.dagnet_op_attn_step_workspace(C.byref(a), 0, 8, 1) == 0
     r = [2, 1, 0, 16, 0, 64, 0, 0, None, 0, 0, 64, 0, 1, 64, 64, 4, 0, 0, 64, 0, 0, None, 0, 0, None]
