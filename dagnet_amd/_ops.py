@@ -1675,15 +1675,23 @@ def _addr(t):
 
 def _attn_struct(q, k, v, slopes, pos, k_pos, nk, scale, softcap):
     """q [nq, H, D], k and v [..., KV, D] (their row and head strides are those of the last three dimensions)."""
-    axes = 0 if slopes is None else pos.shape[-1]
-    qs, ks, vs = q.stride(), k.stride(), v.stride()
-    return _Attn(q.data_ptr(), k.data_ptr(), v.data_ptr(), _addr(slopes), _addr(pos), _addr(k_pos), qs[0], qs[1], ks[-3], ks[-2], vs[-3], vs[-2],
-                 q.shape[0], nk, q.shape[1], k.shape[-2], q.shape[2], axes, int(q.dtype == torch.bfloat16), scale, softcap)
+    qs, ks, vs, (n, H, D) = q.stride(), k.stride(), v.stride(), q.shape
+    if slopes is None:
+        sl = qp = kp = None
+        axes = 0
+    else:
+        sl, qp, kp, axes = slopes.data_ptr(), pos.data_ptr(), k_pos.data_ptr(), pos.shape[-1]
+    return _Attn(q.data_ptr(), k.data_ptr(), v.data_ptr(), sl, qp, kp, qs[0], qs[1], ks[-3], ks[-2], vs[-3], vs[-2], n, nk, H, k.shape[-2], D, axes,
+                 q.dtype is torch.bfloat16, scale, softcap)
 
 
-def _on(device):
+_raw_stream = torch._C._cuda_getCurrentRawStream if hasattr(torch._C, "_cuda_getCurrentRawStream") else None
+_same = contextlib.nullcontext()
+
+
+def _on(index: int):
     """The calls launch on the CURRENT device; tensors of another one make it current for the call."""
-    return contextlib.nullcontext() if device.index == torch.cuda.current_device() else torch.cuda.device(device)
+    return _same if index == torch._C._cuda_getDevice() else torch.cuda.device(index)
 
 
 def _heads(t: torch.Tensor) -> torch.Tensor:
@@ -1691,56 +1699,70 @@ def _heads(t: torch.Tensor) -> torch.Tensor:
     return t if t.stride(-1) == 1 or t.shape[-1] == 1 else t.contiguous()
 
 
+def scene_attn(q, k, v, slopes, tables, scale, softcap, pos, k_pos, grad):
+    """dagnet_op_attn_fwd -> out, and with ``grad`` the rows' statistics and the unrounded output (else None, None)."""
+    dev, index = q.device, q.get_device()
+    out = torch.empty(q.shape, dtype=q.dtype, device=dev)
+    lse = o32 = None
+    if grad:
+        lse = torch.empty(q.shape[0] * q.shape[1], dtype=torch.float32, device=dev)
+        o32 = out if q.dtype is torch.float32 else torch.empty(q.shape, dtype=torch.float32, device=dev)
+    a = _attn_struct(q, k, v, slopes, pos, k_pos, k.shape[0], scale, softcap)
+    lib = _lib()
+    with _on(index):
+        _check(lib.dagnet_op_attn_fwd(C.byref(a), tables[0], tables[1], out.data_ptr(), _addr(lse), None if o32 is out else _addr(o32), _raw_stream(index)))
+    return out, lse, o32
+
+
 class SceneAttnFn(torch.autograd.Function):
     """Attention over the rows of a scene (include/dagnet_hip.h, dagnet_op_attn_fwd / _bwd).  ``tables``: layout.tables(device)."""
 
     @staticmethod
     def forward(ctx, q, k, v, slopes, tables, scale, softcap, pos, k_pos):
-        row_lo, row_hi = tables[:2]
-        grad = any(ctx.needs_input_grad[:4])
-        out = torch.empty(q.shape, dtype=q.dtype, device=q.device)
-        lse = torch.empty(q.shape[0] * q.shape[1], dtype=torch.float32, device=q.device) if grad else None
-        o32 = torch.empty(q.shape, dtype=torch.float32, device=q.device) if grad and q.dtype != torch.float32 else None
-        a = _attn_struct(q, k, v, slopes, pos, k_pos, k.shape[0], scale, softcap)
-        with _on(q.device):
-            _check(_lib().dagnet_op_attn_fwd(C.byref(a), row_lo, row_hi, out.data_ptr(), _addr(lse), _addr(o32), _stream(q.device)))
-        if grad:
-            ctx.save_for_backward(q, k, v, slopes, pos, k_pos, lse, out if o32 is None else o32)
-            ctx.meta = (tables, scale, softcap)
+        out, lse, o = scene_attn(q, k, v, slopes, tables, scale, softcap, pos, k_pos, True)
+        if o is out:
+            ctx.save_for_backward(q, k, v, slopes, pos, k_pos, out)
+            o = None
+        else:
+            ctx.save_for_backward(q, k, v, slopes, pos, k_pos)
+        ctx.meta = (tables, scale, softcap, lse, o)
         return out
 
     @staticmethod
     @torch.autograd.function.once_differentiable
     def backward(ctx, dout):
-        q, k, v, slopes, pos, k_pos, lse, o = ctx.saved_tensors
-        tables, scale, softcap = ctx.meta
-        row_lo, row_hi, key_lo, key_hi = tables[:4]
+        tables, scale, softcap, lse, o = ctx.meta
+        q, k, v, slopes, pos, k_pos, *rest = ctx.saved_tensors
+        o = rest[0] if o is None else o
         need_q, need_k, need_v, need_s = ctx.needs_input_grad[:4]
         dout = _heads(dout)
-        dev = q.device
+        dev, index = q.device, q.get_device()
         a = _attn_struct(q, k, v, slopes, pos, k_pos, k.shape[0], scale, softcap)
         dq = torch.empty(q.shape, dtype=q.dtype, device=dev) if need_q or need_s else None
         dk = torch.empty(k.shape, dtype=k.dtype, device=dev) if need_k or need_v else None
         dv = torch.empty(v.shape, dtype=v.dtype, device=dev) if need_k or need_v else None
-        ds = torch.zeros(slopes.shape, dtype=torch.float32, device=dev) if need_s else None
-        with _on(dev):
-            ws = torch.empty(_lib().dagnet_op_attn_bwd_workspace(C.byref(a)), dtype=torch.float32, device=dev)
-            _check(_lib().dagnet_op_attn_bwd(C.byref(a), row_lo, row_hi, key_lo, key_hi, dout.data_ptr(), dout.stride(0), dout.stride(1),
-                                             lse.data_ptr(), o.data_ptr(), ws.data_ptr(), _addr(dq), _addr(dk), _addr(dv), _addr(ds),
-                                             _stream(dev)))
+        ds = torch.empty(slopes.shape, dtype=torch.float32, device=dev) if need_s else None
+        lib, ref = _lib(), C.byref(a)
+        ws = torch.empty(lib.dagnet_op_attn_bwd_workspace(ref), dtype=torch.float32, device=dev)
+        gs = dout.stride()
+        with _on(index):
+            _check(lib.dagnet_op_attn_bwd(ref, *tables[:4], dout.data_ptr(), gs[0], gs[1], lse.data_ptr(), o.data_ptr(), ws.data_ptr(), _addr(dq),
+                                          _addr(dk), _addr(dv), _addr(ds), _raw_stream(index)))
         return dq if need_q else None, dk if need_k else None, dv if need_v else None, ds, None, None, None, None, None
 
 
 def scene_attn_step(q, k, v, k_len, q_ptr, max_rows, slopes, pos, k_pos, scale, softcap):
     """dagnet_op_attn_step: k, v [S, room, KV, D]; q_ptr, k_len int32 device tensors."""
     S, room = k.shape[:2]
-    out = torch.empty(q.shape, dtype=q.dtype, device=q.device)
+    dev, index = q.device, q.get_device()
+    out = torch.empty(q.shape, dtype=q.dtype, device=dev)
     a = _attn_struct(q, k, v, slopes, pos, k_pos, 0, scale, softcap)
-    with _on(q.device):
-        n = _lib().dagnet_op_attn_step_workspace(C.byref(a), S, room, max_rows)
-        ws = torch.empty(n, dtype=torch.float32, device=q.device) if n else None
-        _check(_lib().dagnet_op_attn_step(C.byref(a), q_ptr, k_len.data_ptr(), S, room, max_rows, k.stride(0), v.stride(0), out.data_ptr(),
-                                          _addr(ws), _stream(q.device)))
+    lib, ref = _lib(), C.byref(a)
+    n = lib.dagnet_op_attn_step_workspace(ref, S, room, max_rows)
+    ws = torch.empty(n, dtype=torch.float32, device=dev) if n else None          # of its own: captured calls must not share one
+    with _on(index):
+        _check(lib.dagnet_op_attn_step(ref, q_ptr, k_len.data_ptr(), S, room, max_rows, k.stride(0), v.stride(0), out.data_ptr(), _addr(ws),
+                                       _raw_stream(index)))
     return out
 
 
@@ -1749,14 +1771,22 @@ _POS_TYPES = {torch.float32: 0, torch.int32: 1, torch.int64: 2}
 
 def rotary_apply(q, k, pos, tables, pairs, interleaved, inverse, qo, ko):
     """dagnet_op_rotary: writes qo (and ko); k and ko may be None."""
-    hk = 0 if k is None else k.shape[1]
-    ks, kos = (k.stride(), ko.stride()) if hk else ((0, 0), (0, 0))
-    qs, qos = q.stride(), qo.stride()
-    with _on(q.device):
-        _check(_lib().dagnet_op_rotary(q.shape[0], q.shape[1], hk, q.shape[2], int(q.dtype == torch.bfloat16), q.data_ptr(), qs[0], qs[1],
-                                       _addr(k), ks[0], ks[1], pos.data_ptr(), _POS_TYPES[pos.dtype], pos.shape[1], tables[0], tables[1], pairs,
-                                       int(interleaved), int(inverse), qo.data_ptr(), qos[0], qos[1], _addr(ko), kos[0], kos[1],
-                                       _stream(q.device)))
+    (n, hq, D), qs, qos, index = q.shape, q.stride(), qo.stride(), q.get_device()
+    if k is None:
+        hk, kp, kop, ks, kos = 0, None, None, (0, 0), (0, 0)
+    else:
+        hk, kp, kop, ks, kos = k.shape[1], k.data_ptr(), ko.data_ptr(), k.stride(), ko.stride()
+    with _on(index):
+        _check(_lib().dagnet_op_rotary(n, hq, hk, D, q.dtype is torch.bfloat16, q.data_ptr(), qs[0], qs[1], kp, ks[0], ks[1], pos.data_ptr(),
+                                       _POS_TYPES[pos.dtype], pos.shape[1], tables[0], tables[1], pairs, interleaved, inverse, qo.data_ptr(), qos[0],
+                                       qos[1], kop, kos[0], kos[1], _raw_stream(index)))
+
+
+def rotary_new(q, k, pos, tables, pairs, interleaved, inverse=False):
+    qo = torch.empty(q.shape, dtype=q.dtype, device=q.device)
+    ko = None if k is None else torch.empty(k.shape, dtype=k.dtype, device=k.device)
+    rotary_apply(q, k, pos, tables, pairs, interleaved, inverse, qo, ko)
+    return qo, ko
 
 
 class RotaryFn(torch.autograd.Function):
@@ -1764,21 +1794,14 @@ class RotaryFn(torch.autograd.Function):
 
     @staticmethod
     def forward(ctx, q, k, pos, tables, pairs, interleaved):
-        qo = torch.empty(q.shape, dtype=q.dtype, device=q.device)
-        ko = None if k is None else torch.empty(k.shape, dtype=k.dtype, device=k.device)
-        rotary_apply(q, k, pos, tables, pairs, interleaved, False, qo, ko)
         ctx.save_for_backward(pos)
         ctx.meta = (tables, pairs, interleaved, k is not None)
-        return qo, ko
+        return rotary_new(q, k, pos, tables, pairs, interleaved)
 
     @staticmethod
     @torch.autograd.function.once_differentiable
     def backward(ctx, gq, gk):
         pos, = ctx.saved_tensors
         tables, pairs, interleaved, has_k = ctx.meta
-        gq = _heads(gq)
-        gk = _heads(gk) if has_k else None
-        dq = torch.empty(gq.shape, dtype=gq.dtype, device=gq.device)
-        dk = torch.empty(gk.shape, dtype=gk.dtype, device=gk.device) if has_k else None
-        rotary_apply(gq, gk, pos, tables, pairs, interleaved, True, dq, dk)
+        dq, dk = rotary_new(_heads(gq), _heads(gk) if has_k else None, pos, tables, pairs, interleaved, True)
         return dq, dk, None, None, None, None

@@ -34,15 +34,20 @@ class _Tables:
     def _host(self) -> torch.Tensor:      # pragma: no cover - overridden
         raise NotImplementedError
 
-    def _on(self, device: torch.device):
-        stream = torch.cuda.current_stream(device)
-        got = self._dev.get(device.index)
+    def _addresses(self, t: torch.Tensor) -> tuple:      # pragma: no cover - overridden
+        raise NotImplementedError
+
+    def tables(self, index: int) -> tuple:
+        """-> the addresses of the tables on device ``index``, and the tensor that holds them."""
+        got = self._dev.get(index)
+        stream = _ops._raw_stream(index)
         if got is None:
             if torch.cuda.is_current_stream_capturing():
                 raise DagnetHipError(f"{type(self).__name__}: make it with device=, or call it once, before capturing a graph")
-            got = self._dev[device.index] = (self._host().to(device), stream.cuda_stream)
-        elif got[1] != stream.cuda_stream:
-            got[0].record_stream(stream)       # its memory is not handed on while a kernel of this stream may read it
+            t = self._host().to(torch.device("cuda", index))
+            got = self._dev[index] = (self._addresses(t) + (t,), stream)
+        elif got[1] != stream:
+            got[0][-1].record_stream(torch.cuda.current_stream(index))       # its memory is not handed on while a kernel of this stream may read it
         return got[0]
 
 
@@ -114,7 +119,7 @@ class SceneLayout(_Tables):
         self._tab = np.concatenate([lo, hi, np.searchsorted(hi, keys, side="right"), np.searchsorted(lo, keys, side="right"), q, k]).astype(np.int32)
         self._at, self._k_at = at, keys - np.repeat(k[:-1], n_k)
         if device is not None:
-            self.tables(_device(device))
+            self.tables(_device(device).index)
 
     def row_bounds(self):
         """-> (lo, hi): int32 arrays; row i sees the keys lo[i] <= j < hi[i]."""
@@ -123,22 +128,19 @@ class SceneLayout(_Tables):
     def _host(self):
         return torch.from_numpy(np.concatenate([self._tab, self._at.astype(np.float32).view(np.int32), self._k_at.astype(np.float32).view(np.int32)]))
 
-    def places(self, device):
-        """-> fp32 [nq, 1], [nk, 1]: the places of rows and keys in their scenes, on ``device``."""
-        t = self._on(device)[len(self._tab):].view(torch.float32)
+    def _addresses(self, t):
+        p, n, m = t.data_ptr(), 4 * self.nq, 4 * self.nk
+        return p, p + n, p + 2 * n, p + 2 * n + m, p + 2 * n + 2 * m          # row_lo, row_hi, key_lo, key_hi, ptr
+
+    def places(self, index):
+        """-> fp32 [nq, 1], [nk, 1]: the places of rows and keys in their scenes, on device ``index``."""
+        t = self.tables(index)[-1][len(self._tab):].view(torch.float32)
         return t[:self.nq, None], t[self.nq:, None]
 
-    def tables(self, device):
-        """-> addresses of row_lo, row_hi, key_lo, key_hi and ptr on ``device``, and the tensor that holds them."""
-        t = self._on(device)
-        p, n, m = t.data_ptr(), 4 * self.nq, 4 * self.nk
-        return p, p + n, p + 2 * n, p + 2 * n + m, p + 2 * n + 2 * m, t
 
-
-def _matrix3(t, what, shape=None):
+def _matrix3(t, what):
     if not isinstance(t, torch.Tensor) or t.dim() != 3:
         raise DagnetHipError(f"{what} must be [rows, heads, head_dim]" + (f", got {tuple(t.shape)}" if isinstance(t, torch.Tensor) else ""))
-    return t
 
 
 def _columns(t):
@@ -146,9 +148,10 @@ def _columns(t):
 
 
 def _check_heads(q, k, v):
-    if q.dtype not in _TYPES or k.dtype != q.dtype or v.dtype != q.dtype:
+    dt = q.dtype
+    if dt not in _TYPES or k.dtype is not dt or v.dtype is not dt:
         raise DagnetHipError(f"q, k and v must all be fp32 or all bf16 (got {q.dtype}, {k.dtype}, {v.dtype})")
-    H, D = q.shape[1], q.shape[2]
+    _, H, D = q.shape
     if not 1 <= D <= 128:
         raise DagnetHipError(f"head_dim must be 1 .. 128, got {D}")
     if k.shape != v.shape or k.shape[-1] != D:
@@ -157,10 +160,13 @@ def _check_heads(q, k, v):
         raise DagnetHipError(f"{H} heads are no multiple of {k.shape[-2]} key heads")
 
 
-def _check_device(device, **tensors):
-    for name, t in tensors.items():
-        if t is not None and (not t.is_cuda or t.device != device):
-            raise DagnetHipError(f"{name} lives on {t.device}; every tensor must live on q's ROCm device ({device}); there is no CPU path")
+def _check_device(names, *tensors) -> int:
+    """-> the device index that all of them share."""
+    index = tensors[0].get_device()
+    for i, t in enumerate(tensors):
+        if t is not None and (index < 0 or t.get_device() != index):
+            raise DagnetHipError(f"{names.split()[i]} lives on {t.device}; every tensor must live on q's ROCm device ({tensors[0].device}); there is no CPU path")
+    return index
 
 
 def _numbers(scale, softcap, D):
@@ -218,12 +224,15 @@ def scene_attention(q, k, v, layout: SceneLayout, *, scale: Optional[float] = No
                 raise DagnetHipError(f"pos has {pos.shape[-1]} axes and k_pos {k_pos.shape[-1]}")
         elif k_pos is not None:
             raise DagnetHipError("k_pos without pos")
-    _check_device(q.device, q=q, k=k, v=v, slopes=slopes, pos=pos, k_pos=k_pos)
+    index = _check_device("q k v slopes pos k_pos", q, k, v, slopes, pos, k_pos)
     if slopes is not None:
         slopes = slopes.contiguous()
         if pos is None:
-            pos, k_pos = layout.places(q.device)
-    return _ops.SceneAttnFn.apply(_columns(q), _columns(k), _columns(v), slopes, layout.tables(q.device), scale, softcap, pos, k_pos)
+            pos, k_pos = layout.places(index)
+    q, k, v, tables = _columns(q), _columns(k), _columns(v), layout.tables(index)
+    if torch.is_grad_enabled() and (q.requires_grad or k.requires_grad or v.requires_grad or (slopes is not None and slopes.requires_grad)):
+        return _ops.SceneAttnFn.apply(q, k, v, slopes, tables, scale, softcap, pos, k_pos)
+    return _ops.scene_attn(q, k, v, slopes, tables, scale, softcap, pos, k_pos, False)[0]
 
 
 def scene_attention_step(q, k_cache, v_cache, k_len, layout: SceneLayout, *, scale: Optional[float] = None, softcap: float = 0.0, slopes=None,
@@ -259,9 +268,9 @@ def scene_attention_step(q, k_cache, v_cache, k_len, layout: SceneLayout, *, sca
         if k_pos.shape[-1] != pos.shape[-1]:
             raise DagnetHipError(f"pos has {pos.shape[-1]} axes and k_pos {k_pos.shape[-1]}")
         slopes = slopes.contiguous()
-    _check_device(q.device, q=q, k_cache=k_cache, v_cache=v_cache, k_len=k_len, slopes=slopes, pos=pos, k_pos=k_pos)
-    return _ops.scene_attn_step(_columns(q), _columns(k_cache), _columns(v_cache), k_len.contiguous(), layout.tables(q.device)[4], layout.max_rows,
-                                slopes, pos, k_pos, scale, softcap)
+    index = _check_device("q k_cache v_cache k_len slopes pos k_pos", q, k_cache, v_cache, k_len, slopes, pos, k_pos)
+    return _ops.scene_attn_step(_columns(q), _columns(k_cache), _columns(v_cache), k_len.contiguous(), layout.tables(index)[4], layout.max_rows, slopes, pos,
+                                k_pos, scale, softcap)
 
 
 class RotaryAxes(_Tables):
@@ -282,16 +291,14 @@ class RotaryAxes(_Tables):
         self.freq = np.concatenate([t ** (-np.arange(n, dtype=np.float64) / n) if n else np.zeros(0) for t, n in zip(th, self.pairs)])
         self.axis = np.repeat(np.arange(self.axes, dtype=np.int32), self.pairs)
         if device is not None:
-            self.tables(_device(device))
+            self.tables(_device(device).index)
 
     def _host(self):
         turns = self.freq / (2.0 * math.pi)
         return torch.from_numpy(np.concatenate([turns.view(np.uint8), self.axis.view(np.uint8)]))
 
-    def tables(self, device):
-        """-> addresses of the frequencies (turns per unit, fp64) and axes on ``device``, and the tensor that holds them."""
-        t = self._on(device)
-        return t.data_ptr(), t.data_ptr() + 8 * self.n_pairs, t
+    def _addresses(self, t):
+        return t.data_ptr(), t.data_ptr() + 8 * self.n_pairs                  # turns per unit (fp64), axis
 
 
 def rotary(q, k, pos, axes: RotaryAxes, *, inplace: bool = False):
@@ -300,7 +307,7 @@ def rotary(q, k, pos, axes: RotaryAxes, *, inplace: bool = False):
     fp32 or bf16, any row and head strides.  Differentiable in q and k; inplace=True overwrites them (without gradient)."""
     if not isinstance(axes, RotaryAxes):
         raise DagnetHipError("axes must be RotaryAxes")
-    both = [("q", q)] + ([("k", k)] if k is not None else [])
+    both = (("q", q),) if k is None else (("q", q), ("k", k))
     for name, t in both:
         _matrix3(t, name)
         if t.dtype not in _TYPES or t.dtype != q.dtype:
@@ -318,10 +325,10 @@ def rotary(q, k, pos, axes: RotaryAxes, *, inplace: bool = False):
         for name, t in both:
             if t.stride(-1) != 1 and t.shape[-1] > 1 or any(s == 0 and n > 1 for s, n in zip(t.stride(), t.shape)):
                 raise DagnetHipError(f"rotary(inplace=True): {name} must have unit column stride and rows of its own (strides {t.stride()})")
-    _check_device(q.device, q=q, k=k, pos=pos)
+    tables = axes.tables(_check_device("q k pos", q, k, pos))
     pos = pos.contiguous()
-    tables = axes.tables(q.device)
     if inplace:
         _ops.rotary_apply(q, k, pos, tables, axes.n_pairs, axes.interleaved, False, q, k)
         return q, k
-    return _ops.RotaryFn.apply(_columns(q), None if k is None else _columns(k), pos, tables, axes.n_pairs, axes.interleaved)
+    q, k = _columns(q), None if k is None else _columns(k)
+    return (_ops.RotaryFn.apply if grad else _ops.rotary_new)(q, k, pos, tables, axes.n_pairs, axes.interleaved)

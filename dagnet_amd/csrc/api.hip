@@ -2167,8 +2167,9 @@ extern "C" hipError_t dn_scene_attn_fwd_bf16(const SceneAttnArgs *, hipStream_t)
 extern "C" hipError_t dn_scene_attn_bwd_f32(const SceneAttnArgs *, float *, hipStream_t);
 extern "C" hipError_t dn_scene_attn_bwd_bf16(const SceneAttnArgs *, float *, hipStream_t);
 extern "C" int dn_scene_attn_bwd_parts(int64_t, int64_t, int, int);
-extern "C" hipError_t dn_scene_attn_step(const SceneStepArgs *, int, hipStream_t);
-extern "C" int dn_scene_attn_step_splits(int64_t groups, int room);
+extern "C" hipError_t dn_scene_attn_step_f32(const SceneStepArgs *, hipStream_t);
+extern "C" hipError_t dn_scene_attn_step_bf16(const SceneStepArgs *, hipStream_t);
+extern "C" void dn_scene_attn_step_shape(int64_t, int64_t, int, int, int *, int *, int *);
 extern "C" hipError_t dn_rotary(const RotaryArgs *, int, int, hipStream_t);
 
 // bytes per load that a matrix of rows allows
@@ -2240,6 +2241,7 @@ extern "C" int dagnet_op_attn_bwd(const dagnet_attn *a, const int32_t *row_lo, c
     A.dout = dout; A.do_rs = do_row; A.do_hs = do_head; A.do_vec = attn_vec(dout, do_row, do_head, a->head_dim, size);
     A.lse = const_cast<float *>(lse); A.o32 = const_cast<float *>(o);
     A.delta = workspace; A.dsl = dslopes ? workspace + (int64_t)a->nq * a->n_heads : nullptr;
+    A.o32_vec = attn_vec(o, (int64_t)a->n_heads * a->head_dim, a->head_dim, a->head_dim, 4);
     A.dq = dq; A.dk = dk; A.dv = dv;
     A.parts = attn_parts(a);
     OP_NEED(((int64_t)a->nk + 63) / 64 * A.KV * A.parts <= 0x7fffffffLL && ((int64_t)a->nk * A.KV + 3) / 4 <= 0x7fffffffLL, "too many keys for one launch");
@@ -2251,16 +2253,14 @@ extern "C" int dagnet_op_attn_bwd(const dagnet_attn *a, const int32_t *row_lo, c
     return DAGNET_OK;
 }
 
-static int step_shape(const dagnet_attn *a, int32_t scenes, int32_t room, int32_t max_rows, int *cblocks, int *splits) {
-    *cblocks = (int)(((int64_t)max_rows * (a->n_heads / a->n_kv_heads) + 15) / 16);
-    *splits = dn_scene_attn_step_splits((int64_t)scenes * a->n_kv_heads * (*cblocks), room);
-    return DAGNET_OK;
+static void step_shape(const dagnet_attn *a, int32_t scenes, int32_t room, int32_t max_rows, int *cblocks, int *splits, int *wide) {
+    dn_scene_attn_step_shape((int64_t)max_rows * (a->n_heads / a->n_kv_heads), (int64_t)scenes * a->n_kv_heads, a->head_dim, room, cblocks, splits, wide);
 }
 
 extern "C" int64_t dagnet_op_attn_step_workspace(const dagnet_attn *a, int32_t scenes, int32_t room, int32_t max_rows) {
     if (!a || scenes < 1 || room < 1 || max_rows < 1 || a->n_kv_heads < 1 || a->n_heads < a->n_kv_heads) return 0;
-    int cb, sp;
-    step_shape(a, scenes, room, max_rows, &cb, &sp);
+    int cb, sp, wide;
+    step_shape(a, scenes, room, max_rows, &cb, &sp, &wide);
     return sp == 1 ? 0 : (int64_t)a->nq * a->n_heads * sp * (a->head_dim + 2);
 }
 
@@ -2272,7 +2272,7 @@ extern "C" int dagnet_op_attn_step(const dagnet_attn *a, const int32_t *q_ptr, c
     if (a->nq == 0 || scenes == 0) return DAGNET_OK;
     OP_NEED(max_rows >= 1 && q_ptr && k_len && out && (room == 0 || (a->k && a->v && (!a->axes || a->k_pos))), "bad argument");
     A.q_ptr = q_ptr; A.k_len = k_len; A.scenes = scenes; A.room = room; A.k_ss = k_scene; A.v_ss = v_scene;
-    step_shape(a, scenes, room, max_rows, &A.cblocks, &A.splits);
+    step_shape(a, scenes, room, max_rows, &A.cblocks, &A.splits, &A.wide);
     OP_NEED((int64_t)scenes * a->n_kv_heads * A.cblocks * A.splits <= 0x7fffffffLL, "too many rows for one launch");
     OP_NEED(A.splits == 1 || workspace, "workspace is NULL");
     const int size = a->dtype ? 2 : 4;
@@ -2282,7 +2282,7 @@ extern "C" int dagnet_op_attn_step(const dagnet_attn *a, const int32_t *q_ptr, c
     if (!attn_base(out, size)) A.a.o_vec = 0;
     A.part = workspace;
     A.stat = workspace ? workspace + (int64_t)a->nq * a->n_heads * A.splits * a->head_dim : nullptr;
-    HIP_TRY(dn_scene_attn_step(&A, a->dtype, OP_ST));
+    HIP_TRY(a->dtype ? dn_scene_attn_step_bf16(&A, OP_ST) : dn_scene_attn_step_f32(&A, OP_ST));
     return DAGNET_OK;
 }
 

@@ -30,7 +30,8 @@ struct SceneAttnArgs {
     float scale, cap;
     int32_t parts;                             // of the rows in the dk / dv kernel; part: [parts][dk, dv][nk][KV][D]
     float *part;
-    int32_t q_vec, k_vec, v_vec, do_vec, o_vec;     // bytes per load that strides, base and width allow: 16, 8 or the element
+    int32_t q_vec, k_vec, v_vec, do_vec, o32_vec;   // bytes per load that strides, base and width allow: 16, 8 or the element
+    int32_t o_vec;                                 // results are stored four at a time
 };
 
 namespace sattn {

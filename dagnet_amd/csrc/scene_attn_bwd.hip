@@ -11,41 +11,55 @@
 
 namespace sattn {
 
-// delta[kvh][row G + g] = sum_d do * o; a wave takes 16 (row, head) pairs, four lanes each
+// One chunk of columns of delta = sum_d do o; lane group g of a row takes the chunks at g CH, KD + g CH, .., in this order in both kernels, so that
+// a gradient does not depend on which others are wanted.
+template <typename T> __device__ __forceinline__ float delta_chunk(float sum, const float *o, typename Tr<T>::frag gf, int d, int D, int vec) {
+#pragma unroll
+    for (int i = 0; i < Tr<T>::CH; i += 4) {
+        const f32x4 v = __builtin_bit_cast(f32x4, load_chunk<float>(o, d + i, D, vec));
+#pragma unroll
+        for (int j = 0; j < 4; ++j) sum = fmaf(d + i + j < D ? v[j] : 0.f, d + i + j < D ? to_f(gf[i + j]) : 0.f, sum);
+    }
+    return sum;
+}
+
+// delta[kvh][row G + g], a (row, head) pair to four lanes.  Only where dq is not wanted: the dq kernel has do in registers and computes it on the way.
 template <typename T> __global__ __launch_bounds__(256) void scene_attn_delta_kernel(const SceneAttnArgs A) {
     const int64_t n = (int64_t)A.nq * A.H, i = (int64_t)blockIdx.x * 64 + (threadIdx.x >> 2);
     const int part = threadIdx.x & 3;
+    const int64_t row = min(i, n - 1) / A.H;
+    const int head = (int)(min(i, n - 1) - row * A.H), kvh = head / A.G;
+    const T *g = reinterpret_cast<const T *>(A.dout) + row * A.do_rs + head * A.do_hs;
+    const float *o = A.o32 + (row * A.H + head) * A.D;
     float s = 0.f;
-    if (i < n) {
-        const int64_t row = i / A.H;
-        const int head = (int)(i - row * A.H);
-        const T *g = reinterpret_cast<const T *>(A.dout) + row * A.do_rs + head * A.do_hs;
-        const float *o = A.o32 + i * A.D;
-        for (int d = part; d < A.D; d += 4) s += to_f(g[d]) * o[d];
-    }
+    for (int d = part * Tr<T>::CH; d < A.D; d += Tr<T>::KD) s = delta_chunk<T>(s, o, as_frag<T>(load_chunk<T>(g, d, A.D, A.do_vec)), d, A.D, A.o32_vec);
     s += __shfl_xor(s, 1);
     s += __shfl_xor(s, 2);
-    if (i < n && part == 0) {
-        const int64_t row = i / A.H;
-        const int head = (int)(i - row * A.H), kvh = head / A.G;
-        A.delta[(int64_t)kvh * A.nq * A.G + row * A.G + (head - kvh * A.G)] = s;
-    }
+    if (i < n && part == 0) A.delta[(int64_t)kvh * A.nq * A.G + row * A.G + (head - kvh * A.G)] = s;
 }
 
-// dslopes[h] = sum over the rows of what the dq kernel left per packed row; one workgroup per head, fp64, fixed order
-static __global__ __launch_bounds__(256) void scene_attn_dslope_kernel(int nq, int G, const float *__restrict__ part, float *__restrict__ out) {
-    __shared__ double sh[256];
+// dslopes[h] = sum over the rows of what the dq kernel left per packed row; one workgroup per head, fp64, fixed order, eight loads a thread in
+// flight (a workgroup alone is bound by their latency)
+static __global__ __launch_bounds__(1024) void scene_attn_dslope_kernel(int nq, int G, const float *__restrict__ part, float *__restrict__ out) {
+    __shared__ double sh[16];
     const int h = blockIdx.x, kvh = h / G, g = h - kvh * G;
     const float *p = part + (int64_t)kvh * nq * G + g;
     double s = 0.0;
-    for (int64_t i = threadIdx.x; i < nq; i += 256) s += p[i * G];
-    sh[threadIdx.x] = s;
-    __syncthreads();
-    for (int o = 128; o > 0; o >>= 1) {
-        if ((int)threadIdx.x < o) sh[threadIdx.x] += sh[threadIdx.x + o];
-        __syncthreads();
+    for (int64_t i = threadIdx.x; i < nq; i += 8192) {
+        float v[8];
+#pragma unroll
+        for (int u = 0; u < 8; ++u) v[u] = i + u * 1024 < nq ? p[(i + u * 1024) * G] : 0.f;
+#pragma unroll
+        for (int u = 0; u < 8; ++u) s += v[u];
     }
-    if (threadIdx.x == 0) out[h] = (float)sh[0];
+#pragma unroll
+    for (int o = 32; o > 0; o >>= 1) s += __shfl_xor(s, o);
+    if ((threadIdx.x & 63) == 0) sh[threadIdx.x >> 6] = s;
+    __syncthreads();
+    if (threadIdx.x == 0) {
+        for (int i = 1; i < 16; ++i) s += sh[i];
+        out[h] = (float)s;
+    }
 }
 
 struct Grad { float p, ds, dz, dist; };     // dz without the factor scale
@@ -175,7 +189,6 @@ __global__ __launch_bounds__(256) void scene_attn_dq_kernel(const SceneAttnArgs 
         const int64_t r = r0 + (w * MB + b) * 16 + c;
         s[b] = row_state(A, kvh, r, R);
         lse[b] = A.lse[kvh * R + min(r, R - 1)];
-        delta[b] = A.delta[kvh * R + min(r, R - 1)];
         const T *Q = reinterpret_cast<const T *>(A.q) + s[b].row * A.q_rs + s[b].head * A.q_hs;
         const T *G = reinterpret_cast<const T *>(A.dout) + s[b].row * A.do_rs + s[b].head * A.do_hs;
 #pragma unroll
@@ -183,6 +196,12 @@ __global__ __launch_bounds__(256) void scene_attn_dq_kernel(const SceneAttnArgs 
             qf[b][f] = as_frag<T>(load_chunk<T>(Q, f * X::KD + g * X::CH, A.D, A.q_vec));
             gf[b][f] = as_frag<T>(load_chunk<T>(G, f * X::KD + g * X::CH, A.D, A.do_vec));
         }
+        const float *o = A.o32 + ((int64_t)s[b].row * A.H + s[b].head) * A.D;
+        float sum = 0.f;
+#pragma unroll
+        for (int f = 0; f < NF; ++f) sum = delta_chunk<T>(sum, o, gf[b][f], f * X::KD + g * X::CH, A.D, A.o32_vec);
+        delta[b] = group_sum(sum);
+        if (A.dk && g == 0 && r < R) A.delta[kvh * R + r] = delta[b];
     }
     const int qa = (int)(r0 / A.G), qb = (int)((min(r0 + ROWS, R) - 1) / A.G);
     const int tlo = uniform(max(A.row_lo[qa], 0)), thi = uniform(min(A.row_hi[qb], A.nk));
@@ -540,14 +559,14 @@ template <typename T, int DP, int BN> hipError_t pick_bwd(const SceneAttnArgs &A
 }
 template <typename T> hipError_t run_bwd(const SceneAttnArgs &A, float *dslopes, hipStream_t st) {
     const int64_t n = (int64_t)A.nq * A.H;
-    if (n > 0) hipLaunchKernelGGL((scene_attn_delta_kernel<T>), dim3((unsigned)((n + 63) / 64)), dim3(256), 0, st, A);
+    if (n > 0 && !A.dq) hipLaunchKernelGGL((scene_attn_delta_kernel<T>), dim3((unsigned)((n + 63) / 64)), dim3(256), 0, st, A);
     const int D = A.D;
     hipError_t e;
     if constexpr (sizeof(T) == 2) e = D <= 32 ? pick_bwd<T, 32, 64>(A, st) : D <= 64 ? pick_bwd<T, 64, 64>(A, st) : D <= 96 ? pick_bwd<T, 96, 32>(A, st) : pick_bwd<T, 128, 32>(A, st);
     else e = D <= 16 ? pick_bwd<T, 16, 64>(A, st) : D <= 32 ? pick_bwd<T, 32, 32>(A, st) : D <= 48 ? pick_bwd<T, 48, 32>(A, st) : D <= 64 ? pick_bwd<T, 64, 32>(A, st)
            : D <= 96 ? pick_bwd<T, 96, 32>(A, st) : pick_bwd<T, 128, 32>(A, st);
     if (e != hipSuccess) return e;
-    if (dslopes) hipLaunchKernelGGL(scene_attn_dslope_kernel, dim3(A.H), dim3(256), 0, st, A.nq, A.G, A.dsl, dslopes);
+    if (dslopes) hipLaunchKernelGGL(scene_attn_dslope_kernel, dim3(A.H), dim3(1024), 0, st, A.nq, A.G, A.dsl, dslopes);
     return hipGetLastError();
 }
 

@@ -11,39 +11,57 @@
 
 namespace sattn {
 
-template <typename T, int DP> __global__ __launch_bounds__(256) void scene_attn_step_kernel(const SceneStepArgs A) {
+// CB: blocks of 16 packed rows a workgroup takes at once: K and V fragments then serve all of them.
+template <typename T, int DP, int CB, bool CAP, int AX> __global__ __launch_bounds__(256) void scene_attn_step_kernel(const SceneStepArgs A) {
     using X = Tr<T>;
     using L = Tile<T, DP>;
     constexpr int NF = DP / X::KD, DB = DP / 16, PB = X::KB / 16, NC = X::KB * L::NCH, PER = NC / 64;
-    static_assert(NC % 64 == 0, "tile");
+    constexpr bool PLAIN = !CAP && AX == 0;
+    static_assert(NC % 64 == 0 && X::KB <= 64, "tile");
     __shared__ u32x4 sv[4][NC];
-    __shared__ float sm[4][16], sl[4][16];
+    __shared__ __attribute__((aligned(16))) float sp[4][AX ? AX : 1][X::KB];
+    __shared__ float sm[CB][4][16], sl[CB][4][16];
     const int tid = threadIdx.x, lane = tid & 63, w = tid >> 6, g = lane >> 4, c = lane & 15;
     int64_t id = blockIdx.x;
-    const int cb = (int)(id % A.cblocks);
-    id /= A.cblocks;
+    const int kvh = (int)(id % A.a.KV);
+    id /= A.a.KV;
     const int split = (int)(id % A.splits);
     id /= A.splits;
-    const int kvh = (int)(id % A.a.KV), sc = (int)(id / A.a.KV);
+    const int cb = (int)(id % A.cblocks) * CB, sc = (int)(id / A.cblocks);
     const int q0 = max(A.q_ptr[sc], 0), q1 = min(A.q_ptr[sc + 1], A.a.nq);
     const int64_t n = (int64_t)(q1 - q0) * A.a.G;
-    if (cb * 16 >= n) return;                                       // the whole workgroup
-    const int64_t pr = min((int64_t)cb * 16 + c, n - 1);
-    const int row = q0 + (int)(pr / A.a.G), head = kvh * A.a.G + (int)(pr % A.a.G);
+    if ((int64_t)cb * 16 >= n) return;                              // the whole workgroup
+    const int live = (int)min((int64_t)CB, (n + 15) / 16 - cb);     // blocks with rows in them
     const int len = min(max(A.k_len[sc], 0), A.room);
     const int per = (int)((((int64_t)len + A.splits - 1) / A.splits + 4 * X::KB - 1) / (4 * X::KB)) * (4 * X::KB);   // whole rounds of the four waves
     const int ka = (int)min((int64_t)split * per, (int64_t)len), kz = (int)min((int64_t)ka + per, (int64_t)len);
-    const float slope2 = A.a.axes ? A.a.slopes[head] * LOG2E : 0.f, inv_cap = A.a.cap > 0.f ? 1.f / A.a.cap : 0.f;
-    float qpos[3] = {0.f, 0.f, 0.f};
-    for (int a = 0; a < A.a.axes; ++a) qpos[a] = A.a.qpos[(int64_t)row * A.a.axes + a];
-    const T *Q = reinterpret_cast<const T *>(A.a.q) + row * A.a.q_rs + head * A.a.q_hs;
+    const Score<T, CAP, AX> S(A.a);
+    const bool flip = PLAIN && A.a.scale < 0.f;
+    const float k = flip ? -S.k : S.k;
     const T *K = reinterpret_cast<const T *>(A.a.k) + sc * A.k_ss + kvh * A.a.k_hs, *V = reinterpret_cast<const T *>(A.a.v) + sc * A.v_ss + kvh * A.a.v_hs;
     const float *kpos = A.a.kpos + (int64_t)sc * A.room * A.a.axes;
-    typename X::frag qf[NF];
-#pragma unroll
-    for (int f = 0; f < NF; ++f) qf[f] = as_frag<T>(load_chunk<T>(Q, f * X::KD + g * X::CH, A.a.D, A.a.q_vec));
 
+    int row[CB], head[CB];
+    float slope[CB], qpos[CB][3];
+    typename X::frag qf[CB][NF];
+#pragma unroll
+    for (int b = 0; b < CB; ++b) {
+        const int64_t pr = min((int64_t)(cb + b) * 16 + c, n - 1);
+        row[b] = q0 + (int)(pr / A.a.G);
+        head[b] = kvh * A.a.G + (int)(pr % A.a.G);
+        slope[b] = AX ? A.a.slopes[head[b]] * LOG2E : 0.f;
+#pragma unroll
+        for (int a = 0; a < 3; ++a) qpos[b][a] = a < AX && a < A.a.axes ? A.a.qpos[(int64_t)row[b] * A.a.axes + a] : 0.f;
+        const T *Q = reinterpret_cast<const T *>(A.a.q) + row[b] * A.a.q_rs + head[b] * A.a.q_hs;
+#pragma unroll
+        for (int f = 0; f < NF; ++f) {
+            u32x4 v = load_chunk<T>(Q, f * X::KD + g * X::CH, A.a.D, A.a.q_vec);
+            if (flip) v ^= sizeof(T) == 4 ? 0x80000000u : 0x80008000u;
+            qf[b][f] = as_frag<T>(v);
+        }
+    }
     u32x4 rk[PB][NF], rv[PER];
+    float rp[AX ? AX : 1];
     auto fetch = [&](int k0) {                                      // keys behind the last one stand in as the last one, masked below
 #pragma unroll
         for (int b = 0; b < PB; ++b) {
@@ -56,11 +74,21 @@ template <typename T, int DP> __global__ __launch_bounds__(256) void scene_attn_
             const int e = lane + i * 64;
             rv[i] = load_chunk<T>(V + (int64_t)min(k0 + e / L::NCH, len - 1) * A.a.v_rs, (e % L::NCH) * X::CH, A.a.D, A.a.v_vec);
         }
-    };
-    f32x4 o[DB];
+        if constexpr (AX > 0) {
+            const float *p = kpos + (int64_t)min(k0 + (lane & (X::KB - 1)), len - 1) * A.a.axes;
 #pragma unroll
-    for (int d = 0; d < DB; ++d) o[d] = f32x4{0.f, 0.f, 0.f, 0.f};
-    float m = NEG_INF, l = 0.f;
+            for (int a = 0; a < AX; ++a) rp[a] = a < A.a.axes ? p[a] : 0.f;
+        }
+    };
+    f32x4 o[CB][DB];
+    float m[CB], l[CB];
+#pragma unroll
+    for (int b = 0; b < CB; ++b) {
+        m[b] = NEG_INF;
+        l[b] = 0.f;
+#pragma unroll
+        for (int d = 0; d < DB; ++d) o[b][d] = f32x4{0.f, 0.f, 0.f, 0.f};
+    }
     int k0 = ka + w * X::KB;
     if (k0 < kz) fetch(k0);
     for (; k0 < kz; k0 += 4 * X::KB) {
@@ -69,134 +97,211 @@ template <typename T, int DP> __global__ __launch_bounds__(256) void scene_attn_
             const int e = lane + i * 64;
             sv[w][L::slot(e / L::NCH, e % L::NCH)] = rv[i];
         }
-        f32x4 x[PB];
-        float top = NEG_INF;
+        if constexpr (AX > 0) {
+            if (lane < X::KB) {
 #pragma unroll
-        for (int b = 0; b < PB; ++b) {
-            f32x4 a = {0.f, 0.f, 0.f, 0.f};
+                for (int a = 0; a < AX; ++a) sp[w][a][lane] = rp[a];
+            }
+        }
+        __builtin_amdgcn_fence(__ATOMIC_RELEASE, "wavefront");      // the wave's own LDS writes, before its reads across lanes
+        __builtin_amdgcn_wave_barrier();
+        f32x4 x[CB][PB];
 #pragma unroll
-            for (int f = 0; f < NF; ++f) a = mma(as_frag<T>(rk[b][f]), qf[f], a);
+        for (int b = 0; b < CB; ++b) {
+            if (b >= live) break;
 #pragma unroll
-            for (int i = 0; i < 4; ++i) {
-                const int key = k0 + b * 16 + 4 * g + i;
-                const float y = score2(A.a, a[i], inv_cap, slope2, qpos, kpos + (int64_t)min(key, len - 1) * A.a.axes);
-                x[b][i] = key < kz ? y : NEG_INF;
-                top = fmaxf(top, x[b][i]);
+            for (int j = 0; j < PB; ++j) {
+                x[b][j] = f32x4{0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+                for (int f = 0; f < NF; ++f) x[b][j] = mma(as_frag<T>(rk[j][f]), qf[b][f], x[b][j]);
             }
         }
         if (k0 + 4 * X::KB < kz) fetch(k0 + 4 * X::KB);
-        top = fmaxf(group_max(top), m);
-        const float base = top == NEG_INF ? 0.f : top, corr = exp2_(m - base);
-        m = top;
-        float sum = 0.f;
+        const bool tail = k0 + X::KB > kz;
+        f32x4 px[PB], py[PB], pz[PB];
 #pragma unroll
-        for (int b = 0; b < PB; ++b)
-#pragma unroll
-            for (int i = 0; i < 4; ++i) {
-                x[b][i] = exp2_(x[b][i] - base);
-                sum += x[b][i];
+        for (int j = 0; j < PB; ++j) {
+            if constexpr (AX > 0) px[j] = *reinterpret_cast<const f32x4 *>(&sp[w][0][j * 16 + 4 * g]);
+            if constexpr (AX > 1) {
+                py[j] = *reinterpret_cast<const f32x4 *>(&sp[w][1][j * 16 + 4 * g]);
+                pz[j] = *reinterpret_cast<const f32x4 *>(&sp[w][2][j * 16 + 4 * g]);
             }
-        l = l * corr + sum;
-        const typename X::frag p = pack_p(x, T());
-        __builtin_amdgcn_fence(__ATOMIC_RELEASE, "wavefront");      // the wave's own LDS writes, before its transposed reads
-        __builtin_amdgcn_wave_barrier();
+        }
 #pragma unroll
-        for (int d = 0; d < DB; ++d) o[d] = mma(frag_cols<DP>(sv[w], 0, d, lane, T()), p, o[d] * corr);
+        for (int b = 0; b < CB; ++b) {
+            if (b >= live) break;
+            float top = NEG_INF;
+#pragma unroll
+            for (int j = 0; j < PB; ++j) {
+                if constexpr (!PLAIN) {
+#pragma unroll
+                    for (int i = 0; i < 4; ++i) {
+                        float t, v = S.value(x[b][j][i], t);
+                        if constexpr (AX > 0) v -= slope[b] * S.dist(qpos[b], px[j][i], AX > 1 ? py[j][i] : 0.f, AX > 1 ? pz[j][i] : 0.f);
+                        x[b][j][i] = v;
+                    }
+                }
+                if (tail) {
+#pragma unroll
+                    for (int i = 0; i < 4; ++i) x[b][j][i] = k0 + j * 16 + 4 * g + i < kz ? x[b][j][i] : NEG_INF;
+                }
+#pragma unroll
+                for (int i = 0; i < 4; ++i) top = fmaxf(top, x[b][j][i]);
+            }
+            top = group_max(top);
+            if constexpr (PLAIN) top = top == NEG_INF ? NEG_INF : top * k;
+            if (__any(top > m[b])) {
+                const float nm = fmaxf(top, m[b]), corr = exp2_(m[b] - (nm == NEG_INF ? 0.f : nm));
+                m[b] = nm;
+                l[b] *= corr;
+#pragma unroll
+                for (int d = 0; d < DB; ++d) o[b][d] *= corr;
+            }
+            const float base = m[b] == NEG_INF ? 0.f : m[b];
+            float sum = 0.f;
+#pragma unroll
+            for (int j = 0; j < PB; ++j)
+#pragma unroll
+                for (int i = 0; i < 4; ++i) {
+                    x[b][j][i] = exp2_(PLAIN ? x[b][j][i] * k - base : x[b][j][i] - base);
+                    sum += x[b][j][i];
+                }
+            l[b] += sum;
+        }
+        typename X::frag p[CB];
+#pragma unroll
+        for (int b = 0; b < CB; ++b) p[b] = pack_p(x[b], T());
+#pragma unroll
+        for (int d = 0; d < DB; ++d) {
+            const typename X::frag a = frag_cols<DP>(sv[w], 0, d, lane, T());
+#pragma unroll
+            for (int b = 0; b < CB; ++b)
+                if (b < live) o[b][d] = mma(a, p[b], o[b][d]);
+        }
         __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "wavefront");
         __builtin_amdgcn_wave_barrier();
     }
-    l = group_sum(l);
     // the four waves' parts: statistics first, then the outputs, rescaled, through the waves' V stretches
-    if (g == 0) { sm[w][c] = m; sl[w][c] = l; }
+#pragma unroll
+    for (int b = 0; b < CB; ++b) {
+        l[b] = group_sum(l[b]);
+        if (g == 0) { sm[b][w][c] = m[b]; sl[b][w][c] = l[b]; }
+    }
     __syncthreads();
-    float M = NEG_INF, Lsum = 0.f;
+    float *so = reinterpret_cast<float *>(&sv[0][0]);                // [4 waves][16][DP]
+    static_assert(4 * NC * 4 >= 4 * 16 * DP, "LDS");
 #pragma unroll
-    for (int i = 0; i < 4; ++i) M = fmaxf(M, sm[i][c]);
-    const float base = M == NEG_INF ? 0.f : M;
+    for (int b = 0; b < CB; ++b) {
+        if (b >= live) break;                                        // the same for the whole workgroup
+        float M = NEG_INF, sum = 0.f;
 #pragma unroll
-    for (int i = 0; i < 4; ++i) Lsum += sl[i][c] * exp2_(sm[i][c] - base);
-    const float corr = exp2_(m - base);
-    // [16][DP] floats a wave
-    float *so = reinterpret_cast<float *>(&sv[0][0]);
-    constexpr int CAPF = 4 * NC * 4 / 16;                            // floats of LDS per row
-    constexpr int WAVES = CAPF >= 4 * DP ? 4 : CAPF / DP;            // waves whose outputs fit at once
-    static_assert(WAVES >= 1, "LDS");
-    f32x4 acc[DB];
+        for (int i = 0; i < 4; ++i) M = fmaxf(M, sm[b][i][c]);
+        const float base = M == NEG_INF ? 0.f : M;
 #pragma unroll
-    for (int d = 0; d < DB; ++d) acc[d] = f32x4{0.f, 0.f, 0.f, 0.f};
+        for (int i = 0; i < 4; ++i) sum += sl[b][i][c] * exp2_(sm[b][i][c] - base);
+        const float corr = exp2_(m[b] - base);
+        if (b) __syncthreads();
 #pragma unroll
-    for (int w0 = 0; w0 < 4; w0 += WAVES) {
-        if (w >= w0 && w < w0 + WAVES) {
-#pragma unroll
-            for (int d = 0; d < DB; ++d) *reinterpret_cast<f32x4 *>(so + ((w - w0) * 16 + c) * DP + d * 16 + g * 4) = o[d] * corr;
-        }
+        for (int d = 0; d < DB; ++d) *reinterpret_cast<f32x4 *>(so + (w * 16 + c) * DP + d * 16 + g * 4) = o[b][d] * corr;
         __syncthreads();
-        if (w == 0) {
+        if ((int64_t)(cb + b) * 16 + c >= n) continue;
+        const int64_t item = (int64_t)row[b] * A.a.H + head[b];
+        const float inv = A.splits > 1 ? 1.f : sum == 0.f ? 0.f : 1.f / sum;
 #pragma unroll
-            for (int i = 0; i < WAVES; ++i)
-                if (w0 + i < 4)
+        for (int d = 0; d < DB; ++d) {                               // every wave sums and stores its share of the columns
+            if (d % 4 != w) continue;
+            f32x4 acc = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll
-                    for (int d = 0; d < DB; ++d) acc[d] += *reinterpret_cast<const f32x4 *>(so + (i * 16 + c) * DP + d * 16 + g * 4);
+            for (int i = 0; i < 4; ++i) acc += *reinterpret_cast<const f32x4 *>(so + (i * 16 + c) * DP + d * 16 + g * 4);
+            if (A.splits > 1) store4(A.part + (item * A.splits + split) * A.a.D, acc, d * 16 + g * 4, A.a.D, A.a.D % 4 == 0);
+            else store4(reinterpret_cast<T *>(A.a.out) + item * A.a.D, acc * inv, d * 16 + g * 4, A.a.D, A.a.o_vec != 0);
         }
-        __syncthreads();
-    }
-    if (w != 0 || (int64_t)cb * 16 + c >= n) return;
-    const int64_t item = (int64_t)row * A.a.H + head;
-    if (A.splits == 1) {
-        const float inv = Lsum == 0.f ? 0.f : 1.f / Lsum;
-#pragma unroll
-        for (int d = 0; d < DB; ++d) store4(reinterpret_cast<T *>(A.a.out) + item * A.a.D, acc[d] * inv, d * 16 + g * 4, A.a.D, A.a.o_vec != 0);
-        return;
-    }
-    float *part = A.part + (item * A.splits + split) * A.a.D;
-#pragma unroll
-    for (int d = 0; d < DB; ++d) store4(part, acc[d], d * 16 + g * 4, A.a.D, A.a.D % 4 == 0);
-    if (g == 0) {
-        A.stat[(item * A.splits + split) * 2] = M;
-        A.stat[(item * A.splits + split) * 2 + 1] = Lsum;
+        if (A.splits > 1 && w == 0 && g == 0) {
+            A.stat[(item * A.splits + split) * 2] = M;
+            A.stat[(item * A.splits + split) * 2 + 1] = sum;
+        }
     }
 }
 
-// one wave per (row, head)
-template <typename T> __global__ __launch_bounds__(256) void scene_attn_join_kernel(const SceneStepArgs A) {
-    const int lane = threadIdx.x & 63;
-    const int64_t item = (int64_t)blockIdx.x * 4 + (threadIdx.x >> 6);
-    if (item >= (int64_t)A.a.nq * A.a.H) return;
-    const float *stat = A.stat + item * A.splits * 2, *part = A.part + item * A.splits * A.a.D;
+// The splits of a (row, head) joined: TP threads, 32 of them over the columns (four each), the rest over the splits.
+template <typename T, int TP> __global__ __launch_bounds__(256) void scene_attn_join_kernel(const SceneStepArgs A) {
+    constexpr int IT = 256 / TP, GR = TP / 32;
+    __shared__ f32x4 so[256];
+    __shared__ float sm[256 / 32], sl[256 / 32];
+    const int t = threadIdx.x % TP, it = threadIdx.x / TP, d = (t % 32) * 4, gr = t / 32, D = A.a.D;
+    const int64_t items = (int64_t)A.a.nq * A.a.H, item = min((int64_t)blockIdx.x * IT + it, items - 1);
+    const float *stat = A.stat + item * A.splits * 2, *part = A.part + item * A.splits * D;
+    const int vec = D % 4 == 0 ? 16 : 4;
+    float m = NEG_INF, l = 0.f;
+    f32x4 o = {0.f, 0.f, 0.f, 0.f};
+    for (int i = gr; i < A.splits; i += GR) {
+        const float mi = stat[2 * i], li = stat[2 * i + 1];
+        const f32x4 v = __builtin_bit_cast(f32x4, load_chunk<float>(part + (int64_t)i * D, d, D, vec));
+        const float nm = fmaxf(m, mi), base = nm == NEG_INF ? 0.f : nm, fa = exp2_(m - base), fb = exp2_(mi - base);
+        l = l * fa + li * fb;
+        o = o * fa + v * fb;
+        m = nm;
+    }
+    so[threadIdx.x] = o;
+    if (t % 32 == 0) { sm[threadIdx.x / 32] = m; sl[threadIdx.x / 32] = l; }
+    __syncthreads();
+    if (gr) return;
     float M = NEG_INF;
-    for (int i = 0; i < A.splits; ++i) M = fmaxf(M, stat[2 * i]);
+#pragma unroll
+    for (int i = 0; i < GR; ++i) M = fmaxf(M, sm[it * GR + i]);
     const float base = M == NEG_INF ? 0.f : M;
-    float l = 0.f, o0 = 0.f, o1 = 0.f;
-    for (int i = 0; i < A.splits; ++i) {
-        const float f = exp2_(stat[2 * i] - base);
-        l += f * stat[2 * i + 1];
-        if (lane < A.a.D) o0 += f * part[(int64_t)i * A.a.D + lane];
-        if (lane + 64 < A.a.D) o1 += f * part[(int64_t)i * A.a.D + lane + 64];
+    l = 0.f;
+    o = f32x4{0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+    for (int i = 0; i < GR; ++i) {
+        const float f = exp2_(sm[it * GR + i] - base);
+        l += f * sl[it * GR + i];
+        o += f * so[it * TP + i * 32 + t];
     }
     const float inv = l == 0.f ? 0.f : 1.f / l;
-    T *out = reinterpret_cast<T *>(A.a.out) + item * A.a.D;
-    if (lane < A.a.D) out[lane] = (T)(o0 * inv);
-    if (lane + 64 < A.a.D) out[lane + 64] = (T)(o1 * inv);
+    if ((int64_t)blockIdx.x * IT + it < items) store4(reinterpret_cast<T *>(A.a.out) + item * D, o * inv, d, D, A.a.o_vec != 0);
 }
 
-template <typename T, int DP> hipError_t launch_step(const SceneStepArgs &A, hipStream_t st) {
-    const int64_t blocks = (int64_t)A.scenes * A.a.KV * A.splits * A.cblocks;
-    hipLaunchKernelGGL((scene_attn_step_kernel<T, DP>), dim3((unsigned)blocks), dim3(256), 0, st, A);
-    if (A.splits > 1) hipLaunchKernelGGL((scene_attn_join_kernel<T>), dim3((unsigned)(((int64_t)A.a.nq * A.a.H + 3) / 4)), dim3(256), 0, st, A);
+template <typename T, int DP, int CB, bool CAP, int AX> hipError_t launch_step(const SceneStepArgs &A, hipStream_t st) {
+    const int64_t blocks = (int64_t)A.scenes * A.a.KV * A.splits * A.cblocks, items = (int64_t)A.a.nq * A.a.H;
+    hipLaunchKernelGGL((scene_attn_step_kernel<T, DP, CB, CAP, AX>), dim3((unsigned)blocks), dim3(256), 0, st, A);
+    if (A.splits > 8) hipLaunchKernelGGL((scene_attn_join_kernel<T, 256>), dim3((unsigned)items), dim3(256), 0, st, A);
+    else if (A.splits > 1) hipLaunchKernelGGL((scene_attn_join_kernel<T, 64>), dim3((unsigned)((items + 3) / 4)), dim3(256), 0, st, A);
     return hipGetLastError();
+}
+template <typename T, int DP, int CB> hipError_t pick_step(const SceneStepArgs &A, hipStream_t st) {
+    const int ax = A.a.axes;
+    if (A.a.cap > 0.f) return ax == 0 ? launch_step<T, DP, CB, true, 0>(A, st) : ax == 1 ? launch_step<T, DP, CB, true, 1>(A, st) : launch_step<T, DP, CB, true, 3>(A, st);
+    return ax == 0 ? launch_step<T, DP, CB, false, 0>(A, st) : ax == 1 ? launch_step<T, DP, CB, false, 1>(A, st) : launch_step<T, DP, CB, false, 3>(A, st);
+}
+// row blocks a workgroup takes at once where there are more than one: what the registers hold
+static constexpr int step_blocks(int D) { return D <= 64 ? 4 : 2; }
+template <typename T, int DP> hipError_t step_rows(const SceneStepArgs &A, hipStream_t st) {
+    return A.wide ? pick_step<T, DP, step_blocks(DP)>(A, st) : pick_step<T, DP, 1>(A, st);
 }
 
 }  // namespace sattn
 
-extern "C" hipError_t dn_scene_attn_step(const SceneStepArgs *A, int bf, hipStream_t st) {
+// one object file per type (the Makefile compiles this source twice)
+#ifdef SCENE_ATTN_BF16
+extern "C" hipError_t dn_scene_attn_step_bf16(const SceneStepArgs *A, hipStream_t st) {
     using namespace sattn;
     const int D = A->a.D;
-    if (bf) return D <= 32 ? launch_step<bf16, 32>(*A, st) : D <= 64 ? launch_step<bf16, 64>(*A, st) : launch_step<bf16, 128>(*A, st);
-    return D <= 16 ? launch_step<float, 16>(*A, st) : D <= 32 ? launch_step<float, 32>(*A, st) : D <= 64 ? launch_step<float, 64>(*A, st) : launch_step<float, 128>(*A, st);
+    return D <= 32 ? step_rows<bf16, 32>(*A, st) : D <= 64 ? step_rows<bf16, 64>(*A, st) : step_rows<bf16, 128>(*A, st);
 }
-
-// Splits of the keys: a multiple of the chip's 256 CUs in workgroups (four to a CU), but no split below 256 keys of the cache.
-extern "C" int dn_scene_attn_step_splits(int64_t groups, int room) {
-    const int64_t want = (1024 + groups - 1) / groups, most = (room + 255) / 256;
-    return (int)std::max<int64_t>(1, std::min<int64_t>(std::min(want, most), 64));
+#else
+extern "C" hipError_t dn_scene_attn_step_f32(const SceneStepArgs *A, hipStream_t st) {
+    using namespace sattn;
+    const int D = A->a.D;
+    return D <= 16 ? step_rows<float, 16>(*A, st) : D <= 32 ? step_rows<float, 32>(*A, st) : D <= 64 ? step_rows<float, 64>(*A, st) : step_rows<float, 128>(*A, st);
 }
+// rows: packed rows of the largest scene; kv_scenes: scenes x kv heads.  Splits of the keys: four workgroups to each of the chip's 256 CUs, but
+// no split below 256 keys of the cache.
+extern "C" void dn_scene_attn_step_shape(int64_t rows, int64_t kv_scenes, int D, int room, int *cblocks, int *splits, int *wide) {
+    const int64_t blocks = (rows + 15) / 16, at_once = blocks > 1 ? sattn::step_blocks(D) : 1;
+    *wide = blocks > 1;
+    *cblocks = (int)((blocks + at_once - 1) / at_once);
+    const int64_t groups = kv_scenes * *cblocks, want = (1024 + groups - 1) / groups, most = ((int64_t)room + 255) / 256;
+    *splits = (int)std::max<int64_t>(1, std::min<int64_t>(std::min(want, most), 64));
+}
+#endif
