@@ -2169,7 +2169,7 @@ extern "C" hipError_t dn_scene_attn_bwd_bf16(const SceneAttnArgs *, float *, hip
 extern "C" int dn_scene_attn_bwd_parts(int64_t, int64_t, int, int);
 extern "C" hipError_t dn_scene_attn_step_f32(const SceneStepArgs *, hipStream_t);
 extern "C" hipError_t dn_scene_attn_step_bf16(const SceneStepArgs *, hipStream_t);
-extern "C" void dn_scene_attn_step_shape(int64_t, int64_t, int, int, int *, int *, int *);
+extern "C" void dn_scene_attn_step_shape(int64_t, int64_t, int, int *, int *, int *);
 extern "C" hipError_t dn_rotary(const RotaryArgs *, int, int, hipStream_t);
 
 // bytes per load that a matrix of rows allows
@@ -2254,7 +2254,7 @@ extern "C" int dagnet_op_attn_bwd(const dagnet_attn *a, const int32_t *row_lo, c
 }
 
 static void step_shape(const dagnet_attn *a, int32_t scenes, int32_t room, int32_t max_rows, int *cblocks, int *splits, int *wide) {
-    dn_scene_attn_step_shape((int64_t)max_rows * (a->n_heads / a->n_kv_heads), (int64_t)scenes * a->n_kv_heads, a->head_dim, room, cblocks, splits, wide);
+    dn_scene_attn_step_shape((int64_t)max_rows * (a->n_heads / a->n_kv_heads), (int64_t)scenes * a->n_kv_heads, room, cblocks, splits, wide);
 }
 
 extern "C" int64_t dagnet_op_attn_step_workspace(const dagnet_attn *a, int32_t scenes, int32_t room, int32_t max_rows) {

@@ -107,34 +107,48 @@ template <typename T, int DP> struct Tile {
     static __device__ __forceinline__ int slot(int r, int c) { return r * NCH + (c ^ swz(r)); }
 };
 
-// Fills a tile of ROWS rows with the rows row(r) points to (columns behind D: anything finite that the row holds - the other operand is 0
-// there, or the result is not stored).  vec 16: straight into LDS, 64 lanes x 16 bytes an instruction, the swizzle applied to the
-// source; nothing waits until landed().  Else through registers, done on return.
-template <typename T, int DP, int ROWS, int NT, typename Row> __device__ __forceinline__ void stage(u32x4 *tile, Row row, int D, int vec) {
+// Fills tiles of ROWS rows (columns behind D: anything finite that the row holds - the other operand is 0 there, or the result is not
+// stored).  Loads of 16 bytes go straight into LDS, 64 lanes an instruction, the swizzle applied to the source; nothing waits until landed().
+// Where rows follow each other evenly, a thread's places in a tile are offsets that never change (off[]) on a base that moves from tile to tile:
+// no address arithmetic per tile (it took a third of the plain forward's vector instructions).
+template <typename T, int DP, int ROWS, int NT> struct Stage {
     using L = Tile<T, DP>;
-    constexpr int NC = ROWS * L::NCH, PER = (NC + NT - 1) / NT;
+    static constexpr int NC = ROWS * L::NCH, PER = (NC + NT - 1) / NT;
     static_assert(NC % 64 == 0, "whole waves");
     typedef __attribute__((address_space(3))) void *lp;
     typedef const __attribute__((address_space(1))) void *gp;
-    const int lane = threadIdx.x & 63, w0 = __builtin_amdgcn_readfirstlane(threadIdx.x & ~63);
-    if (vec == 16) {
+    uint32_t off[PER];
+    // span(r): bytes from the tile's first row to row r
+    template <typename Span> __device__ __forceinline__ void offsets(Span span, int D) {
         const int last = (D - 1) / Tr<T>::CH;
 #pragma unroll
         for (int i = 0; i < PER; ++i) {
-            const int s0 = i * NT + w0;
-            if (NC % NT == 0 || s0 < NC) {
-                const int s = s0 + lane, r = s / L::NCH, c = (s % L::NCH) ^ L::swz(r);
-                __builtin_amdgcn_global_load_lds((gp)(row(r) + min(c, last) * Tr<T>::CH), (lp)(tile + s0), 16, 0, 0);
-            }
-        }
-    } else {
-#pragma unroll 1
-        for (int s = threadIdx.x; s < NC; s += NT) {
-            const int r = s / L::NCH, c = (s % L::NCH) ^ L::swz(r);
-            tile[s] = load_chunk<T>(row(r), c * Tr<T>::CH, D, vec);
+            const int s = min(i * NT + (int)threadIdx.x, NC - 1), r = s / L::NCH, c = (s % L::NCH) ^ L::swz(r);
+            off[i] = span(r) + (uint32_t)min(c, last) * 16;
         }
     }
-}
+    // the rows from base on, all of them there
+    __device__ __forceinline__ void even(u32x4 *tile, const T *base) const {
+        const int w0 = __builtin_amdgcn_readfirstlane(threadIdx.x & ~63);
+        const char *p = reinterpret_cast<const char *>(base);
+#pragma unroll
+        for (int i = 0; i < PER; ++i)
+            if (NC % NT == 0 || i * NT + w0 < NC) __builtin_amdgcn_global_load_lds((gp)(p + off[i]), (lp)(tile + i * NT + w0), 16, 0, 0);
+    }
+    // any rows: row(r) points to row r
+    template <typename Row> static __device__ __forceinline__ void any(u32x4 *tile, Row row, int D, int vec) {
+        const int w0 = __builtin_amdgcn_readfirstlane(threadIdx.x & ~63), last = (D - 1) / Tr<T>::CH;
+#pragma unroll 1
+        for (int i = 0; i < PER; ++i) {
+            const int s = i * NT + (int)threadIdx.x, r = s / L::NCH, c = (s % L::NCH) ^ L::swz(r);
+            if (NC % NT != 0 && i * NT + w0 >= NC) break;
+            if (vec == 16) __builtin_amdgcn_global_load_lds((gp)(row(r) + min(c, last) * Tr<T>::CH), (lp)(tile + i * NT + w0), 16, 0, 0);
+            else tile[s] = load_chunk<T>(row(r), c * Tr<T>::CH, D, vec);            // through registers: in LDS on return
+        }
+    }
+};
+// bytes of a tile of rows fit the offsets
+__device__ __forceinline__ bool short_rows(int64_t stride, int rows, int size) { return stride >= 0 && stride * rows * size < (1ll << 31); }
 // this wave's part of every stage() so far is in LDS (a barrier then says so of the workgroup's)
 __device__ __forceinline__ void landed() { __builtin_amdgcn_s_waitcnt(0x0f70); }      // vmcnt(0)
 
@@ -166,37 +180,39 @@ template <int DP> __device__ __forceinline__ bf16x8 frag_cols(const u32x4 *t, in
     return x.f;
 }
 
+typedef __bf16 bf16x2 __attribute__((ext_vector_type(2)));
+__device__ __forceinline__ uint32_t cvt2(float a, float b) {                // one v_cvt_pk_bf16_f32
+    const f32x2 v = {a, b};
+    return __builtin_bit_cast(uint32_t, __builtin_convertvector(v, bf16x2));
+}
+
 // B operand of the second product from score-shaped registers; P and dS are rounded to the inputs' type here and nowhere else
 __device__ __forceinline__ f32x4 pack_p(const f32x4 *p, float) { return p[0]; }
 __device__ __forceinline__ bf16x8 pack_p(const f32x4 *p, bf16) {
-    bf16x8 r;
-#pragma unroll
-    for (int i = 0; i < 4; ++i) { r[i] = (bf16)p[0][i]; r[4 + i] = (bf16)p[1][i]; }
-    return r;
+    const u32x4 r = {cvt2(p[0][0], p[0][1]), cvt2(p[0][2], p[0][3]), cvt2(p[1][0], p[1][1]), cvt2(p[1][2], p[1][3])};
+    return __builtin_bit_cast(bf16x8, r);
 }
-
 // what that rounding left over, rounded in turn: p to 16 bits through two products
 __device__ __forceinline__ bf16x8 pack_rest(const f32x4 *p, bf16x8 hi) {
-    bf16x8 r;
+    const u32x4 h = __builtin_bit_cast(u32x4, hi);
+    u32x4 r;
 #pragma unroll
-    for (int i = 0; i < 4; ++i) { r[i] = (bf16)(p[0][i] - (float)hi[i]); r[4 + i] = (bf16)(p[1][i] - (float)hi[4 + i]); }
-    return r;
+    for (int i = 0; i < 4; ++i)
+        r[i] = cvt2(p[i >> 1][(i & 1) * 2] - __uint_as_float(h[i] << 16), p[i >> 1][(i & 1) * 2 + 1] - __uint_as_float(h[i] & 0xffff0000u));
+    return __builtin_bit_cast(bf16x8, r);
 }
 __device__ __forceinline__ f32x4 pack_rest(const f32x4 *, f32x4 hi) { return hi; }      // fp32 rounds nothing: never used
 
-// tanh to about 1 ulp of fp32: near zero the odd rational [7/6] from the continued fraction x / (1 + x^2 / (3 + x^2 / (5 + ...)))
-// (its next term is below 2^-27 for |x| <= 1), else 1 - 2 / (1 + e^2x), which loses nothing there.
-__device__ __forceinline__ float tanh_(float x) {
-    const float a = fabsf(x);
-    const float e = exp2_(a * (2.f * LOG2E));
-    const float far = 1.f - 2.f * rcp_(1.f + e);
+// tanh to about 1 ulp of fp32: near zero the odd rational [5/4] from the continued fraction x / (1 + x^2 / (3 + x^2 / (5 + ...))) (off by less than
+// 5e-8 of tanh for |x| <= 1), else 1 - 2 / (1 + e^2x), which loses nothing there.
+__device__ __forceinline__ float tanh_near(float x) {
     const float s = x * x;
-    const float n = a * (135135.f + s * (17325.f + s * (378.f + s)));
-    const float d = 135135.f + s * (62370.f + s * (3150.f + s * 28.f));
-    const float near = n * rcp_(d);
-    return copysignf(a < 1.f ? near : far, x);
+    return x * (945.f + s * (105.f + s)) * rcp_(945.f + s * (420.f + s * 15.f));
 }
-
+__device__ __forceinline__ float tanh_(float x) {
+    const float far = 1.f - 2.f * rcp_(1.f + exp2_(fabsf(x) * (2.f * LOG2E)));
+    return fabsf(x) < 1.f ? tanh_near(x) : copysignf(far, x);
+}
 __device__ __forceinline__ float distance(int axes, const float *a, const float *b) {
     const float x = a[0] - b[0];
     if (axes == 1) return fabsf(x);
@@ -218,14 +234,19 @@ __device__ __forceinline__ float wave_sum(float v) {
     for (int o = 32; o > 0; o >>= 1) v += __shfl_xor(v, o);
     return v;
 }
-// over the four lane groups of one column
+// over the four lane groups of one column: v_permlane16_swap of a register with itself puts its rows 0 and 2 (of 16 lanes) in one result and 1 and 3
+// in the other, v_permlane32_swap its halves - vector instructions, where a shuffle goes through LDS
 __device__ __forceinline__ float group_max(float v) {
-    v = fmaxf(v, __shfl_xor(v, 16));
-    return fmaxf(v, __shfl_xor(v, 32));
+    auto a = __builtin_amdgcn_permlane16_swap(__float_as_uint(v), __float_as_uint(v), false, false);
+    v = fmaxf(__uint_as_float(a[0]), __uint_as_float(a[1]));
+    auto b = __builtin_amdgcn_permlane32_swap(__float_as_uint(v), __float_as_uint(v), false, false);
+    return fmaxf(__uint_as_float(b[0]), __uint_as_float(b[1]));
 }
 __device__ __forceinline__ float group_sum(float v) {
-    v += __shfl_xor(v, 16);
-    return v + __shfl_xor(v, 32);
+    auto a = __builtin_amdgcn_permlane16_swap(__float_as_uint(v), __float_as_uint(v), false, false);
+    v = __uint_as_float(a[0]) + __uint_as_float(a[1]);
+    auto b = __builtin_amdgcn_permlane32_swap(__float_as_uint(v), __float_as_uint(v), false, false);
+    return __uint_as_float(b[0]) + __uint_as_float(b[1]);
 }
 
 // Row c of the wave (all four lane groups hold the same), as the kernels keep it per lane.
@@ -251,51 +272,101 @@ __device__ __forceinline__ RowState row_state(const SceneAttnArgs &A, int kvh, i
 }
 
 __device__ __forceinline__ int uniform(int v) { return __builtin_amdgcn_readfirstlane(v); }
+// a value that all lanes share, in a scalar register
+__device__ __forceinline__ float uniform(float v) { return __uint_as_float(__builtin_amdgcn_readfirstlane(__float_as_uint(v))); }
 
-// Coordinate a of a tile's keys, loaded by the first lanes; missing axes are 0.
-template <int AX, int N> struct KeyPos {
-    float r[AX ? AX : 1];
-    __device__ __forceinline__ void fetch(const SceneAttnArgs &A, const float *kpos, int key) {
-        if constexpr (AX > 0)
-            if (threadIdx.x < N) {
-#pragma unroll
-                for (int a = 0; a < AX; ++a) r[a] = a < A.axes ? kpos[(int64_t)key * A.axes + a] : 0.f;
-            }
+// Which tile a workgroup takes, heaviest first in rounds of one workgroup a CU, every other round backwards: a CU that got a heavy tile
+// in one round gets a light one in the next.  (Causal masks: tiles differ by the length of the sequence.)  n: tiles, i: 0 .. n - 1, per: rounds' length.
+__device__ __forceinline__ int64_t snake(int64_t i, int64_t n, int per) {
+    const int64_t r = i / per, in = i - r * per, len = min((int64_t)per, n - r * per);
+    return r * per + (r & 1 ? len - 1 - in : in);
+}
+constexpr int CUS = 256;
+
+// Single values of a tile's N rows (N <= 64) straight into LDS: src is this lane's
+template <int N> __device__ __forceinline__ void stage_values(float *dst, const void *src) {
+    typedef __attribute__((address_space(3))) void *lp;
+    typedef const __attribute__((address_space(1))) void *gp;
+    if ((int)(threadIdx.x & 63) < N) __builtin_amdgcn_global_load_lds((gp)src, (lp)dst, 4, 0, 0);
+}
+// The coordinates of N keys from key on, one array an axis, axis a by wave a; last: the last key there is (it stands in for those behind it)
+template <int AX, int N> __device__ __forceinline__ void stage_positions(float (*dst)[N], const SceneAttnArgs &A, const float *kpos, int key, int last) {
+    const int a = uniform((int)(threadIdx.x >> 6));
+    if (AX > 0 && a < A.axes) stage_values<N>(dst[a], kpos + (int64_t)min(key + (int)(threadIdx.x & 63), last) * A.axes + a);
+}
+// axes that the launch does not have
+template <int AX, int N> __device__ __forceinline__ void clear_positions(float (*dst)[N], int axes) {
+    if constexpr (AX > 0)
+        for (int i = threadIdx.x; i < AX * N; i += 256)
+            if (i / N >= axes) dst[i / N][i % N] = 0.f;
+}
+template <int AX, int N> __device__ __forceinline__ void read_positions(const float (*s)[N], int at, f32x4 &px, f32x4 &py, f32x4 &pz) {
+    if constexpr (AX > 0) px = *reinterpret_cast<const f32x4 *>(&s[0][at]);
+    if constexpr (AX > 1) {
+        py = *reinterpret_cast<const f32x4 *>(&s[1][at]);
+        pz = *reinterpret_cast<const f32x4 *>(&s[2][at]);
     }
-    __device__ __forceinline__ void put(float (*s)[N]) const {
-        if constexpr (AX > 0)
-            if (threadIdx.x < N) {
-#pragma unroll
-                for (int a = 0; a < AX; ++a) s[a][threadIdx.x] = r[a];
-            }
-    }
-};
+}
 
 // Scores in base 2 from raw products, the constants of one launch folded together.  CAP and AX (0, 1, or 3 for two and three
 // coordinates) are compiled in: the kernels are bound by vector instructions per score, not by the products.
-//   cap: t = tanh(raw scale / cap) = 1 - 2 r with r = 1 / (1 + e^2z); x = cap t.  In fp32 near zero through tanh_() (1 - 2 r is off by 2^-24 there
-//   whatever t is); for bf16 that is far below what the operands' type can tell.
-template <typename T, bool CAP, int AX> struct Score {
-    float k, cap2, arg;
-    __device__ __forceinline__ Score(const SceneAttnArgs &A) {
-        k = A.scale * LOG2E;
-        cap2 = A.cap * LOG2E;
-        arg = CAP ? (sizeof(T) == 4 ? A.scale / A.cap : 2.f * LOG2E * A.scale / A.cap) : 0.f;
-    }
-    // x in base 2; t: the tanh (for its derivative)
-    __device__ __forceinline__ float value(float raw, float &t) const {
-        if constexpr (!CAP) return raw * k;
-        else {
-            if constexpr (sizeof(T) == 4) t = tanh_(raw * arg);
-            else t = 1.f - 2.f * rcp_(1.f + exp2_(raw * arg));
-            return cap2 * t;
+// Capped: with s = raw^2 the rational tanh_near() and both factors become raw (k + s (n1 + s n2)) / (1 + s (d1 + s d2)), eight instructions.
+// Scores of a trained model lie well inside the cap, so a wave seldom takes the form for |raw| >= edge.
+template <bool CAP, int AX> struct Score {
+    float k, arg, cap2, inv2, edge, n1, n2, d1, d2;
+    __device__ __forceinline__ Score(const SceneAttnArgs &A) : k(uniform(A.scale * LOG2E)) {
+        if constexpr (CAP) {
+            arg = uniform(A.scale / A.cap);
+            cap2 = uniform(A.cap * LOG2E);
+            inv2 = uniform(1.f / cap2);
+            edge = uniform(1.f / fabsf(arg));
+            const float a2 = arg * arg;
+            n1 = uniform(k * a2 * (105.f / 945.f));
+            n2 = uniform(k * a2 * a2 * (1.f / 945.f));
+            d1 = uniform(a2 * (420.f / 945.f));
+            d2 = uniform(a2 * a2 * (15.f / 945.f));
         }
     }
-    static __device__ __forceinline__ float dist(const float *a, float bx, float by, float bz) {
-        const float x = a[0] - bx;
+    // N vectors of raw products to scores without the distance
+    template <int N> __device__ __forceinline__ void apply(f32x4 *x) const {
+        if constexpr (!CAP) {
+#pragma unroll
+            for (int n = 0; n < N; ++n) x[n] *= k;
+            return;
+        }
+        bool far = false;
+#pragma unroll
+        for (int n = 0; n < N; ++n) far = far || !(fmaxf(fmaxf(fabsf(x[n][0]), fabsf(x[n][1])), fmaxf(fabsf(x[n][2]), fabsf(x[n][3]))) < edge);
+        if (__any(far)) {
+#pragma unroll
+            for (int n = 0; n < N; ++n)
+#pragma unroll
+                for (int i = 0; i < 4; ++i) x[n][i] = cap2 * tanh_(x[n][i] * arg);
+        } else {
+#pragma unroll
+            for (int n = 0; n < N; ++n)
+#pragma unroll
+                for (int i = 0; i < 4; ++i) {
+                    const float s = x[n][i] * x[n][i];
+                    x[n][i] = x[n][i] * fmaf(s, fmaf(s, n2, n1), k) * rcp_(fmaf(s, fmaf(s, d2, d1), 1.f));
+                }
+        }
+    }
+    // 1 - tanh^2 from such a score
+    __device__ __forceinline__ f32x4 slope_of(f32x4 x) const {
+        const f32x4 t = x * inv2;
+        return 1.f - t * t;
+    }
+    static __device__ __forceinline__ float dist(float x, float y, float z) {
         if constexpr (AX == 1) return fabsf(x);
-        const float y = a[1] - by, z = a[2] - bz;
         return __builtin_amdgcn_sqrtf(x * x + y * y + z * z);
+    }
+    // of one row's position to four positions
+    static __device__ __forceinline__ f32x4 dist4(const float *a, f32x4 px, f32x4 py, f32x4 pz) {
+        f32x4 d;
+#pragma unroll
+        for (int i = 0; i < 4; ++i) d[i] = AX == 1 ? fabsf(a[0] - px[i]) : dist(a[0] - px[i], a[1] - py[i], a[2] - pz[i]);
+        return d;
     }
 };
 
@@ -314,10 +385,8 @@ template <typename T> __device__ __forceinline__ void store4(T *p, f32x4 v, int 
         if (d < D) {
             if constexpr (sizeof(T) == 4) *reinterpret_cast<f32x4 *>(p + d) = v;
             else {
-                bf16x4 h;
-#pragma unroll
-                for (int i = 0; i < 4; ++i) h[i] = (bf16)v[i];
-                *reinterpret_cast<bf16x4 *>(p + d) = h;
+                const u32x2 h = {cvt2(v[0], v[1]), cvt2(v[2], v[3])};
+                *reinterpret_cast<u32x2 *>(p + d) = h;
             }
         }
         return;

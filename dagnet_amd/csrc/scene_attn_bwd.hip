@@ -179,8 +179,29 @@ __global__ __launch_bounds__(256) void scene_attn_dq_kernel(const SceneAttnArgs 
     __shared__ __attribute__((aligned(16))) float sp[2][AX ? AX : 1][BN];
     const int tid = threadIdx.x, lane = tid & 63, w = tid >> 6, g = lane >> 4, c = lane & 15;
     const int kvh = (int)(blockIdx.x % A.KV);
-    const int64_t R = (int64_t)A.nq * A.G, r0 = (int64_t)(gridDim.x / A.KV - 1 - blockIdx.x / A.KV) * ROWS;
-    const Score<T, CAP, AX> S(A);
+    const int64_t R = (int64_t)A.nq * A.G, tiles = gridDim.x / A.KV, r0 = (tiles - 1 - snake(blockIdx.x / A.KV, tiles, max(CUS / A.KV, 1))) * ROWS;
+    const Score<CAP, AX> S(A);
+    const int qa = (int)(r0 / A.G), qb = (int)((min(r0 + ROWS, R) - 1) / A.G);
+    const int tlo = uniform(max(A.row_lo[qa], 0)), thi = uniform(min(A.row_hi[qb], A.nk));
+    const T *K = reinterpret_cast<const T *>(A.k) + kvh * A.k_hs, *V = reinterpret_cast<const T *>(A.v) + kvh * A.v_hs;
+    const bool even = A.k_vec == 16 && A.v_vec == 16 && short_rows(A.k_rs, BN, sizeof(T)) && short_rows(A.v_rs, BN, sizeof(T));
+    Stage<T, DP, BN, 256> tk, tv;
+    tk.offsets([&](int r) { return (uint32_t)(r * A.k_rs * sizeof(T)); }, A.D);
+    tv.offsets([&](int r) { return (uint32_t)(r * A.v_rs * sizeof(T)); }, A.D);
+    auto issue = [&](int kb, int buf) {
+        if (even && kb + BN <= thi) {
+            tk.even(sk[buf], K + (int64_t)kb * A.k_rs);
+            tv.even(sv[buf], V + (int64_t)kb * A.v_rs);
+        } else {
+            tk.any(sk[buf], [&](int r) { return K + (int64_t)min(kb + r, thi - 1) * A.k_rs; }, A.D, A.k_vec);
+            tv.any(sv[buf], [&](int r) { return V + (int64_t)min(kb + r, thi - 1) * A.v_rs; }, A.D, A.v_vec);
+        }
+        stage_positions<AX>(sp[buf], A, A.kpos, kb, thi - 1);
+    };
+    if (tlo < thi) issue(tlo, 0);
+    if (tlo + BN < thi) issue(tlo + BN, 1);
+    clear_positions<AX>(sp[0], A.axes);
+    clear_positions<AX>(sp[1], A.axes);
     RowState s[MB];
     float lse[MB], delta[MB];
     typename X::frag qf[MB][NF], gf[MB][NF];
@@ -203,38 +224,23 @@ __global__ __launch_bounds__(256) void scene_attn_dq_kernel(const SceneAttnArgs 
         delta[b] = group_sum(sum);
         if (A.dk && g == 0 && r < R) A.delta[kvh * R + r] = delta[b];
     }
-    const int qa = (int)(r0 / A.G), qb = (int)((min(r0 + ROWS, R) - 1) / A.G);
-    const int tlo = uniform(max(A.row_lo[qa], 0)), thi = uniform(min(A.row_hi[qb], A.nk));
     const int wlo = uniform(__shfl(s[0].lo, 0)), whi = uniform(__shfl(s[MB - 1].hi, 15));
-    int lo_last[MB], hi_first[MB];
-#pragma unroll
-    for (int b = 0; b < MB; ++b) {
-        lo_last[b] = uniform(__shfl(s[b].lo, 15));
-        hi_first[b] = uniform(__shfl(s[b].hi, 0));
-    }
-    const T *K = reinterpret_cast<const T *>(A.k) + kvh * A.k_hs, *V = reinterpret_cast<const T *>(A.v) + kvh * A.v_hs;
-    KeyPos<AX, BN> kp;
-    auto issue = [&](int kb, int buf) {
-        stage<T, DP, BN, 256>(sk[buf], [&](int r) { return K + (int64_t)min(kb + r, thi - 1) * A.k_rs; }, A.D, A.k_vec);
-        stage<T, DP, BN, 256>(sv[buf], [&](int r) { return V + (int64_t)min(kb + r, thi - 1) * A.v_rs; }, A.D, A.v_vec);
-        kp.fetch(A, A.kpos, min(kb + tid, thi - 1));
-    };
+    const int alo = uniform(__shfl(s[MB - 1].lo, 15)), ahi = uniform(__shfl(s[0].hi, 0));
     f32x4 acc[MB][DB];
     Slope sl[MB];
 #pragma unroll
     for (int b = 0; b < MB; ++b)
 #pragma unroll
         for (int d = 0; d < DB; ++d) acc[b][d] = f32x4{0.f, 0.f, 0.f, 0.f};
-    if (tlo < thi) issue(tlo, 0);
+
     int buf = 0;
     for (int kb = tlo; kb < thi; kb += BN, buf ^= 1) {
-        kp.put(sp[buf]);
         landed();
         __syncthreads();
-        if (kb + BN < thi) issue(kb + BN, buf ^ 1);
+        if (kb > tlo && kb + BN < thi) issue(kb + BN, buf ^ 1);
 #pragma unroll
         for (int j = 0; j < BN / X::KB; ++j) {
-            const int k0 = kb + j * X::KB;
+            const int k0 = kb + j * X::KB, at = j * X::KB;
             if (k0 >= whi || k0 + X::KB <= wlo) continue;
             f32x4 x[MB][PB], e[MB][PB];
 #pragma unroll
@@ -243,52 +249,48 @@ __global__ __launch_bounds__(256) void scene_attn_dq_kernel(const SceneAttnArgs 
                 for (int b = 0; b < MB; ++b) x[b][n] = e[b][n] = f32x4{0.f, 0.f, 0.f, 0.f};
 #pragma unroll
                 for (int f = 0; f < NF; ++f) {
-                    const typename X::frag ka = frag_rows<T, DP>(sk[buf], j * X::KB + n * 16, f, lane);
-                    const typename X::frag va = frag_rows<T, DP>(sv[buf], j * X::KB + n * 16, f, lane);
+                    const typename X::frag ka = frag_rows<T, DP>(sk[buf], at + n * 16, f, lane);
+                    const typename X::frag va = frag_rows<T, DP>(sv[buf], at + n * 16, f, lane);
 #pragma unroll
                     for (int b = 0; b < MB; ++b) {
                         x[b][n] = mma(ka, qf[b][f], x[b][n]);
                         e[b][n] = mma(va, gf[b][f], e[b][n]);
                     }
                 }
-                f32x4 px, py, pz;
-                const int at = j * X::KB + n * 16 + 4 * g;
-                if constexpr (AX > 0) px = *reinterpret_cast<const f32x4 *>(&sp[buf][0][at]);
-                if constexpr (AX > 1) {
-                    py = *reinterpret_cast<const f32x4 *>(&sp[buf][1][at]);
-                    pz = *reinterpret_cast<const f32x4 *>(&sp[buf][2][at]);
-                }
+            }
+#pragma unroll
+            for (int b = 0; b < MB; ++b) S.template apply<PB>(x[b]);
+#pragma unroll
+            for (int n = 0; n < PB; ++n) {
+                f32x4 px = {}, py = {}, pz = {};
+                if constexpr (AX > 0) read_positions<AX>(sp[buf], at + n * 16 + 4 * g, px, py, pz);
 #pragma unroll
                 for (int b = 0; b < MB; ++b) {
-                    const bool masked = k0 + n * 16 < lo_last[b] || k0 + n * 16 + 16 > hi_first[b];
-                    f32x4 p, ds, dist;
+                    f32x4 p, ds, dist, t = x[b][n];
+                    p = t - lse[b];
+                    if constexpr (AX > 0) {
+                        dist = S.dist4(s[b].pos, px, py, pz);
+                        p -= s[b].slope * dist;
+                    }
 #pragma unroll
                     for (int i = 0; i < 4; ++i) {
-                        float t = 0.f, v;
-                        if constexpr (!CAP && AX == 0) v = x[b][n][i] * S.k - lse[b];
-                        else v = S.value(x[b][n][i], t) - lse[b];
-                        if constexpr (AX > 0) {
-                            dist[i] = S.dist(s[b].pos, px[i], AX > 1 ? py[i] : 0.f, AX > 1 ? pz[i] : 0.f);
-                            v -= s[b].slope * dist[i];
-                        }
-                        p[i] = exp2_(v);
-                        x[b][n][i] = t;
+                        p[i] = exp2_(p[i]);
+                        ds[i] = e[b][n][i] - delta[b];
                     }
-                    if (masked) {
+                    if (k0 + n * 16 < alo || k0 + n * 16 + 16 > ahi) {       // a masked place is 0, not 0 * inf
 #pragma unroll
                         for (int i = 0; i < 4; ++i) {
-                            const int key = kb + at + i;
-                            p[i] = key >= s[b].lo && key < s[b].hi ? p[i] : 0.f;
-                            e[b][n][i] = key >= s[b].lo && key < s[b].hi ? e[b][n][i] : 0.f;        // 0 * inf
-                            if constexpr (CAP) x[b][n][i] = key >= s[b].lo && key < s[b].hi ? x[b][n][i] : 0.f;
+                            const int key = k0 + n * 16 + 4 * g + i;
+                            const bool seen = key >= s[b].lo && key < s[b].hi;
+                            p[i] = seen ? p[i] : 0.f;
+                            ds[i] = seen ? ds[i] : 0.f;
+                            if constexpr (CAP) t[i] = seen ? t[i] : 0.f;
                         }
                     }
-#pragma unroll
-                    for (int i = 0; i < 4; ++i) ds[i] = p[i] * (e[b][n][i] - delta[b]);
+                    ds *= p;
                     if constexpr (AX > 0)
                         if (A.dsl) sl[b].add(p, ds, dist);
-#pragma unroll
-                    for (int i = 0; i < 4; ++i) e[b][n][i] = CAP ? ds[i] * (1.f - x[b][n][i] * x[b][n][i]) : ds[i];
+                    e[b][n] = CAP ? ds * S.slope_of(t) : ds;
                 }
             }
             typename X::frag z[MB];
@@ -296,7 +298,7 @@ __global__ __launch_bounds__(256) void scene_attn_dq_kernel(const SceneAttnArgs 
             for (int b = 0; b < MB; ++b) z[b] = pack_p(e[b], T());
 #pragma unroll
             for (int d = 0; d < DB; ++d) {
-                const typename X::frag a = frag_cols<DP>(sk[buf], j * X::KB, d, lane, T());
+                const typename X::frag a = frag_cols<DP>(sk[buf], at, d, lane, T());
 #pragma unroll
                 for (int b = 0; b < MB; ++b) acc[b][d] = mma(a, z[b], acc[b][d]);
             }
@@ -335,18 +337,64 @@ __global__ __launch_bounds__(256) void scene_attn_dq_kernel(const SceneAttnArgs 
 // parts > 1: a workgroup takes one part of the rows that see its keys and leaves fp32 sums; scene_attn_dkv_join_kernel adds them.
 // ---------------------------------------------------------------------------------------------------------------------
 template <typename T, int DP, int BM, int MB, bool CAP, int AX>
-__global__ __launch_bounds__(256) void scene_attn_dkv_kernel(const SceneAttnArgs A) {
+__global__ __launch_bounds__(256, DP <= 32 ? 4 : DP <= 96 ? 3 : 2) void scene_attn_dkv_kernel(const SceneAttnArgs A) {
     using X = Tr<T>;
     using L = Tile<T, DP>;
     constexpr int NF = DP / X::KD, DB = DP / 16, PB = X::KB / 16, NC = BM * L::NCH, KEYS = 64 * MB, NV = 5 + AX;
     static_assert(BM % X::KB == 0 && BM <= 64, "tile");
     __shared__ u32x4 sq[2][NC], sg[2][NC];
-    __shared__ __attribute__((aligned(16))) float srow[2][NV][BM];      // lse, delta, slope, lo, hi, position
+    __shared__ __attribute__((aligned(16))) float srow[2][NV][BM];      // lse, delta, lo, hi, slope, position
     const int tid = threadIdx.x, lane = tid & 63, w = tid >> 6, g = lane >> 4, c = lane & 15;
     const int kvh = (int)(blockIdx.x % A.KV), part = (int)(blockIdx.x / A.KV % A.parts);
     const int64_t R = (int64_t)A.nq * A.G;
-    const int k0 = (int)(blockIdx.x / A.KV / A.parts) * KEYS, kw = k0 + w * 16 * MB;
-    const Score<T, CAP, AX> S(A);
+    const int both = A.KV * A.parts, k0 = (int)snake(blockIdx.x / both, gridDim.x / both, max(CUS / both, 1)) * KEYS, kw = k0 + w * 16 * MB;
+    const Score<CAP, AX> S(A);
+    // the packed rows that see the workgroup's keys (this part of them)
+    int64_t ra = (int64_t)max(A.key_lo[k0], 0) * A.G, rb = (int64_t)min(A.key_hi[min(k0 + KEYS - 1, A.nk - 1)], A.nq) * A.G;
+    if (A.parts > 1) {
+        const int64_t per = ((rb - ra + A.parts - 1) / A.parts + BM - 1) / BM * BM;
+        ra += per * part;
+        rb = min(rb, ra + per);
+    }
+    // packed rows start at a row's first head and BM holds whole rows
+    const bool even = BM % A.G == 0 && A.q_vec == 16 && A.do_vec == 16 && short_rows(A.q_rs, BM, sizeof(T)) && short_rows(A.do_rs, BM, sizeof(T)) &&
+                      short_rows(A.q_hs, BM, sizeof(T)) && short_rows(A.do_hs, BM, sizeof(T));
+    Stage<T, DP, BM, 256> tq, tg;
+    tq.offsets([&](int r) { return (uint32_t)((r / A.G * A.q_rs + r % A.G * A.q_hs) * sizeof(T)); }, A.D);
+    tg.offsets([&](int r) { return (uint32_t)((r / A.G * A.do_rs + r % A.G * A.do_hs) * sizeof(T)); }, A.D);
+    auto issue = [&](int64_t rbase, int buf) {              // rows behind the last one: the last one again, masked below
+        auto at = [&](int r, int64_t rs, int64_t hs) {
+            const int64_t rr = min(rbase + r, rb - 1), row = A.G == 1 ? rr : rr / A.G;
+            return row * rs + (kvh * A.G + (rr - row * A.G)) * hs;
+        };
+        const T *Q = reinterpret_cast<const T *>(A.q), *G = reinterpret_cast<const T *>(A.dout);
+        if (even && rbase + BM <= rb) {
+            tq.even(sq[buf], Q + at(0, A.q_rs, A.q_hs));
+            tg.even(sg[buf], G + at(0, A.do_rs, A.do_hs));
+        } else {
+            tq.any(sq[buf], [&](int r) { return Q + at(r, A.q_rs, A.q_hs); }, A.D, A.q_vec);
+            tg.any(sg[buf], [&](int r) { return G + at(r, A.do_rs, A.do_hs); }, A.D, A.do_vec);
+        }
+        const int64_t rr = min(rbase + lane, rb - 1), row = A.G == 1 ? rr : rr / A.G;
+        if (w == 0) {
+            stage_values<BM>(srow[buf][0], A.lse + kvh * R + rr);
+            stage_values<BM>(srow[buf][1], A.delta + kvh * R + rr);
+        } else if (w == 1) {
+            stage_values<BM>(srow[buf][2], A.row_lo + row);
+            stage_values<BM>(srow[buf][3], A.row_hi + row);
+        } else if (AX > 0 && w == 2) {
+            stage_values<BM>(srow[buf][4], A.slopes + kvh * A.G + (rr - row * A.G));
+            stage_values<BM>(srow[buf][5], A.qpos + row * A.axes);
+        } else if (AX > 1) {
+            stage_values<BM>(srow[buf][6], A.qpos + row * A.axes + 1);
+            if (A.axes > 2) stage_values<BM>(srow[buf][NV - 1], A.qpos + row * A.axes + 2);
+        }
+    };
+    if (ra < rb) issue(ra, 0);
+    if (ra + BM < rb) issue(ra + BM, 1);
+    if (AX > 1 && A.axes < 3)
+        for (int i = tid; i < 2 * BM; i += 256) srow[i / BM][NV - 1][i % BM] = 0.f;
+
     typename X::frag kf[MB][NF], vf[MB][NF];
     float kpos[MB][3];
 #pragma unroll
@@ -361,110 +409,79 @@ __global__ __launch_bounds__(256) void scene_attn_dkv_kernel(const SceneAttnArgs
 #pragma unroll
         for (int a = 0; a < 3; ++a) kpos[b][a] = a < AX && a < A.axes ? A.kpos[(int64_t)kk * A.axes + a] : 0.f;
     }
-    // the packed rows that see the workgroup's keys (this part of them), and this wave's
-    int64_t ra = (int64_t)max(A.key_lo[k0], 0) * A.G, rb = (int64_t)min(A.key_hi[min(k0 + KEYS - 1, A.nk - 1)], A.nq) * A.G;
+    // the rows that see a key of this wave
     const int64_t wa = (int64_t)max(A.key_lo[min(kw, A.nk - 1)], 0) * A.G, wb = (int64_t)min(A.key_hi[min(kw + 16 * MB - 1, A.nk - 1)], A.nq) * A.G;
-    if (A.parts > 1) {
-        const int64_t per = ((rb - ra + A.parts - 1) / A.parts + BM - 1) / BM * BM;
-        ra += per * part;
-        rb = min(rb, ra + per);
-    }
-    float extra[NV];
-    auto issue = [&](int64_t rbase, int buf) {
-        auto at = [&](int r, int64_t rs, int64_t hs) {
-            const int64_t rr = min(rbase + r, rb - 1), row = A.G == 1 ? rr : rr / A.G;
-            return row * rs + (kvh * A.G + (rr - row * A.G)) * hs;
-        };
-        stage<T, DP, BM, 256>(sq[buf], [&](int r) { return reinterpret_cast<const T *>(A.q) + at(r, A.q_rs, A.q_hs); }, A.D, A.q_vec);
-        stage<T, DP, BM, 256>(sg[buf], [&](int r) { return reinterpret_cast<const T *>(A.dout) + at(r, A.do_rs, A.do_hs); }, A.D, A.do_vec);
-        if (tid < BM) {
-            const int64_t rr = rbase + tid;
-            const bool in = rr < rb;
-            const RowState s = row_state(A, kvh, rr, R);
-            extra[0] = A.lse[kvh * R + min(rr, rb - 1)];
-            extra[1] = A.delta[kvh * R + min(rr, rb - 1)];
-            extra[2] = s.slope;
-            extra[3] = __int_as_float(in ? s.lo : 0x7fffffff);           // rows behind the last one see nothing
-            extra[4] = __int_as_float(in ? s.hi : 0);
-#pragma unroll
-            for (int a = 0; a < AX; ++a) extra[5 + a] = s.pos[a];
-        }
-    };
     f32x4 dk[MB][DB], dv[MB][DB];
 #pragma unroll
     for (int b = 0; b < MB; ++b)
 #pragma unroll
         for (int d = 0; d < DB; ++d) dk[b][d] = dv[b][d] = f32x4{0.f, 0.f, 0.f, 0.f};
-    if (ra < rb) issue(ra, 0);
+
     int buf = 0;
     for (int64_t rbase = ra; rbase < rb; rbase += BM, buf ^= 1) {
-        if (tid < BM) {
-#pragma unroll
-            for (int i = 0; i < NV; ++i) srow[buf][i][tid] = extra[i];
-        }
         landed();
         __syncthreads();
-        if (rbase + BM < rb) issue(rbase + BM, buf ^ 1);
+        if (rbase > ra && rbase + BM < rb) issue(rbase + BM, buf ^ 1);
 #pragma unroll
         for (int j = 0; j < BM / X::KB; ++j) {
             const int64_t r0 = rbase + j * X::KB;
-            if (r0 >= wb || r0 + X::KB <= wa) continue;
+            const int at = j * X::KB;
+            if (r0 >= wb || r0 + X::KB <= wa || r0 >= rb) continue;
+            // bounds never decrease: the last row has the latest lo, the first the earliest hi
+            const int lo_last = uniform(__float_as_int(srow[buf][2][at + X::KB - 1])), hi_first = uniform(__float_as_int(srow[buf][3][at]));
+            const bool masked = kw < lo_last || kw + 16 * MB > hi_first || r0 + X::KB > rb;
             f32x4 p[MB][PB], z[MB][PB];
 #pragma unroll
             for (int n = 0; n < PB; ++n) {
-                const int at = j * X::KB + n * 16;
 #pragma unroll
                 for (int b = 0; b < MB; ++b) p[b][n] = z[b][n] = f32x4{0.f, 0.f, 0.f, 0.f};
 #pragma unroll
                 for (int f = 0; f < NF; ++f) {
-                    const typename X::frag qa = frag_rows<T, DP>(sq[buf], at, f, lane);
-                    const typename X::frag ga = frag_rows<T, DP>(sg[buf], at, f, lane);
+                    const typename X::frag qa = frag_rows<T, DP>(sq[buf], at + n * 16, f, lane);
+                    const typename X::frag ga = frag_rows<T, DP>(sg[buf], at + n * 16, f, lane);
 #pragma unroll
                     for (int b = 0; b < MB; ++b) {
                         p[b][n] = mma(qa, kf[b][f], p[b][n]);
                         z[b][n] = mma(ga, vf[b][f], z[b][n]);
                     }
                 }
-                auto col = [&](int v) { return *reinterpret_cast<const f32x4 *>(&srow[buf][v][at + 4 * g]); };
+            }
+#pragma unroll
+            for (int b = 0; b < MB; ++b) S.template apply<PB>(p[b]);
+#pragma unroll
+            for (int n = 0; n < PB; ++n) {
+                auto col = [&](int v) { return *reinterpret_cast<const f32x4 *>(&srow[buf][v][at + n * 16 + 4 * g]); };
                 const f32x4 lse = col(0), delta = col(1);
-                f32x4 slope, px, py, pz;
-                if constexpr (AX > 0) { slope = col(2); px = col(5); }
-                if constexpr (AX > 1) { py = col(6); pz = col(7); }
-                // do all 16 rows see all of the block's keys?
-                const int lo_last = uniform(__float_as_int(srow[buf][3][at + 15])), hi_first = uniform(__float_as_int(srow[buf][4][at]));
+                f32x4 slope = {}, px = {}, py = {}, pz = {};
+                if constexpr (AX > 0) {
+                    slope = col(4) * LOG2E;
+                    px = col(5);
+                }
+                if constexpr (AX > 1) {
+                    py = col(6);
+                    pz = col(NV - 1);
+                }
 #pragma unroll
                 for (int b = 0; b < MB; ++b) {
-                    const bool masked = kw + b * 16 < lo_last || kw + b * 16 + 16 > hi_first;
-                    f32x4 t;
+                    f32x4 t = p[b][n];
+                    p[b][n] = t - lse;
+                    if constexpr (AX > 0) p[b][n] -= slope * S.dist4(kpos[b], px, py, pz);
+                    z[b][n] -= delta;
 #pragma unroll
-                    for (int i = 0; i < 4; ++i) {
-                        float v;
-                        t[i] = 0.f;
-                        if constexpr (!CAP && AX == 0) v = p[b][n][i] * S.k - lse[i];
-                        else {
-                            float tt;
-                            v = S.value(p[b][n][i], tt) - lse[i];
-                            if constexpr (CAP) t[i] = tt;
-                        }
-                        if constexpr (AX > 0) v -= slope[i] * S.dist(kpos[b], px[i], AX > 1 ? py[i] : 0.f, AX > 1 ? pz[i] : 0.f);
-                        p[b][n][i] = exp2_(v);
-                    }
-                    if (masked) {
-                        const f32x4 lo = col(3), hi = col(4);
+                    for (int i = 0; i < 4; ++i) p[b][n][i] = exp2_(p[b][n][i]);
+                    if (masked) {                           // a masked place is 0, not 0 * inf
+                        const f32x4 lo = col(2), hi = col(3);
                         const int key = kw + b * 16 + c;
 #pragma unroll
                         for (int i = 0; i < 4; ++i) {
-                            const bool seen = key >= __float_as_int(lo[i]) && key < __float_as_int(hi[i]);
+                            const bool seen = key >= __float_as_int(lo[i]) && key < __float_as_int(hi[i]) && r0 + n * 16 + 4 * g + i < rb;
                             p[b][n][i] = seen ? p[b][n][i] : 0.f;
-                            z[b][n][i] = seen ? z[b][n][i] - delta[i] : 0.f;             // 0 * inf
+                            z[b][n][i] = seen ? z[b][n][i] : 0.f;
                             if constexpr (CAP) t[i] = seen ? t[i] : 0.f;
                         }
-                    } else {
-#pragma unroll
-                        for (int i = 0; i < 4; ++i) z[b][n][i] -= delta[i];
                     }
-#pragma unroll
-                    for (int i = 0; i < 4; ++i) z[b][n][i] *= CAP ? p[b][n][i] * (1.f - t[i] * t[i]) : p[b][n][i];
+                    z[b][n] *= p[b][n];
+                    if constexpr (CAP) z[b][n] *= S.slope_of(t);
                 }
             }
             typename X::frag pf[MB], zf[MB];
@@ -475,8 +492,8 @@ __global__ __launch_bounds__(256) void scene_attn_dkv_kernel(const SceneAttnArgs
             }
 #pragma unroll
             for (int d = 0; d < DB; ++d) {
-                const typename X::frag ga = frag_cols<DP>(sg[buf], j * X::KB, d, lane, T());
-                const typename X::frag qa = frag_cols<DP>(sq[buf], j * X::KB, d, lane, T());
+                const typename X::frag ga = frag_cols<DP>(sg[buf], at, d, lane, T());
+                const typename X::frag qa = frag_cols<DP>(sq[buf], at, d, lane, T());
 #pragma unroll
                 for (int b = 0; b < MB; ++b) {
                     dv[b][d] = mma(ga, pf[b], dv[b][d]);

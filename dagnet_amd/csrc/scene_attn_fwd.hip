@@ -41,9 +41,10 @@ template <typename T> __device__ void row_slow(const SceneAttnArgs &A, int kvh, 
 }
 
 // MB: 16-row blocks per wave.  One (64 rows a workgroup) where the rows would not fill the chip otherwise, two (128 rows) where they do: every K and
-// V fragment read from LDS then serves two products.
-template <typename T, int DP, int BN, int MB, bool CAP, int AX>
-__global__ __launch_bounds__(256) void scene_attn_fwd_kernel(const SceneAttnArgs A) {
+// V fragment read from LDS then serves two products.  EXACT (bf16, for a backward pass): what rounding p left over goes through the second
+// product too, so that o, and delta with it, does not carry that rounding.
+template <typename T, int DP, int BN, int MB, bool CAP, int AX, bool EXACT>
+__global__ __launch_bounds__(256, MB == 2 ? 2 : 3) void scene_attn_fwd_kernel(const SceneAttnArgs A) {
     using X = Tr<T>;
     using L = Tile<T, DP>;
     constexpr int NF = DP / X::KD, NB = BN / 16, DB = DP / 16, PB = X::KB / 16, NC = BN * L::NCH, ROWS = 64 * MB;
@@ -52,11 +53,34 @@ __global__ __launch_bounds__(256) void scene_attn_fwd_kernel(const SceneAttnArgs
     __shared__ __attribute__((aligned(16))) float sp[2][AX ? AX : 1][BN];
     const int tid = threadIdx.x, lane = tid & 63, w = tid >> 6, g = lane >> 4, c = lane & 15;
     const int kvh = (int)(blockIdx.x % A.KV);
-    const int64_t R = (int64_t)A.nq * A.G, r0 = (int64_t)(gridDim.x / A.KV - 1 - blockIdx.x / A.KV) * ROWS;
-    const Score<T, CAP, AX> S(A);
+    const int64_t R = (int64_t)A.nq * A.G, tiles = gridDim.x / A.KV, r0 = (tiles - 1 - snake(blockIdx.x / A.KV, tiles, max(CUS / A.KV, 1))) * ROWS;
+    const Score<CAP, AX> S(A);
     constexpr bool PLAIN = !CAP && AX == 0;                 // scores stay raw until the exponent: 2^(raw k - base) in one fma
     const bool flip = PLAIN && A.scale < 0.f;               // their maximum then needs k >= 0: the sign goes to q
     const float k = flip ? -S.k : S.k;
+
+    // the keys of the workgroup's rows; the first two tiles are on their way before anything else is read
+    const int qa = (int)(r0 / A.G), qb = (int)((min(r0 + ROWS, R) - 1) / A.G);
+    const int tlo = uniform(max(A.row_lo[qa], 0)), thi = uniform(min(A.row_hi[qb], A.nk));
+    const T *K = reinterpret_cast<const T *>(A.k) + kvh * A.k_hs, *V = reinterpret_cast<const T *>(A.v) + kvh * A.v_hs;
+    const bool even = A.k_vec == 16 && A.v_vec == 16 && short_rows(A.k_rs, BN, sizeof(T)) && short_rows(A.v_rs, BN, sizeof(T));
+    Stage<T, DP, BN, 256> tk, tv;
+    tk.offsets([&](int r) { return (uint32_t)(r * A.k_rs * sizeof(T)); }, A.D);
+    tv.offsets([&](int r) { return (uint32_t)(r * A.v_rs * sizeof(T)); }, A.D);
+    auto issue = [&](int kb, int buf) {                     // keys behind the last one: the last one again, masked below
+        if (even && kb + BN <= thi) {
+            tk.even(sk[buf], K + (int64_t)kb * A.k_rs);
+            tv.even(sv[buf], V + (int64_t)kb * A.v_rs);
+        } else {
+            tk.any(sk[buf], [&](int r) { return K + (int64_t)min(kb + r, thi - 1) * A.k_rs; }, A.D, A.k_vec);
+            tv.any(sv[buf], [&](int r) { return V + (int64_t)min(kb + r, thi - 1) * A.v_rs; }, A.D, A.v_vec);
+        }
+        stage_positions<AX>(sp[buf], A, A.kpos, kb, thi - 1);
+    };
+    if (tlo < thi) issue(tlo, 0);
+    if (tlo + BN < thi) issue(tlo + BN, 1);
+    clear_positions<AX>(sp[0], A.axes);
+    clear_positions<AX>(sp[1], A.axes);
 
     RowState s[MB];
     typename X::frag qf[MB][NF];
@@ -71,24 +95,9 @@ __global__ __launch_bounds__(256) void scene_attn_fwd_kernel(const SceneAttnArgs
             qf[b][f] = as_frag<T>(v);
         }
     }
-    // the keys of the workgroup's rows, of this wave's, and those that all rows of a block see
-    const int qa = (int)(r0 / A.G), qb = (int)((min(r0 + ROWS, R) - 1) / A.G);
-    const int tlo = uniform(max(A.row_lo[qa], 0)), thi = uniform(min(A.row_hi[qb], A.nk));
+    // the keys of this wave's rows, and those that all of them see
     const int wlo = uniform(__shfl(s[0].lo, 0)), whi = uniform(__shfl(s[MB - 1].hi, 15));
-    int lo_last[MB], hi_first[MB];
-#pragma unroll
-    for (int b = 0; b < MB; ++b) {
-        lo_last[b] = uniform(__shfl(s[b].lo, 15));
-        hi_first[b] = uniform(__shfl(s[b].hi, 0));
-    }
-    const T *K = reinterpret_cast<const T *>(A.k) + kvh * A.k_hs, *V = reinterpret_cast<const T *>(A.v) + kvh * A.v_hs;
-
-    KeyPos<AX, BN> kp;
-    auto issue = [&](int kb, int buf) {                     // keys behind the last one: the last one again, masked below
-        stage<T, DP, BN, 256>(sk[buf], [&](int r) { return K + (int64_t)min(kb + r, thi - 1) * A.k_rs; }, A.D, A.k_vec);
-        stage<T, DP, BN, 256>(sv[buf], [&](int r) { return V + (int64_t)min(kb + r, thi - 1) * A.v_rs; }, A.D, A.v_vec);
-        kp.fetch(A, A.kpos, min(kb + tid, thi - 1));
-    };
+    const int alo = uniform(__shfl(s[MB - 1].lo, 15)), ahi = uniform(__shfl(s[0].hi, 0));
     f32x4 o[MB][DB];
     float m[MB], l[MB];
 #pragma unroll
@@ -98,26 +107,18 @@ __global__ __launch_bounds__(256) void scene_attn_fwd_kernel(const SceneAttnArgs
 #pragma unroll
         for (int d = 0; d < DB; ++d) o[b][d] = f32x4{0.f, 0.f, 0.f, 0.f};
     }
-    if (tlo < thi) issue(tlo, 0);
+
     int buf = 0;
     for (int kb = tlo; kb < thi; kb += BN, buf ^= 1) {
-        kp.put(sp[buf]);
         landed();
         __syncthreads();                                    // this tile is in LDS, and nobody reads the other one any more
-        if (kb + BN < thi) issue(kb + BN, buf ^ 1);
+        if (kb > tlo && kb + BN < thi) issue(kb + BN, buf ^ 1);
         if (kb >= whi || kb + BN <= wlo) continue;
         f32x4 x[MB][NB];
         float top[MB];
 #pragma unroll
         for (int b = 0; b < MB; ++b) top[b] = NEG_INF;
-#pragma unroll
-        for (int n = 0; n < NB; ++n) {
-            const int k0 = kb + n * 16;
-            if (k0 >= whi || k0 + 16 <= wlo) {
-#pragma unroll
-                for (int b = 0; b < MB; ++b) x[b][n] = f32x4{NEG_INF, NEG_INF, NEG_INF, NEG_INF};
-                continue;
-            }
+        auto products = [&](int n) {
 #pragma unroll
             for (int b = 0; b < MB; ++b) x[b][n] = f32x4{0.f, 0.f, 0.f, 0.f};
 #pragma unroll
@@ -126,32 +127,46 @@ __global__ __launch_bounds__(256) void scene_attn_fwd_kernel(const SceneAttnArgs
 #pragma unroll
                 for (int b = 0; b < MB; ++b) x[b][n] = mma(a, qf[b][f], x[b][n]);
             }
-            f32x4 px, py, pz;
-            if constexpr (AX > 0) px = *reinterpret_cast<const f32x4 *>(&sp[buf][0][n * 16 + 4 * g]);
-            if constexpr (AX > 1) {
-                py = *reinterpret_cast<const f32x4 *>(&sp[buf][1][n * 16 + 4 * g]);
-                pz = *reinterpret_cast<const f32x4 *>(&sp[buf][2][n * 16 + 4 * g]);
-            }
+        };
+        auto scores = [&](int n) {
+            f32x4 px = {}, py = {}, pz = {};
+            if constexpr (AX > 0) read_positions<AX>(sp[buf], n * 16 + 4 * g, px, py, pz);
 #pragma unroll
             for (int b = 0; b < MB; ++b) {
-                if constexpr (!PLAIN) {
+                if constexpr (!PLAIN) S.template apply<1>(&x[b][n]);
+                if constexpr (AX > 0) x[b][n] -= s[b].slope * S.dist4(s[b].pos, px, py, pz);
+            }
+        };
+        if (kb >= alo && kb + BN <= ahi) {                  // every row of the wave sees all of it: no branches between the products
 #pragma unroll
-                    for (int i = 0; i < 4; ++i) {
-                        float t;
-                        float v = S.value(x[b][n][i], t);
-                        if constexpr (AX > 0) v -= s[b].slope * S.dist(s[b].pos, px[i], AX > 1 ? py[i] : 0.f, AX > 1 ? pz[i] : 0.f);
-                        x[b][n][i] = v;
-                    }
+            for (int n = 0; n < NB; ++n) products(n);
+#pragma unroll
+            for (int n = 0; n < NB; ++n) {
+                scores(n);
+#pragma unroll
+                for (int b = 0; b < MB; ++b)
+#pragma unroll
+                    for (int i = 0; i < 4; ++i) top[b] = fmaxf(top[b], x[b][n][i]);
+            }
+        } else {
+#pragma unroll
+            for (int n = 0; n < NB; ++n) {
+                const int k0 = kb + n * 16;
+                if (k0 >= whi || k0 + 16 <= wlo) {
+#pragma unroll
+                    for (int b = 0; b < MB; ++b) x[b][n] = f32x4{NEG_INF, NEG_INF, NEG_INF, NEG_INF};
+                    continue;
                 }
-                if (k0 < lo_last[b] || k0 + 16 > hi_first[b]) {
+                products(n);
+                scores(n);
+#pragma unroll
+                for (int b = 0; b < MB; ++b)
 #pragma unroll
                     for (int i = 0; i < 4; ++i) {
                         const int key = k0 + 4 * g + i;
                         x[b][n][i] = key >= s[b].lo && key < s[b].hi ? x[b][n][i] : NEG_INF;
+                        top[b] = fmaxf(top[b], x[b][n][i]);
                     }
-                }
-#pragma unroll
-                for (int i = 0; i < 4; ++i) top[b] = fmaxf(top[b], x[b][n][i]);
             }
         }
 #pragma unroll
@@ -179,22 +194,28 @@ __global__ __launch_bounds__(256) void scene_attn_fwd_kernel(const SceneAttnArgs
 #pragma unroll
         for (int j = 0; j < NB / PB; ++j) {
             const int k0 = kb + j * X::KB;
-            if (k0 >= whi || k0 + X::KB <= wlo) continue;
+            if (MB == 1 && (k0 >= whi || k0 + X::KB <= wlo)) continue;
             typename X::frag p[MB], rest[MB];
 #pragma unroll
-            for (int b = 0; b < MB; ++b) p[b] = pack_p(&x[b][j * PB], T());
-            const bool exact = sizeof(T) == 2 && A.o32;     // training: what rounding p left over goes through the product too
-            if (exact) {
-#pragma unroll
-                for (int b = 0; b < MB; ++b) rest[b] = pack_rest(&x[b][j * PB], p[b]);
+            for (int b = 0; b < MB; ++b) {
+                p[b] = pack_p(&x[b][j * PB], T());
+                if constexpr (EXACT) rest[b] = pack_rest(&x[b][j * PB], p[b]);
             }
+            constexpr int DU = DB % 2 == 0 ? 2 : 1;         // EXACT: two accumulators in turn, so that no product waits for the one before it
 #pragma unroll
-            for (int d = 0; d < DB; ++d) {
-                const typename X::frag a = frag_cols<DP>(sv[buf], j * X::KB, d, lane, T());
+            for (int d = 0; d < DB; d += DU) {
+                typename X::frag a[DU];
 #pragma unroll
-                for (int b = 0; b < MB; ++b) {
-                    o[b][d] = mma(a, p[b], o[b][d]);
-                    if (exact) o[b][d] = mma(a, rest[b], o[b][d]);
+                for (int u = 0; u < DU; ++u) a[u] = frag_cols<DP>(sv[buf], j * X::KB, d + u, lane, T());
+#pragma unroll
+                for (int u = 0; u < DU; ++u)
+#pragma unroll
+                    for (int b = 0; b < MB; ++b) o[b][d + u] = mma(a[u], p[b], o[b][d + u]);
+                if constexpr (EXACT) {
+#pragma unroll
+                    for (int u = 0; u < DU; ++u)
+#pragma unroll
+                        for (int b = 0; b < MB; ++b) o[b][d + u] = mma(a[u], rest[b], o[b][d + u]);
                 }
             }
         }
@@ -232,7 +253,9 @@ __global__ __launch_bounds__(256) void scene_attn_fwd_kernel(const SceneAttnArgs
 
 template <typename T, int DP, int BN, int MB, bool CAP, int AX> hipError_t launch_fwd(const SceneAttnArgs &A, hipStream_t st) {
     const int64_t tiles = ((int64_t)A.nq * A.G + 64 * MB - 1) / (64 * MB);
-    hipLaunchKernelGGL((scene_attn_fwd_kernel<T, DP, BN, MB, CAP, AX>), dim3((unsigned)(tiles * A.KV)), dim3(256), 0, st, A);
+    const dim3 grid((unsigned)(tiles * A.KV));
+    if (sizeof(T) == 2 && A.o32) hipLaunchKernelGGL((scene_attn_fwd_kernel<T, DP, BN, MB, CAP, AX, sizeof(T) == 2>), grid, dim3(256), 0, st, A);
+    else hipLaunchKernelGGL((scene_attn_fwd_kernel<T, DP, BN, MB, CAP, AX, false>), grid, dim3(256), 0, st, A);
     return hipGetLastError();
 }
 template <typename T, int DP, int BN, int MB> hipError_t pick_fwd(const SceneAttnArgs &A, hipStream_t st) {
@@ -247,7 +270,7 @@ template <typename T, int DP, int BN, int MB> hipError_t pick_fwd(const SceneAtt
 template <int DP, int BN> static hipError_t fwd_rows(const SceneAttnArgs &A, hipStream_t st) {
     using namespace sattn;
     const int64_t tiles = ((int64_t)A.nq * A.G + 127) / 128;
-    return tiles * A.KV >= 512 ? pick_fwd<bf16, DP, BN, 2>(A, st) : pick_fwd<bf16, DP, BN, 1>(A, st);
+    return tiles * A.KV >= 1536 ? pick_fwd<bf16, DP, BN, 2>(A, st) : pick_fwd<bf16, DP, BN, 1>(A, st);
 }
 extern "C" hipError_t dn_scene_attn_fwd_bf16(const SceneAttnArgs *A, hipStream_t st) {
     const int D = A->D;

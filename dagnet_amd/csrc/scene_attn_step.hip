@@ -35,7 +35,7 @@ template <typename T, int DP, int CB, bool CAP, int AX> __global__ __launch_boun
     const int len = min(max(A.k_len[sc], 0), A.room);
     const int per = (int)((((int64_t)len + A.splits - 1) / A.splits + 4 * X::KB - 1) / (4 * X::KB)) * (4 * X::KB);   // whole rounds of the four waves
     const int ka = (int)min((int64_t)split * per, (int64_t)len), kz = (int)min((int64_t)ka + per, (int64_t)len);
-    const Score<T, CAP, AX> S(A.a);
+    const Score<CAP, AX> S(A.a);
     const bool flip = PLAIN && A.a.scale < 0.f;
     const float k = flip ? -S.k : S.k;
     const T *K = reinterpret_cast<const T *>(A.a.k) + sc * A.k_ss + kvh * A.a.k_hs, *V = reinterpret_cast<const T *>(A.a.v) + sc * A.v_ss + kvh * A.a.v_hs;
@@ -118,29 +118,19 @@ template <typename T, int DP, int CB, bool CAP, int AX> __global__ __launch_boun
         }
         if (k0 + 4 * X::KB < kz) fetch(k0 + 4 * X::KB);
         const bool tail = k0 + X::KB > kz;
-        f32x4 px[PB], py[PB], pz[PB];
+        f32x4 px[PB] = {}, py[PB] = {}, pz[PB] = {};
 #pragma unroll
         for (int j = 0; j < PB; ++j) {
-            if constexpr (AX > 0) px[j] = *reinterpret_cast<const f32x4 *>(&sp[w][0][j * 16 + 4 * g]);
-            if constexpr (AX > 1) {
-                py[j] = *reinterpret_cast<const f32x4 *>(&sp[w][1][j * 16 + 4 * g]);
-                pz[j] = *reinterpret_cast<const f32x4 *>(&sp[w][2][j * 16 + 4 * g]);
-            }
+            if constexpr (AX > 0) read_positions<AX>(sp[w], j * 16 + 4 * g, px[j], py[j], pz[j]);
         }
 #pragma unroll
         for (int b = 0; b < CB; ++b) {
             if (b >= live) break;
+            if constexpr (!PLAIN) S.template apply<PB>(x[b]);
             float top = NEG_INF;
 #pragma unroll
             for (int j = 0; j < PB; ++j) {
-                if constexpr (!PLAIN) {
-#pragma unroll
-                    for (int i = 0; i < 4; ++i) {
-                        float t, v = S.value(x[b][j][i], t);
-                        if constexpr (AX > 0) v -= slope[b] * S.dist(qpos[b], px[j][i], AX > 1 ? py[j][i] : 0.f, AX > 1 ? pz[j][i] : 0.f);
-                        x[b][j][i] = v;
-                    }
-                }
+                if constexpr (AX > 0) x[b][j] -= slope[b] * S.dist4(qpos[b], px[j], py[j], pz[j]);
                 if (tail) {
 #pragma unroll
                     for (int i = 0; i < 4; ++i) x[b][j][i] = k0 + j * 16 + 4 * g + i < kz ? x[b][j][i] : NEG_INF;
@@ -275,9 +265,9 @@ template <typename T, int DP, int CB> hipError_t pick_step(const SceneStepArgs &
     return ax == 0 ? launch_step<T, DP, CB, false, 0>(A, st) : ax == 1 ? launch_step<T, DP, CB, false, 1>(A, st) : launch_step<T, DP, CB, false, 3>(A, st);
 }
 // row blocks a workgroup takes at once where there are more than one: what the registers hold
-static constexpr int step_blocks(int D) { return D <= 64 ? 4 : 2; }
+constexpr int STEP_BLOCKS = 2;
 template <typename T, int DP> hipError_t step_rows(const SceneStepArgs &A, hipStream_t st) {
-    return A.wide ? pick_step<T, DP, step_blocks(DP)>(A, st) : pick_step<T, DP, 1>(A, st);
+    return A.wide ? pick_step<T, DP, STEP_BLOCKS>(A, st) : pick_step<T, DP, 1>(A, st);
 }
 
 }  // namespace sattn
@@ -297,8 +287,8 @@ extern "C" hipError_t dn_scene_attn_step_f32(const SceneStepArgs *A, hipStream_t
 }
 // rows: packed rows of the largest scene; kv_scenes: scenes x kv heads.  Splits of the keys: four workgroups to each of the chip's 256 CUs, but
 // no split below 256 keys of the cache.
-extern "C" void dn_scene_attn_step_shape(int64_t rows, int64_t kv_scenes, int D, int room, int *cblocks, int *splits, int *wide) {
-    const int64_t blocks = (rows + 15) / 16, at_once = blocks > 1 ? sattn::step_blocks(D) : 1;
+extern "C" void dn_scene_attn_step_shape(int64_t rows, int64_t kv_scenes, int room, int *cblocks, int *splits, int *wide) {
+    const int64_t blocks = (rows + 15) / 16, at_once = blocks > 1 ? sattn::STEP_BLOCKS : 1;
     *wide = blocks > 1;
     *cblocks = (int)((blocks + at_once - 1) / at_once);
     const int64_t groups = kv_scenes * *cblocks, want = (1024 + groups - 1) / groups, most = ((int64_t)room + 255) / 256;
