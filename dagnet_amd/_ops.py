@@ -28,7 +28,7 @@ OP_EXPORTS = (
     "dagnet_op_bn_moments", "dagnet_op_bn_merge", "dagnet_op_bn_apply", "dagnet_op_bn_bwd_sums", "dagnet_op_bn_bwd_apply",
     "dagnet_op_gat_attn_fwd", "dagnet_op_gat_attn_bwd", "dagnet_op_adj_matmul", "dagnet_op_disposition", "dagnet_op_sumsq",
     "dagnet_op_adam",
-    "dagnet_op_attn_fwd", "dagnet_op_attn_bwd_workspace", "dagnet_op_attn_bwd", "dagnet_op_attn_step_workspace", "dagnet_op_attn_step",
+    "dagnet_op_attn_fwd_workspace", "dagnet_op_attn_fwd", "dagnet_op_attn_bwd_workspace", "dagnet_op_attn_bwd", "dagnet_op_attn_step_workspace", "dagnet_op_attn_step",
     "dagnet_op_rotary",
 )
 
@@ -95,7 +95,9 @@ def _lib():
         lib.dagnet_op_disposition.argtypes = [vp, i32, vp, vp, i64, vp]
         lib.dagnet_op_sumsq.argtypes = [i64, vp, vp, vp]
         lib.dagnet_op_adam.argtypes = [i64, vp, vp, vp, vp, vp, f32, f32, f32, f32, f32, i32, vp]
-        lib.dagnet_op_attn_fwd.argtypes = [vp, vp, vp, vp, vp, vp, vp]
+        lib.dagnet_op_attn_fwd_workspace.argtypes = [vp]
+        lib.dagnet_op_attn_fwd_workspace.restype = i64
+        lib.dagnet_op_attn_fwd.argtypes = [vp, vp, vp, vp, vp, vp, vp, vp]
         lib.dagnet_op_attn_bwd_workspace.argtypes = [vp]
         lib.dagnet_op_attn_bwd_workspace.restype = i64
         lib.dagnet_op_attn_bwd.argtypes = [vp, vp, vp, vp, vp, vp, i64, i64, vp, vp, vp, vp, vp, vp, vp, vp]
@@ -1665,7 +1667,7 @@ class ClipAdam:
 class _Attn(C.Structure):                       # dagnet_attn
     _fields_ = [(n, C.c_void_p) for n in ("q", "k", "v", "slopes", "q_pos", "k_pos")] + \
                [(n, C.c_int64) for n in ("q_row", "q_head", "k_row", "k_head", "v_row", "v_head")] + \
-               [(n, C.c_int32) for n in ("nq", "nk", "n_heads", "n_kv_heads", "head_dim", "axes", "dtype")] + \
+               [(n, C.c_int32) for n in ("nq", "nk", "n_heads", "n_kv_heads", "head_dim", "axes", "dtype", "max_keys", "mean_keys")] + \
                [("scale", C.c_float), ("softcap", C.c_float)]
 
 
@@ -1673,7 +1675,7 @@ def _addr(t):
     return None if t is None else t.data_ptr()
 
 
-def _attn_struct(q, k, v, slopes, pos, k_pos, nk, scale, softcap):
+def _attn_struct(q, k, v, slopes, pos, k_pos, nk, span, scale, softcap):
     """q [nq, H, D], k and v [..., KV, D] (their row and head strides are those of the last three dimensions)."""
     qs, ks, vs, (n, H, D) = q.stride(), k.stride(), v.stride(), q.shape
     if slopes is None:
@@ -1682,7 +1684,7 @@ def _attn_struct(q, k, v, slopes, pos, k_pos, nk, scale, softcap):
     else:
         sl, qp, kp, axes = slopes.data_ptr(), pos.data_ptr(), k_pos.data_ptr(), pos.shape[-1]
     return _Attn(q.data_ptr(), k.data_ptr(), v.data_ptr(), sl, qp, kp, qs[0], qs[1], ks[-3], ks[-2], vs[-3], vs[-2], n, nk, H, k.shape[-2], D, axes,
-                 q.dtype is torch.bfloat16, scale, softcap)
+                 q.dtype is torch.bfloat16, span[0], span[1], scale, softcap)
 
 
 _raw_stream = torch._C._cuda_getCurrentRawStream if hasattr(torch._C, "_cuda_getCurrentRawStream") else None
@@ -1700,18 +1702,20 @@ def _heads(t: torch.Tensor) -> torch.Tensor:
 
 
 def scene_attn(q, k, v, slopes, tables, scale, softcap, pos, k_pos, grad):
-    """dagnet_op_attn_fwd -> out, and with ``grad`` the rows' statistics and the unrounded output (else None, None)."""
-    dev, index = q.device, q.get_device()
-    out = torch.empty(q.shape, dtype=q.dtype, device=dev)
+    """dagnet_op_attn_fwd -> out; with ``grad`` also the call's arguments, the rows' statistics and the unrounded output (else None)."""
+    index, fp32 = q.get_device(), q.dtype is torch.float32
+    out = torch.empty_like(q, memory_format=torch.contiguous_format)
     lse = o32 = None
     if grad:
-        lse = torch.empty(q.shape[0] * q.shape[1], dtype=torch.float32, device=dev)
-        o32 = out if q.dtype is torch.float32 else torch.empty(q.shape, dtype=torch.float32, device=dev)
-    a = _attn_struct(q, k, v, slopes, pos, k_pos, k.shape[0], scale, softcap)
-    lib = _lib()
+        lse = q.new_empty(q.shape[0] * q.shape[1], dtype=torch.float32)
+        o32 = None if fp32 else q.new_empty(q.shape, dtype=torch.float32)
+    a = _attn_struct(q, k, v, slopes, pos, k_pos, k.shape[0], tables[5], scale, softcap)
+    lib, ref = _lib(), C.byref(a)
+    n = lib.dagnet_op_attn_fwd_workspace(ref)
+    ws = q.new_empty(n, dtype=torch.float32) if n else None          # of its own: captured calls must not share one
     with _on(index):
-        _check(lib.dagnet_op_attn_fwd(C.byref(a), tables[0], tables[1], out.data_ptr(), _addr(lse), None if o32 is out else _addr(o32), _raw_stream(index)))
-    return out, lse, o32
+        _check(lib.dagnet_op_attn_fwd(ref, tables[0], tables[1], out.data_ptr(), _addr(lse), _addr(o32), _addr(ws), _raw_stream(index)))
+    return out, a, lse, (out if fp32 else o32) if grad else None
 
 
 class SceneAttnFn(torch.autograd.Function):
@@ -1719,47 +1723,40 @@ class SceneAttnFn(torch.autograd.Function):
 
     @staticmethod
     def forward(ctx, q, k, v, slopes, tables, scale, softcap, pos, k_pos):
-        out, lse, o = scene_attn(q, k, v, slopes, tables, scale, softcap, pos, k_pos, True)
-        if o is out:
-            ctx.save_for_backward(q, k, v, slopes, pos, k_pos, out)
-            o = None
-        else:
-            ctx.save_for_backward(q, k, v, slopes, pos, k_pos)
-        ctx.meta = (tables, scale, softcap, lse, o)
+        out, a, lse, o = scene_attn(q, k, v, slopes, tables, scale, softcap, pos, k_pos, True)
+        # saved: what the call's addresses point to, watched for changes in place; the output too where the backward reads it (fp32)
+        ctx.save_for_backward(q, k, v, slopes, pos, k_pos, out if o is out else None)
+        ctx.meta = (a, _lib().dagnet_op_attn_bwd_workspace(C.byref(a)), tables, lse, None if o is out else o)
         return out
 
     @staticmethod
     @torch.autograd.function.once_differentiable
     def backward(ctx, dout):
-        tables, scale, softcap, lse, o = ctx.meta
-        q, k, v, slopes, pos, k_pos, *rest = ctx.saved_tensors
-        o = rest[0] if o is None else o
+        a, n, tables, lse, o = ctx.meta
+        q, k, v, slopes, _, _, out = ctx.saved_tensors
         need_q, need_k, need_v, need_s = ctx.needs_input_grad[:4]
         dout = _heads(dout)
-        dev, index = q.device, q.get_device()
-        a = _attn_struct(q, k, v, slopes, pos, k_pos, k.shape[0], scale, softcap)
-        dq = torch.empty(q.shape, dtype=q.dtype, device=dev) if need_q or need_s else None
-        dk = torch.empty(k.shape, dtype=k.dtype, device=dev) if need_k or need_v else None
-        dv = torch.empty(v.shape, dtype=v.dtype, device=dev) if need_k or need_v else None
-        ds = torch.empty(slopes.shape, dtype=torch.float32, device=dev) if need_s else None
-        lib, ref = _lib(), C.byref(a)
-        ws = torch.empty(lib.dagnet_op_attn_bwd_workspace(ref), dtype=torch.float32, device=dev)
-        gs = dout.stride()
+        index, gs = q.get_device(), dout.stride()
+        dense = torch.contiguous_format
+        dq = torch.empty_like(q, memory_format=dense) if need_q or need_s else None
+        dk, dv = (torch.empty_like(k, memory_format=dense), torch.empty_like(v, memory_format=dense)) if need_k or need_v else (None, None)
+        ds = torch.empty_like(slopes) if need_s else None
+        ws = lse.new_empty(n)
         with _on(index):
-            _check(lib.dagnet_op_attn_bwd(ref, *tables[:4], dout.data_ptr(), gs[0], gs[1], lse.data_ptr(), o.data_ptr(), ws.data_ptr(), _addr(dq),
-                                          _addr(dk), _addr(dv), _addr(ds), _raw_stream(index)))
+            _check(_lib().dagnet_op_attn_bwd(C.byref(a), *tables[:4], dout.data_ptr(), gs[0], gs[1], lse.data_ptr(), (out if o is None else o).data_ptr(),
+                                             ws.data_ptr(), _addr(dq), _addr(dk), _addr(dv), _addr(ds), _raw_stream(index)))
         return dq if need_q else None, dk if need_k else None, dv if need_v else None, ds, None, None, None, None, None
 
 
 def scene_attn_step(q, k, v, k_len, q_ptr, max_rows, slopes, pos, k_pos, scale, softcap):
     """dagnet_op_attn_step: k, v [S, room, KV, D]; q_ptr, k_len int32 device tensors."""
     S, room = k.shape[:2]
-    dev, index = q.device, q.get_device()
-    out = torch.empty(q.shape, dtype=q.dtype, device=dev)
-    a = _attn_struct(q, k, v, slopes, pos, k_pos, 0, scale, softcap)
+    index = q.get_device()
+    out = torch.empty_like(q, memory_format=torch.contiguous_format)
+    a = _attn_struct(q, k, v, slopes, pos, k_pos, 0, (0, 0), scale, softcap)
     lib, ref = _lib(), C.byref(a)
     n = lib.dagnet_op_attn_step_workspace(ref, S, room, max_rows)
-    ws = torch.empty(n, dtype=torch.float32, device=dev) if n else None          # of its own: captured calls must not share one
+    ws = q.new_empty(n, dtype=torch.float32) if n else None
     with _on(index):
         _check(lib.dagnet_op_attn_step(ref, q_ptr, k_len.data_ptr(), S, room, max_rows, k.stride(0), v.stride(0), out.data_ptr(), _addr(ws),
                                        _raw_stream(index)))
@@ -1783,8 +1780,9 @@ def rotary_apply(q, k, pos, tables, pairs, interleaved, inverse, qo, ko):
 
 
 def rotary_new(q, k, pos, tables, pairs, interleaved, inverse=False):
-    qo = torch.empty(q.shape, dtype=q.dtype, device=q.device)
-    ko = None if k is None else torch.empty(k.shape, dtype=k.dtype, device=k.device)
+    dense = torch.contiguous_format
+    qo = torch.empty_like(q, memory_format=dense)
+    ko = None if k is None else torch.empty_like(k, memory_format=dense)
     rotary_apply(q, k, pos, tables, pairs, interleaved, inverse, qo, ko)
     return qo, ko
 

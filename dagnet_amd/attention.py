@@ -115,6 +115,7 @@ class SceneLayout(_Tables):
         end = np.where(group[scene] > 0, np.maximum((at // g + 1) * g, pre[scene]), n_k[scene])
         lo = k[scene]
         hi = lo + np.clip(end, 0, n_k[scene])
+        self.span = (int((hi - lo).max()), int((hi - lo).mean())) if self.nq else (0, 0)        # keys that a row sees: most, mean
         keys = np.arange(self.nk)
         self._tab = np.concatenate([lo, hi, np.searchsorted(hi, keys, side="right"), np.searchsorted(lo, keys, side="right"), q, k]).astype(np.int32)
         self._at, self._k_at = at, keys - np.repeat(k[:-1], n_k)
@@ -130,7 +131,7 @@ class SceneLayout(_Tables):
 
     def _addresses(self, t):
         p, n, m = t.data_ptr(), 4 * self.nq, 4 * self.nk
-        return p, p + n, p + 2 * n, p + 2 * n + m, p + 2 * n + 2 * m          # row_lo, row_hi, key_lo, key_hi, ptr
+        return p, p + n, p + 2 * n, p + 2 * n + m, p + 2 * n + 2 * m, self.span          # row_lo, row_hi, key_lo, key_hi, ptr
 
     def places(self, index):
         """-> fp32 [nq, 1], [nk, 1]: the places of rows and keys in their scenes, on device ``index``."""

@@ -2167,6 +2167,7 @@ extern "C" hipError_t dn_scene_attn_fwd_bf16(const SceneAttnArgs *, hipStream_t)
 extern "C" hipError_t dn_scene_attn_bwd_f32(const SceneAttnArgs *, float *, hipStream_t);
 extern "C" hipError_t dn_scene_attn_bwd_bf16(const SceneAttnArgs *, float *, hipStream_t);
 extern "C" int dn_scene_attn_bwd_parts(int64_t, int64_t, int, int);
+extern "C" int dn_scene_attn_key_parts(int64_t, int, int, int64_t, int64_t);
 extern "C" hipError_t dn_scene_attn_step_f32(const SceneStepArgs *, hipStream_t);
 extern "C" hipError_t dn_scene_attn_step_bf16(const SceneStepArgs *, hipStream_t);
 extern "C" void dn_scene_attn_step_shape(int64_t, int64_t, int, int *, int *, int *);
@@ -2185,6 +2186,7 @@ static int attn_args(const dagnet_attn *a, SceneAttnArgs *A) {
     OP_NEED(a->head_dim >= 1 && a->head_dim <= 128, "head_dim must be 1 .. 128");
     OP_NEED(a->n_kv_heads >= 1 && a->n_heads >= 1 && a->n_heads % a->n_kv_heads == 0, "n_heads must be a multiple of n_kv_heads");
     OP_NEED(a->nq >= 0 && a->nk >= 0 && a->nq <= 0x7fff0000 && a->nk <= 0x7fff0000, "row counts must be 0 .. 2^31 - 65536");
+    OP_NEED(a->max_keys >= 0 && a->mean_keys >= 0, "max_keys and mean_keys must not be negative");
     OP_NEED(a->axes >= 0 && a->axes <= 3, "axes must be 0 .. 3");
     OP_NEED(a->softcap >= 0.f && a->softcap < INFINITY && a->scale == a->scale && fabsf(a->scale) < INFINITY, "scale and softcap must be finite, softcap not negative");
     OP_NEED(a->nq == 0 || a->q, "null q");
@@ -2208,25 +2210,39 @@ static int attn_args(const dagnet_attn *a, SceneAttnArgs *A) {
 // 4 values at once need a base of that alignment
 static bool attn_base(const void *p, int size) { return reinterpret_cast<uintptr_t>(p) % (4 * size) == 0; }
 
+static bool attn_counts(const dagnet_attn *a) { return a && a->nq >= 0 && a->nk >= 0 && a->n_kv_heads >= 1 && a->n_heads >= a->n_kv_heads && a->head_dim >= 1; }
+static int key_parts(const dagnet_attn *a) { return dn_scene_attn_key_parts(a->nq, a->n_kv_heads, a->n_heads / a->n_kv_heads, a->max_keys, a->mean_keys); }
+static int row_parts(const dagnet_attn *a) { return dn_scene_attn_bwd_parts(a->nq, a->nk, a->n_kv_heads, a->n_heads / a->n_kv_heads); }
+static int64_t up4(int64_t n) { return (n + 3) / 4 * 4; }        // floats to a multiple of 16 bytes
+
+extern "C" int64_t dagnet_op_attn_fwd_workspace(const dagnet_attn *a) {
+    if (!attn_counts(a)) return 0;
+    const int p = key_parts(a);
+    return p == 1 ? 0 : (int64_t)a->nq * a->n_heads * p * (a->head_dim + 2);
+}
 extern "C" int dagnet_op_attn_fwd(const dagnet_attn *a, const int32_t *row_lo, const int32_t *row_hi, void *out, float *lse, float *o32,
-                                  void *stream) {
+                                  float *workspace, void *stream) {
     SceneAttnArgs A;
     if (int rc = attn_args(a, &A)) return rc;
     if (a->nq == 0) return DAGNET_OK;
     OP_NEED(row_lo && row_hi && out && (a->nk == 0 || (a->k && a->v && (!a->axes || a->k_pos))), "null argument");
     A.row_lo = row_lo; A.row_hi = row_hi; A.out = out; A.lse = lse; A.o32 = o32;
+    A.key_parts = key_parts(a);
+    OP_NEED(A.key_parts == 1 || (workspace && attn_base(workspace, 4)), "workspace must be there and 16-byte aligned");
+    A.part = workspace;
+    A.stat = workspace ? workspace + (int64_t)a->nq * a->n_heads * A.key_parts * a->head_dim : nullptr;
     if (!attn_base(out, a->dtype ? 2 : 4) || !attn_base(o32, 4)) A.o_vec = 0;
     HIP_TRY(a->dtype ? dn_scene_attn_fwd_bf16(&A, OP_ST) : dn_scene_attn_fwd_f32(&A, OP_ST));
     return DAGNET_OK;
 }
 
-static int attn_parts(const dagnet_attn *a) { return dn_scene_attn_bwd_parts(a->nq, a->nk, a->n_kv_heads, a->n_heads / a->n_kv_heads); }
+// delta | dsl | parts of dq | their sums for dslope | parts of dk and dv
 extern "C" int64_t dagnet_op_attn_bwd_workspace(const dagnet_attn *a) {
-    if (!a || a->nq < 0 || a->nk < 0 || a->n_kv_heads < 1 || a->n_heads < a->n_kv_heads || a->head_dim < 1) return 0;
-    const int parts = attn_parts(a);
-    return 2 * (int64_t)a->nq * a->n_heads + 3 + (parts > 1 ? 2 * (int64_t)parts * a->nk * a->n_kv_heads * a->head_dim : 0);
+    if (!attn_counts(a)) return 0;
+    const int64_t items = (int64_t)a->nq * a->n_heads, keys = (int64_t)a->nk * a->n_kv_heads * a->head_dim;
+    const int kp = key_parts(a), rp = row_parts(a);
+    return up4(2 * items) + (kp > 1 ? up4(items * kp * a->head_dim) + up4(items * kp * 3) : 0) + (rp > 1 ? 2 * rp * keys : 0);
 }
-
 extern "C" int dagnet_op_attn_bwd(const dagnet_attn *a, const int32_t *row_lo, const int32_t *row_hi, const int32_t *key_lo,
                                   const int32_t *key_hi, const void *dout, int64_t do_row, int64_t do_head, const float *lse, const float *o,
                                   float *workspace, void *dq, void *dk, void *dv, float *dslopes, void *stream) {
@@ -2237,18 +2253,25 @@ extern "C" int dagnet_op_attn_bwd(const dagnet_attn *a, const int32_t *row_lo, c
     const int size = a->dtype ? 2 : 4;
     OP_NEED(a->nq == 0 || (row_lo && row_hi && dout && lse && o && workspace), "null argument");
     OP_NEED(a->nk == 0 || (a->k && a->v && (!dk || (key_lo && key_hi)) && (!a->axes || a->k_pos)), "null argument");
+    OP_NEED(attn_base(workspace, 4), "workspace must be 16-byte aligned");
+    const int64_t items = (int64_t)a->nq * a->n_heads;
     A.row_lo = row_lo; A.row_hi = row_hi; A.key_lo = key_lo; A.key_hi = key_hi;
     A.dout = dout; A.do_rs = do_row; A.do_hs = do_head; A.do_vec = attn_vec(dout, do_row, do_head, a->head_dim, size);
     A.lse = const_cast<float *>(lse); A.o32 = const_cast<float *>(o);
-    A.delta = workspace; A.dsl = dslopes ? workspace + (int64_t)a->nq * a->n_heads : nullptr;
     A.o32_vec = attn_vec(o, (int64_t)a->n_heads * a->head_dim, a->head_dim, a->head_dim, 4);
     A.dq = dq; A.dk = dk; A.dv = dv;
-    A.parts = attn_parts(a);
+    A.delta = workspace; A.dsl = dslopes ? workspace + items : nullptr;
+    A.key_parts = key_parts(a);
+    A.parts = row_parts(a);
+    float *next = workspace + up4(2 * items);
+    if (A.key_parts > 1) {
+        A.part = next;
+        A.stat = next + up4(items * A.key_parts * a->head_dim);
+        next = A.stat + up4(items * A.key_parts * 3);
+    }
+    if (A.parts > 1) A.part2 = next;
     OP_NEED(((int64_t)a->nk + 63) / 64 * A.KV * A.parts <= 0x7fffffffLL && ((int64_t)a->nk * A.KV + 3) / 4 <= 0x7fffffffLL, "too many keys for one launch");
-    // behind delta and dsl, at a multiple of 16 bytes of the workspace
-    if (A.parts > 1) A.part = workspace + (2 * (int64_t)a->nq * a->n_heads + 3) / 4 * 4;
     if (!attn_base(dq, size) || !attn_base(dk, size) || !attn_base(dv, size)) A.o_vec = 0;
-    OP_NEED(A.parts == 1 || attn_base(workspace, 4), "workspace must be 16-byte aligned");
     HIP_TRY(a->dtype ? dn_scene_attn_bwd_bf16(&A, dslopes, OP_ST) : dn_scene_attn_bwd_f32(&A, dslopes, OP_ST));
     return DAGNET_OK;
 }

@@ -28,8 +28,10 @@ struct SceneAttnArgs {
     int64_t q_rs, q_hs, k_rs, k_hs, v_rs, v_hs, do_rs, do_hs;      // element strides of rows and heads (out, dq, dk, dv: contiguous)
     int32_t nq, nk, H, KV, G, D, axes;
     float scale, cap;
-    int32_t parts;                             // of the rows in the dk / dv kernel; part: [parts][dk, dv][nk][KV][D]
-    float *part;
+    // Few tiles: their long axis is cut, the parts' sums meet in a join kernel.  key_parts: of a row tile's keys (forward: part [nq H][parts][D], stat
+    // [nq H][parts][2]; dq: part [nq H][parts][D], stat [nq H][parts][3]); parts: of a key tile's rows (part2 [parts][dk, dv][nk][KV][D])
+    int32_t key_parts, parts;
+    float *part, *stat, *part2;
     int32_t q_vec, k_vec, v_vec, do_vec, o32_vec;   // bytes per load that strides, base and width allow: 16, 8 or the element
     int32_t o_vec;                                 // results are stored four at a time
 };
@@ -282,6 +284,13 @@ __device__ __forceinline__ int64_t snake(int64_t i, int64_t n, int per) {
     return r * per + (r & 1 ? len - 1 - in : in);
 }
 constexpr int CUS = 256;
+
+// part i of n of the keys lo .. hi - 1, in whole tiles of BN
+template <int BN> __device__ __forceinline__ void key_part(int &lo, int &hi, int i, int n) {
+    const int64_t per = ((max(hi - lo, 0) + (int64_t)n * BN - 1) / ((int64_t)n * BN)) * BN, at = lo + per * i;
+    lo = (int)min(at, (int64_t)hi);
+    hi = (int)min(at + per, (int64_t)hi);
+}
 
 // Single values of a tile's N rows (N <= 64) straight into LDS: src is this lane's
 template <int N> __device__ __forceinline__ void stage_values(float *dst, const void *src) {

@@ -93,17 +93,29 @@ struct Slope {
         dsd += g.ds * g.dist;
         pd += g.p * g.dist;
     }
-    __device__ __forceinline__ void add(f32x4 p, f32x4 d, f32x4 dist) {          // four scores in fp32, then fp64: long rows lose nothing
-        ds += (d[0] + d[1]) + (d[2] + d[3]);
-        dsd += (d[0] * dist[0] + d[1] * dist[1]) + (d[2] * dist[2] + d[3] * dist[3]);
-        pd += (p[0] * dist[0] + p[1] * dist[1]) + (p[2] * dist[2] + p[3] * dist[3]);
-    }
     __device__ __forceinline__ float row() const { return (float)(ds * pd - dsd); }
-    __device__ __forceinline__ float row_of_groups() {                            // the four lane groups of a row together
+    __device__ __forceinline__ void over_groups() {                               // the four lane groups of a row together
         ds += __shfl_xor(ds, 16);   ds += __shfl_xor(ds, 32);
         dsd += __shfl_xor(dsd, 16); dsd += __shfl_xor(dsd, 32);
         pd += __shfl_xor(pd, 16);   pd += __shfl_xor(pd, 32);
-        return row();
+    }
+};
+
+// the same of one tile, in fp32 (a lane sees at most 16 of its scores)
+struct TileSlope {
+    float ds = 0.f, dsd = 0.f, pd = 0.f;
+    __device__ __forceinline__ void add(f32x4 p, f32x4 d, f32x4 dist) {
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            ds += d[i];
+            dsd = fmaf(d[i], dist[i], dsd);
+            pd = fmaf(p[i], dist[i], pd);
+        }
+    }
+    __device__ __forceinline__ void into(Slope &s) const {
+        s.ds += ds;
+        s.dsd += dsd;
+        s.pd += pd;
     }
 };
 
@@ -178,11 +190,12 @@ __global__ __launch_bounds__(256) void scene_attn_dq_kernel(const SceneAttnArgs 
     __shared__ u32x4 sk[2][NC], sv[2][NC];
     __shared__ __attribute__((aligned(16))) float sp[2][AX ? AX : 1][BN];
     const int tid = threadIdx.x, lane = tid & 63, w = tid >> 6, g = lane >> 4, c = lane & 15;
-    const int kvh = (int)(blockIdx.x % A.KV);
-    const int64_t R = (int64_t)A.nq * A.G, tiles = gridDim.x / A.KV, r0 = (tiles - 1 - snake(blockIdx.x / A.KV, tiles, max(CUS / A.KV, 1))) * ROWS;
+    const int kvh = (int)(blockIdx.x % A.KV), both = A.KV * A.key_parts, part = (int)(blockIdx.x / A.KV % A.key_parts);
+    const int64_t R = (int64_t)A.nq * A.G, tiles = gridDim.x / both, r0 = (tiles - 1 - snake(blockIdx.x / both, tiles, max(CUS / both, 1))) * ROWS;
     const Score<CAP, AX> S(A);
     const int qa = (int)(r0 / A.G), qb = (int)((min(r0 + ROWS, R) - 1) / A.G);
-    const int tlo = uniform(max(A.row_lo[qa], 0)), thi = uniform(min(A.row_hi[qb], A.nk));
+    int tlo = uniform(max(A.row_lo[qa], 0)), thi = uniform(min(A.row_hi[qb], A.nk));
+    if (A.key_parts > 1) key_part<BN>(tlo, thi, part, A.key_parts);
     const T *K = reinterpret_cast<const T *>(A.k) + kvh * A.k_hs, *V = reinterpret_cast<const T *>(A.v) + kvh * A.v_hs;
     const bool even = A.k_vec == 16 && A.v_vec == 16 && short_rows(A.k_rs, BN, sizeof(T)) && short_rows(A.v_rs, BN, sizeof(T));
     Stage<T, DP, BN, 256> tk, tv;
@@ -222,7 +235,7 @@ __global__ __launch_bounds__(256) void scene_attn_dq_kernel(const SceneAttnArgs 
 #pragma unroll
         for (int f = 0; f < NF; ++f) sum = delta_chunk<T>(sum, o, gf[b][f], f * X::KD + g * X::CH, A.D, A.o32_vec);
         delta[b] = group_sum(sum);
-        if (A.dk && g == 0 && r < R) A.delta[kvh * R + r] = delta[b];
+        if (A.dk && part == 0 && g == 0 && r < R) A.delta[kvh * R + r] = delta[b];
     }
     const int wlo = uniform(__shfl(s[0].lo, 0)), whi = uniform(__shfl(s[MB - 1].hi, 15));
     const int alo = uniform(__shfl(s[MB - 1].lo, 15)), ahi = uniform(__shfl(s[0].hi, 0));
@@ -238,6 +251,7 @@ __global__ __launch_bounds__(256) void scene_attn_dq_kernel(const SceneAttnArgs 
         landed();
         __syncthreads();
         if (kb > tlo && kb + BN < thi) issue(kb + BN, buf ^ 1);
+        TileSlope ts[MB];
 #pragma unroll
         for (int j = 0; j < BN / X::KB; ++j) {
             const int k0 = kb + j * X::KB, at = j * X::KB;
@@ -289,7 +303,7 @@ __global__ __launch_bounds__(256) void scene_attn_dq_kernel(const SceneAttnArgs 
                     }
                     ds *= p;
                     if constexpr (AX > 0)
-                        if (A.dsl) sl[b].add(p, ds, dist);
+                        if (A.dsl) ts[b].add(p, ds, dist);
                     e[b][n] = CAP ? ds * S.slope_of(t) : ds;
                 }
             }
@@ -303,11 +317,28 @@ __global__ __launch_bounds__(256) void scene_attn_dq_kernel(const SceneAttnArgs 
                 for (int b = 0; b < MB; ++b) acc[b][d] = mma(a, z[b], acc[b][d]);
             }
         }
+        if constexpr (AX > 0)
+            if (A.dsl) {
+#pragma unroll
+                for (int b = 0; b < MB; ++b) ts[b].into(sl[b]);
+            }
     }
 #pragma unroll
     for (int b = 0; b < MB; ++b) {
-        const int64_t r = r0 + (w * MB + b) * 16 + c;
-        const float dslope = AX > 0 ? sl[b].row_of_groups() : 0.f;
+        const int64_t r = r0 + (w * MB + b) * 16 + c, item = (int64_t)s[b].row * A.H + s[b].head;
+        if constexpr (AX > 0) sl[b].over_groups();
+        if (A.key_parts > 1) {
+            if (r < R) {
+#pragma unroll
+                for (int d = 0; d < DB; ++d) store4(A.part + (item * A.key_parts + part) * A.D, acc[b][d] * A.scale, d * 16 + g * 4, A.D, A.D % 4 == 0);
+                if (AX > 0 && g == 0) {
+                    float *st = A.stat + (item * A.key_parts + part) * 3;
+                    st[0] = (float)sl[b].ds; st[1] = (float)sl[b].dsd; st[2] = (float)sl[b].pd;
+                }
+            }
+            continue;
+        }
+        const float dslope = AX > 0 ? sl[b].row() : 0.f;
         bool fine = finite_(dslope);
 #pragma unroll
         for (int d = 0; d < DB; ++d)
@@ -317,7 +348,7 @@ __global__ __launch_bounds__(256) void scene_attn_dq_kernel(const SceneAttnArgs 
                 fine = fine && finite_(acc[b][d][i]);
             }
         if (r < R) {
-            T *out = reinterpret_cast<T *>(A.dq) + ((int64_t)s[b].row * A.H + s[b].head) * A.D;
+            T *out = reinterpret_cast<T *>(A.dq) + item * A.D;
 #pragma unroll
             for (int d = 0; d < DB; ++d) store4(out, acc[b][d], d * 16 + g * 4, A.D, A.o_vec != 0);
             if (AX > 0 && A.dsl && g == 0) A.dsl[kvh * R + r] = dslope;
@@ -519,8 +550,8 @@ __global__ __launch_bounds__(256, DP <= 32 ? 4 : DP <= 96 ? 3 : 2) void scene_at
             if (key < A.nk) {
 #pragma unroll
                 for (int d = 0; d < DB; ++d) {
-                    store4(A.part + 2 * part * n + at, dk[b][d], d * 16 + g * 4, A.D, A.D % 4 == 0);
-                    store4(A.part + (2 * part + 1) * n + at, dv[b][d], d * 16 + g * 4, A.D, A.D % 4 == 0);
+                    store4(A.part2 + 2 * part * n + at, dk[b][d], d * 16 + g * 4, A.D, A.D % 4 == 0);
+                    store4(A.part2 + (2 * part + 1) * n + at, dv[b][d], d * 16 + g * 4, A.D, A.D % 4 == 0);
                 }
             }
             continue;
@@ -541,32 +572,64 @@ __global__ __launch_bounds__(256, DP <= 32 ? 4 : DP <= 96 ? 3 : 2) void scene_at
     }
 }
 
-// dk and dv from the parts' sums, in order; a wave per (key, kv head)
-template <typename T> __global__ __launch_bounds__(256) void scene_attn_dkv_join_kernel(const SceneAttnArgs A) {
-    const int lane = threadIdx.x & 63;
-    const int64_t item = (int64_t)blockIdx.x * 4 + (threadIdx.x >> 6), n = (int64_t)A.nk * A.KV * A.D;
-    if (item >= (int64_t)A.nk * A.KV) return;
-    bool fine = true;
-    for (int d = lane; d < A.D; d += 64) {
-        const float *p = A.part + item * A.D + d;
-        float a = 0.f, b = 0.f;
-        for (int i = 0; i < A.parts; ++i) {
-            a += p[2 * i * n];
-            b += p[(2 * i + 1) * n];
+// dq (and a row's part of dslope) from the parts' sums, in order; 32 lanes per (row, head), four columns a lane
+template <typename T> __global__ __launch_bounds__(256) void scene_attn_dq_join_kernel(const SceneAttnArgs A) {
+    const int lane = threadIdx.x & 63, P = A.key_parts, d = (lane & 31) * 4, vec = A.D % 4 == 0 ? 16 : 4;
+    const int64_t items = (int64_t)A.nq * A.H, R = (int64_t)A.nq * A.G, own = (int64_t)blockIdx.x * 8 + (threadIdx.x >> 5), item = min(own, items - 1);
+    const int64_t row = item / A.H;
+    const int head = (int)(item - row * A.H), kvh = head / A.G;
+    const int64_t r = row * A.G + head - kvh * A.G;
+    f32x4 a = {0.f, 0.f, 0.f, 0.f};
+    for (int i = 0; i < P; ++i) a += __builtin_bit_cast(f32x4, load_chunk<float>(A.part + (item * P + i) * A.D, d, A.D, vec));
+    Slope s;
+    if (A.dsl)
+        for (int i = 0; i < P; ++i) {
+            const float *st = A.stat + (item * P + i) * 3;
+            s.ds += st[0];
+            s.dsd += st[1];
+            s.pd += st[2];
         }
-        reinterpret_cast<T *>(A.dk)[item * A.D + d] = (T)a;
-        reinterpret_cast<T *>(A.dv)[item * A.D + d] = (T)b;
-        fine = fine && finite_(a) && finite_(b);
+    if (own < items) {
+        store4(reinterpret_cast<T *>(A.dq) + item * A.D, a, d, A.D, A.o_vec != 0);
+        if (A.dsl && d == 0) A.dsl[kvh * R + r] = s.row();
     }
-    if (__any(!fine)) dkv_slow<T>(A, (int)(item % A.KV), item / A.KV, (int64_t)A.nq * A.G);
+    const bool fine = own >= items || (finite_(s.row()) && finite_(a[0]) && finite_(a[1]) && finite_(a[2]) && finite_(a[3]));
+    const uint64_t bad = __ballot(!fine);
+    for (int h = 0; h < 2; ++h)                              // the wave's two pairs
+        if (bad >> (32 * h) & 0xffffffffull) dq_slow<T>(A, __shfl(kvh, 32 * h), row_state(A, __shfl(kvh, 32 * h), __shfl(r, 32 * h), R), __shfl(r, 32 * h), R);
+}
+
+// dk and dv from the parts' sums, in order; 32 lanes per (key, kv head), four columns a lane
+template <typename T> __global__ __launch_bounds__(256) void scene_attn_dkv_join_kernel(const SceneAttnArgs A) {
+    const int lane = threadIdx.x & 63, d = (lane & 31) * 4, vec = A.D % 4 == 0 ? 16 : 4;
+    const int64_t items = (int64_t)A.nk * A.KV, n = items * A.D, own = (int64_t)blockIdx.x * 8 + (threadIdx.x >> 5), item = min(own, items - 1);
+    f32x4 a = {0.f, 0.f, 0.f, 0.f}, b = {0.f, 0.f, 0.f, 0.f};
+    for (int i = 0; i < A.parts; ++i) {
+        a += __builtin_bit_cast(f32x4, load_chunk<float>(A.part2 + 2 * i * n + item * A.D, d, A.D, vec));
+        b += __builtin_bit_cast(f32x4, load_chunk<float>(A.part2 + (2 * i + 1) * n + item * A.D, d, A.D, vec));
+    }
+    bool fine = true;
+    if (own < items) {
+        store4(reinterpret_cast<T *>(A.dk) + item * A.D, a, d, A.D, A.o_vec != 0);
+        store4(reinterpret_cast<T *>(A.dv) + item * A.D, b, d, A.D, A.o_vec != 0);
+#pragma unroll
+        for (int i = 0; i < 4; ++i) fine = fine && finite_(a[i]) && finite_(b[i]);
+    }
+    const uint64_t bad = __ballot(!fine);
+    for (int h = 0; h < 2; ++h)                              // the wave's two pairs
+        if (bad >> (32 * h) & 0xffffffffull) {
+            const int64_t it = __shfl(item, 32 * h);
+            dkv_slow<T>(A, (int)(it % A.KV), it / A.KV, (int64_t)A.nq * A.G);
+        }
 }
 
 template <typename T, int DP, int BN, bool CAP, int AX> hipError_t launch_bwd(const SceneAttnArgs &A, hipStream_t st) {
     const int64_t tiles = ((int64_t)A.nq * A.G + 63) / 64;
-    if (tiles > 0 && A.dq) hipLaunchKernelGGL((scene_attn_dq_kernel<T, DP, BN, 1, CAP, AX>), dim3((unsigned)(tiles * A.KV)), dim3(256), 0, st, A);
+    if (tiles > 0 && A.dq) hipLaunchKernelGGL((scene_attn_dq_kernel<T, DP, BN, 1, CAP, AX>), dim3((unsigned)(tiles * A.KV * A.key_parts)), dim3(256), 0, st, A);
+    if (tiles > 0 && A.dq && A.key_parts > 1) hipLaunchKernelGGL((scene_attn_dq_join_kernel<T>), dim3((unsigned)(((int64_t)A.nq * A.H + 7) / 8)), dim3(256), 0, st, A);
     if (A.nk > 0 && A.dk) {
         hipLaunchKernelGGL((scene_attn_dkv_kernel<T, DP, BN, 1, CAP, AX>), dim3((unsigned)(((int64_t)A.nk + 63) / 64 * A.KV * A.parts)), dim3(256), 0, st, A);
-        if (A.parts > 1) hipLaunchKernelGGL((scene_attn_dkv_join_kernel<T>), dim3((unsigned)(((int64_t)A.nk * A.KV + 3) / 4)), dim3(256), 0, st, A);
+        if (A.parts > 1) hipLaunchKernelGGL((scene_attn_dkv_join_kernel<T>), dim3((unsigned)(((int64_t)A.nk * A.KV + 7) / 8)), dim3(256), 0, st, A);
     }
     return hipGetLastError();
 }

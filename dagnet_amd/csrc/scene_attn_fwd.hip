@@ -52,8 +52,8 @@ __global__ __launch_bounds__(256, MB == 2 ? 2 : 3) void scene_attn_fwd_kernel(co
     __shared__ u32x4 sk[2][NC], sv[2][NC];
     __shared__ __attribute__((aligned(16))) float sp[2][AX ? AX : 1][BN];
     const int tid = threadIdx.x, lane = tid & 63, w = tid >> 6, g = lane >> 4, c = lane & 15;
-    const int kvh = (int)(blockIdx.x % A.KV);
-    const int64_t R = (int64_t)A.nq * A.G, tiles = gridDim.x / A.KV, r0 = (tiles - 1 - snake(blockIdx.x / A.KV, tiles, max(CUS / A.KV, 1))) * ROWS;
+    const int kvh = (int)(blockIdx.x % A.KV), both = A.KV * A.key_parts, part = (int)(blockIdx.x / A.KV % A.key_parts);
+    const int64_t R = (int64_t)A.nq * A.G, tiles = gridDim.x / both, r0 = (tiles - 1 - snake(blockIdx.x / both, tiles, max(CUS / both, 1))) * ROWS;
     const Score<CAP, AX> S(A);
     constexpr bool PLAIN = !CAP && AX == 0;                 // scores stay raw until the exponent: 2^(raw k - base) in one fma
     const bool flip = PLAIN && A.scale < 0.f;               // their maximum then needs k >= 0: the sign goes to q
@@ -61,7 +61,8 @@ __global__ __launch_bounds__(256, MB == 2 ? 2 : 3) void scene_attn_fwd_kernel(co
 
     // the keys of the workgroup's rows; the first two tiles are on their way before anything else is read
     const int qa = (int)(r0 / A.G), qb = (int)((min(r0 + ROWS, R) - 1) / A.G);
-    const int tlo = uniform(max(A.row_lo[qa], 0)), thi = uniform(min(A.row_hi[qb], A.nk));
+    int tlo = uniform(max(A.row_lo[qa], 0)), thi = uniform(min(A.row_hi[qb], A.nk));
+    if (A.key_parts > 1) key_part<BN>(tlo, thi, part, A.key_parts);
     const T *K = reinterpret_cast<const T *>(A.k) + kvh * A.k_hs, *V = reinterpret_cast<const T *>(A.v) + kvh * A.v_hs;
     const bool even = A.k_vec == 16 && A.v_vec == 16 && short_rows(A.k_rs, BN, sizeof(T)) && short_rows(A.v_rs, BN, sizeof(T));
     Stage<T, DP, BN, 256> tk, tv;
@@ -222,7 +223,19 @@ __global__ __launch_bounds__(256, MB == 2 ? 2 : 3) void scene_attn_fwd_kernel(co
     }
 #pragma unroll
     for (int b = 0; b < MB; ++b) {
-        const int64_t r = r0 + (w * MB + b) * 16 + c;
+        const int64_t r = r0 + (w * MB + b) * 16 + c, item = (int64_t)s[b].row * A.H + s[b].head;
+        if (A.key_parts > 1) {
+            const float sum = group_sum(l[b]);
+            if (r < R) {
+#pragma unroll
+                for (int d = 0; d < DB; ++d) store4(A.part + (item * A.key_parts + part) * A.D, o[b][d], d * 16 + g * 4, A.D, A.D % 4 == 0);
+                if (g == 0) {
+                    A.stat[(item * A.key_parts + part) * 2] = m[b];
+                    A.stat[(item * A.key_parts + part) * 2 + 1] = sum;
+                }
+            }
+            continue;
+        }
         const float sum = group_sum(l[b]), inv = sum == 0.f ? 0.f : 1.f / sum;
         bool fine = finite_(sum);
 #pragma unroll
@@ -233,7 +246,7 @@ __global__ __launch_bounds__(256, MB == 2 ? 2 : 3) void scene_attn_fwd_kernel(co
                 fine = fine && finite_(o[b][d][i]);
             }
         if (r < R) {
-            const int64_t at = ((int64_t)s[b].row * A.H + s[b].head) * A.D;
+            const int64_t at = item * A.D;
 #pragma unroll
             for (int d = 0; d < DB; ++d) {
                 store4(reinterpret_cast<T *>(A.out) + at, o[b][d], d * 16 + g * 4, A.D, A.o_vec != 0);
@@ -251,11 +264,41 @@ __global__ __launch_bounds__(256, MB == 2 ? 2 : 3) void scene_attn_fwd_kernel(co
     }
 }
 
+// (row, head) pairs from their parts, 32 lanes each, four columns a lane
+template <typename T> __global__ __launch_bounds__(256) void scene_attn_fwd_join_kernel(const SceneAttnArgs A) {
+    const int lane = threadIdx.x & 63, P = A.key_parts, d = (lane & 31) * 4, vec = A.D % 4 == 0 ? 16 : 4;
+    const int64_t items = (int64_t)A.nq * A.H, R = (int64_t)A.nq * A.G, own = (int64_t)blockIdx.x * 8 + (threadIdx.x >> 5), item = min(own, items - 1);
+    const float *stat = A.stat + item * P * 2, *part = A.part + item * P * A.D;
+    float m = NEG_INF, l = 0.f;
+    f32x4 o = {0.f, 0.f, 0.f, 0.f};
+    for (int i = 0; i < P; ++i) m = fmaxf(m, stat[2 * i]);
+    const float base = m == NEG_INF ? 0.f : m;
+    for (int i = 0; i < P; ++i) {
+        const float f = exp2_(stat[2 * i] - base);
+        l += f * stat[2 * i + 1];
+        o += f * __builtin_bit_cast(f32x4, load_chunk<float>(part + (int64_t)i * A.D, d, A.D, vec));
+    }
+    o *= l == 0.f ? 0.f : 1.f / l;
+    const int64_t row = item / A.H;
+    const int head = (int)(item - row * A.H), kvh = head / A.G;
+    const int64_t r = row * A.G + head - kvh * A.G;
+    if (own < items) {
+        store4(reinterpret_cast<T *>(A.out) + item * A.D, o, d, A.D, A.o_vec != 0);
+        if (A.o32) store4(A.o32 + item * A.D, o, d, A.D, A.o_vec != 0);
+        if (A.lse && d == 0) A.lse[kvh * R + r] = l == 0.f ? 0.f : m + log2_(l);
+    }
+    const bool fine = own >= items || (finite_(l) && finite_(o[0]) && finite_(o[1]) && finite_(o[2]) && finite_(o[3]));
+    const uint64_t bad = __ballot(!fine);
+    for (int h = 0; h < 2; ++h)                              // the wave's two pairs
+        if (bad >> (32 * h) & 0xffffffffull) row_slow<T>(A, __shfl(kvh, 32 * h), row_state(A, __shfl(kvh, 32 * h), __shfl(r, 32 * h), R), __shfl(r, 32 * h), R);
+}
+
 template <typename T, int DP, int BN, int MB, bool CAP, int AX> hipError_t launch_fwd(const SceneAttnArgs &A, hipStream_t st) {
     const int64_t tiles = ((int64_t)A.nq * A.G + 64 * MB - 1) / (64 * MB);
-    const dim3 grid((unsigned)(tiles * A.KV));
+    const dim3 grid((unsigned)(tiles * A.KV * A.key_parts));
     if (sizeof(T) == 2 && A.o32) hipLaunchKernelGGL((scene_attn_fwd_kernel<T, DP, BN, MB, CAP, AX, sizeof(T) == 2>), grid, dim3(256), 0, st, A);
     else hipLaunchKernelGGL((scene_attn_fwd_kernel<T, DP, BN, MB, CAP, AX, false>), grid, dim3(256), 0, st, A);
+    if (A.key_parts > 1) hipLaunchKernelGGL((scene_attn_fwd_join_kernel<T>), dim3((unsigned)(((int64_t)A.nq * A.H + 7) / 8)), dim3(256), 0, st, A);
     return hipGetLastError();
 }
 template <typename T, int DP, int BN, int MB> hipError_t pick_fwd(const SceneAttnArgs &A, hipStream_t st) {
@@ -282,5 +325,12 @@ extern "C" hipError_t dn_scene_attn_fwd_f32(const SceneAttnArgs *A, hipStream_t 
     const int D = A->D;
     return D <= 16 ? pick_fwd<float, 16, 64, 1>(*A, st) : D <= 32 ? pick_fwd<float, 32, 64, 1>(*A, st) : D <= 48 ? pick_fwd<float, 48, 32, 1>(*A, st)
          : D <= 64 ? pick_fwd<float, 64, 32, 1>(*A, st) : D <= 96 ? pick_fwd<float, 96, 32, 1>(*A, st) : pick_fwd<float, 128, 32, 1>(*A, st);
+}
+// Parts of the keys of a row tile, forward and dq, where there are few tiles: none below 256 of the keys that a row sees (most), and as many as give the
+// chip's CUs three workgroups each (what their registers and LDS hold) - four where rows see unlike numbers of keys (mean far below most): then the
+// longest tile is what the rest waits for.  4096 causal rows of 8 heads: 102 us in one part, 66 + 8 to join in two; seeing all keys: 92 and 121.
+extern "C" int dn_scene_attn_key_parts(int64_t nq, int KV, int G, int64_t most, int64_t mean) {
+    const int64_t tiles = (nq * G + 63) / 64 * KV, want = tiles ? (3 * mean < 2 * most ? 1024 : 768) / tiles : 1, parts = want < most / 256 ? want : most / 256;
+    return (int)(parts < 1 ? 1 : parts < 8 ? parts : 8);
 }
 #endif

@@ -415,11 +415,16 @@ typedef struct {
     const float *slopes, *q_pos, *k_pos; /* [n_heads], [nq][axes], [nk][axes] */
     int64_t q_row, q_head, k_row, k_head, v_row, v_head;
     int32_t nq, nk, n_heads, n_kv_heads, head_dim, axes, dtype;
+    int32_t max_keys, mean_keys;         /* of what the rows see: whether a row's keys are split over workgroups (0, 0: never); no effect on results
+                                          * but for the order of sums */
     float scale, softcap;
 } dagnet_attn;
 /* row_lo, row_hi [nq]: int32, neither decreasing.  For a later backward pass (NULL: none wanted): lse [nq * n_heads] receives the rows'
- * statistics, o32 [nq][n_heads][head_dim] the unrounded output (bf16 only; fp32 passes NULL and keeps out). */
-int dagnet_op_attn_fwd(const dagnet_attn *a, const int32_t *row_lo, const int32_t *row_hi, void *out, float *lse, float *o32, void *stream);
+ * statistics, o32 [nq][n_heads][head_dim] the unrounded output (bf16 only; fp32 passes NULL and keeps out).  workspace:
+ * dagnet_op_attn_fwd_workspace(a) floats (0: may be NULL), 16-byte aligned and private to the call until it has run, like that of the others. */
+int64_t dagnet_op_attn_fwd_workspace(const dagnet_attn *a);
+int dagnet_op_attn_fwd(const dagnet_attn *a, const int32_t *row_lo, const int32_t *row_hi, void *out, float *lse, float *o32, float *workspace,
+                       void *stream);
 /* key_lo, key_hi [nk]: the rows that see a key lie in key_lo[j] <= i < key_hi[j], neither decreasing.  o: o32, or out for fp32.
  * dq (with dslopes) or dk and dv may be NULL: not wanted; dslopes [n_heads] is NULL or has axes > 0.  Deterministic: no atomics.
  * workspace: dagnet_op_attn_bwd_workspace(a) floats. */

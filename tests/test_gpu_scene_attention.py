@@ -52,6 +52,9 @@ LAYOUTS = {
     "steps_prefix": ([0, 60, 63, 135], [5, 3, 8], [20, 3, 0]),
     "prefix_longer_than_scene": ([0, 20, 90], 1, 40),
     "long": ([0, 333], [7], 31),
+    "keys_in_parts": ([0, 1100], 1, 0),
+    "two_in_parts": ([0, 1, 640, 1290], 0, 0),
+    "prefix_in_parts": ([0, 1027], 9, 600),
 }
 
 
@@ -157,6 +160,27 @@ def test_masked_places_do_not_reach_a_row(dt, bad):
     got = run(t)
     assert torch.isfinite(got[0][:39].float()).all() and not torch.isfinite(got[0][39].float()).all()
     assert torch.isfinite(got[1][:39].float()).all()
+
+
+@pytest.mark.parametrize("dt", [F32, BF16], ids=["fp32", "bf16"])
+def test_masked_places_in_long_rows_whose_keys_are_split(dt):
+    N, H, D = 1100, 2, 24
+    layout = SceneLayout([0, N], causal=1)
+
+    def run(spoil):
+        t = inputs(4, N, N, H, H, D, dt, 1)
+        if spoil:
+            t["k"][900], t["v"][900], t["q"][950], t["dout"][950] = float("nan"), float("inf"), float("inf"), float("nan")
+        leaves = [t[n].requires_grad_() for n in ("q", "k", "v", "slopes")]
+        o = scene_attention(t["q"], t["k"], t["v"], layout, slopes=t["slopes"], pos=t["pos"])
+        return (o,) + torch.autograd.grad(o, leaves, t["dout"])
+    clean, got = run(False), run(True)
+    for a, b, n in zip(got[:2], clean[:2], ("out", "dq")):                      # rows before the spoilt key
+        x, y = a[:900].float(), b[:900].float()
+        assert torch.isfinite(x).all() and not torch.isfinite(a[900:].float()).all()
+        assert (x - y).abs().max() <= 2.0 ** (-7 if dt is BF16 else -17) * y.abs().max(), n
+    for a in got[2:4]:                                                          # keys behind the spoilt row are seen by fine rows alone, but for those
+        assert torch.isfinite(a[951:].float()).all() == torch.isfinite(got[1][951:].float()).all()
 
 
 def test_values_at_the_ends_of_the_type():

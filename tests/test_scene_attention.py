@@ -125,12 +125,12 @@ def test_c_entries_refuse_before_any_launch():
 
     def rc(**kw):
         a = _ops._Attn(**{**ok, **kw})
-        return lib.dagnet_op_attn_fwd(C.byref(a), None, None, None, None, None, None)
+        return lib.dagnet_op_attn_fwd(C.byref(a), *[None] * 7)
     for kw, word in ((dict(head_dim=129), b"head_dim"), (dict(head_dim=0), b"head_dim"), (dict(n_heads=3, n_kv_heads=2), b"multiple"), (dict(dtype=2), b"dtype"),
-                     (dict(axes=4), b"axes"), (dict(nq=-1), b"row counts"), (dict(softcap=float("nan")), b"softcap"), (dict(scale=float("inf")), b"scale"),
+                     (dict(axes=4), b"axes"), (dict(max_keys=-1), b"max_keys"), (dict(nq=-1), b"row counts"), (dict(softcap=float("nan")), b"softcap"), (dict(scale=float("inf")), b"scale"),
                      (dict(q=None), b"null q"), (dict(axes=2), b"positions"), (dict(), b"null argument")):
         assert rc(**kw) == -1 and word in lib.dagnet_last_error()
-    assert lib.dagnet_op_attn_fwd(None, None, None, None, None, None, None) == -1
+    assert lib.dagnet_op_attn_fwd(None, *[None] * 7) == -1
     assert rc(nq=0, q=None) == 0
     a = _ops._Attn(**ok)
     assert lib.dagnet_op_attn_bwd(C.byref(a), *[None] * 5, 0, 0, *[None] * 3, 64, 64, None, None, None) == -1 and b"dk and dv" in lib.dagnet_last_error()
@@ -145,4 +145,4 @@ def test_c_entries_refuse_before_any_launch():
         assert lib.dagnet_op_rotary(*bad) == -1
     assert lib.dagnet_op_rotary(0, *r[1:]) == 0
     with pytest.raises(DagnetHipError, match="null argument"):
-        _capi._check(lib.dagnet_op_attn_fwd(C.byref(a), *[None] * 6))
+        _capi._check(lib.dagnet_op_attn_fwd(C.byref(a), *[None] * 7))
