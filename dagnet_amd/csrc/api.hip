@@ -2170,7 +2170,7 @@ extern "C" int dn_scene_attn_bwd_parts(int64_t, int64_t, int, int);
 extern "C" int dn_scene_attn_key_parts(int64_t, int, int, int64_t, int64_t);
 extern "C" hipError_t dn_scene_attn_step_f32(const SceneStepArgs *, hipStream_t);
 extern "C" hipError_t dn_scene_attn_step_bf16(const SceneStepArgs *, hipStream_t);
-extern "C" void dn_scene_attn_step_shape(int64_t, int64_t, int, int *, int *, int *);
+extern "C" void dn_scene_attn_step_shape(int64_t, int64_t, int, int *, int *);
 extern "C" hipError_t dn_rotary(const RotaryArgs *, int, int, hipStream_t);
 
 // bytes per load that a matrix of rows allows
@@ -2276,14 +2276,14 @@ extern "C" int dagnet_op_attn_bwd(const dagnet_attn *a, const int32_t *row_lo, c
     return DAGNET_OK;
 }
 
-static void step_shape(const dagnet_attn *a, int32_t scenes, int32_t room, int32_t max_rows, int *cblocks, int *splits, int *wide) {
-    dn_scene_attn_step_shape((int64_t)max_rows * (a->n_heads / a->n_kv_heads), (int64_t)scenes * a->n_kv_heads, room, cblocks, splits, wide);
+static void step_shape(const dagnet_attn *a, int32_t scenes, int32_t room, int32_t max_rows, int *cblocks, int *splits) {
+    dn_scene_attn_step_shape((int64_t)max_rows * (a->n_heads / a->n_kv_heads), (int64_t)scenes * a->n_kv_heads, room, cblocks, splits);
 }
 
 extern "C" int64_t dagnet_op_attn_step_workspace(const dagnet_attn *a, int32_t scenes, int32_t room, int32_t max_rows) {
     if (!a || scenes < 1 || room < 1 || max_rows < 1 || a->n_kv_heads < 1 || a->n_heads < a->n_kv_heads) return 0;
-    int cb, sp, wide;
-    step_shape(a, scenes, room, max_rows, &cb, &sp, &wide);
+    int cb, sp;
+    step_shape(a, scenes, room, max_rows, &cb, &sp);
     return sp == 1 ? 0 : (int64_t)a->nq * a->n_heads * sp * (a->head_dim + 2);
 }
 
@@ -2295,7 +2295,7 @@ extern "C" int dagnet_op_attn_step(const dagnet_attn *a, const int32_t *q_ptr, c
     if (a->nq == 0 || scenes == 0) return DAGNET_OK;
     OP_NEED(max_rows >= 1 && q_ptr && k_len && out && (room == 0 || (a->k && a->v && (!a->axes || a->k_pos))), "bad argument");
     A.q_ptr = q_ptr; A.k_len = k_len; A.scenes = scenes; A.room = room; A.k_ss = k_scene; A.v_ss = v_scene;
-    step_shape(a, scenes, room, max_rows, &A.cblocks, &A.splits, &A.wide);
+    step_shape(a, scenes, room, max_rows, &A.cblocks, &A.splits);
     OP_NEED((int64_t)scenes * a->n_kv_heads * A.cblocks * A.splits <= 0x7fffffffLL, "too many rows for one launch");
     OP_NEED(A.splits == 1 || workspace, "workspace is NULL");
     const int size = a->dtype ? 2 : 4;

@@ -11,8 +11,7 @@
 
 namespace sattn {
 
-// CB: blocks of 16 packed rows a workgroup takes at once: K and V fragments then serve all of them.
-template <typename T, int DP, int CB, bool CAP, int AX> __global__ __launch_bounds__(256) void scene_attn_step_kernel(const SceneStepArgs A) {
+template <typename T, int DP, bool CAP, int AX> __global__ __launch_bounds__(256) void scene_attn_step_kernel(const SceneStepArgs A) {
     using X = Tr<T>;
     using L = Tile<T, DP>;
     constexpr int NF = DP / X::KD, DB = DP / 16, PB = X::KB / 16, NC = X::KB * L::NCH, PER = NC / 64;
@@ -20,18 +19,17 @@ template <typename T, int DP, int CB, bool CAP, int AX> __global__ __launch_boun
     static_assert(NC % 64 == 0 && X::KB <= 64, "tile");
     __shared__ u32x4 sv[4][NC];
     __shared__ __attribute__((aligned(16))) float sp[4][AX ? AX : 1][X::KB];
-    __shared__ float sm[CB][4][16], sl[CB][4][16];
+    __shared__ float sm[4][16], sl[4][16];
     const int tid = threadIdx.x, lane = tid & 63, w = tid >> 6, g = lane >> 4, c = lane & 15;
     int64_t id = blockIdx.x;
     const int kvh = (int)(id % A.a.KV);
     id /= A.a.KV;
     const int split = (int)(id % A.splits);
     id /= A.splits;
-    const int cb = (int)(id % A.cblocks) * CB, sc = (int)(id / A.cblocks);
+    const int cb = (int)(id % A.cblocks), sc = (int)(id / A.cblocks);
     const int q0 = max(A.q_ptr[sc], 0), q1 = min(A.q_ptr[sc + 1], A.a.nq);
     const int64_t n = (int64_t)(q1 - q0) * A.a.G;
     if ((int64_t)cb * 16 >= n) return;                              // the whole workgroup
-    const int live = (int)min((int64_t)CB, (n + 15) / 16 - cb);     // blocks with rows in them
     const int len = min(max(A.k_len[sc], 0), A.room);
     const int per = (int)((((int64_t)len + A.splits - 1) / A.splits + 4 * X::KB - 1) / (4 * X::KB)) * (4 * X::KB);   // whole rounds of the four waves
     const int ka = (int)min((int64_t)split * per, (int64_t)len), kz = (int)min((int64_t)ka + per, (int64_t)len);
@@ -41,25 +39,6 @@ template <typename T, int DP, int CB, bool CAP, int AX> __global__ __launch_boun
     const T *K = reinterpret_cast<const T *>(A.a.k) + sc * A.k_ss + kvh * A.a.k_hs, *V = reinterpret_cast<const T *>(A.a.v) + sc * A.v_ss + kvh * A.a.v_hs;
     const float *kpos = A.a.kpos + (int64_t)sc * A.room * A.a.axes;
 
-    int row[CB], head[CB];
-    float slope[CB], qpos[CB][3];
-    typename X::frag qf[CB][NF];
-#pragma unroll
-    for (int b = 0; b < CB; ++b) {
-        const int64_t pr = min((int64_t)(cb + b) * 16 + c, n - 1);
-        row[b] = q0 + (int)(pr / A.a.G);
-        head[b] = kvh * A.a.G + (int)(pr % A.a.G);
-        slope[b] = AX ? A.a.slopes[head[b]] * LOG2E : 0.f;
-#pragma unroll
-        for (int a = 0; a < 3; ++a) qpos[b][a] = a < AX && a < A.a.axes ? A.a.qpos[(int64_t)row[b] * A.a.axes + a] : 0.f;
-        const T *Q = reinterpret_cast<const T *>(A.a.q) + row[b] * A.a.q_rs + head[b] * A.a.q_hs;
-#pragma unroll
-        for (int f = 0; f < NF; ++f) {
-            u32x4 v = load_chunk<T>(Q, f * X::KD + g * X::CH, A.a.D, A.a.q_vec);
-            if (flip) v ^= sizeof(T) == 4 ? 0x80000000u : 0x80008000u;
-            qf[b][f] = as_frag<T>(v);
-        }
-    }
     u32x4 rk[PB][NF], rv[PER];
     float rp[AX ? AX : 1];
     auto fetch = [&](int k0) {                                      // keys behind the last one stand in as the last one, masked below
@@ -80,17 +59,27 @@ template <typename T, int DP, int CB, bool CAP, int AX> __global__ __launch_boun
             for (int a = 0; a < AX; ++a) rp[a] = a < A.a.axes ? p[a] : 0.f;
         }
     };
-    f32x4 o[CB][DB];
-    float m[CB], l[CB];
-#pragma unroll
-    for (int b = 0; b < CB; ++b) {
-        m[b] = NEG_INF;
-        l[b] = 0.f;
-#pragma unroll
-        for (int d = 0; d < DB; ++d) o[b][d] = f32x4{0.f, 0.f, 0.f, 0.f};
-    }
     int k0 = ka + w * X::KB;
     if (k0 < kz) fetch(k0);
+
+    const int64_t pr = min((int64_t)cb * 16 + c, n - 1);
+    const int row = q0 + (int)(pr / A.a.G), head = kvh * A.a.G + (int)(pr % A.a.G);
+    const float slope = AX ? A.a.slopes[head] * LOG2E : 0.f;
+    float qpos[3];
+#pragma unroll
+    for (int a = 0; a < 3; ++a) qpos[a] = a < AX && a < A.a.axes ? A.a.qpos[(int64_t)row * A.a.axes + a] : 0.f;
+    const T *Q = reinterpret_cast<const T *>(A.a.q) + row * A.a.q_rs + head * A.a.q_hs;
+    typename X::frag qf[NF];
+#pragma unroll
+    for (int f = 0; f < NF; ++f) {
+        u32x4 v = load_chunk<T>(Q, f * X::KD + g * X::CH, A.a.D, A.a.q_vec);
+        if (flip) v ^= sizeof(T) == 4 ? 0x80000000u : 0x80008000u;
+        qf[f] = as_frag<T>(v);
+    }
+    f32x4 o[DB];
+    float m = NEG_INF, l = 0.f;
+#pragma unroll
+    for (int d = 0; d < DB; ++d) o[d] = f32x4{0.f, 0.f, 0.f, 0.f};
     for (; k0 < kz; k0 += 4 * X::KB) {
 #pragma unroll
         for (int i = 0; i < PER; ++i) {
@@ -105,111 +94,90 @@ template <typename T, int DP, int CB, bool CAP, int AX> __global__ __launch_boun
         }
         __builtin_amdgcn_fence(__ATOMIC_RELEASE, "wavefront");      // the wave's own LDS writes, before its reads across lanes
         __builtin_amdgcn_wave_barrier();
-        f32x4 x[CB][PB];
-#pragma unroll
-        for (int b = 0; b < CB; ++b) {
-            if (b >= live) break;
-#pragma unroll
-            for (int j = 0; j < PB; ++j) {
-                x[b][j] = f32x4{0.f, 0.f, 0.f, 0.f};
-#pragma unroll
-                for (int f = 0; f < NF; ++f) x[b][j] = mma(as_frag<T>(rk[j][f]), qf[b][f], x[b][j]);
-            }
-        }
-        if (k0 + 4 * X::KB < kz) fetch(k0 + 4 * X::KB);
-        const bool tail = k0 + X::KB > kz;
-        f32x4 px[PB] = {}, py[PB] = {}, pz[PB] = {};
+        f32x4 x[PB];
 #pragma unroll
         for (int j = 0; j < PB; ++j) {
-            if constexpr (AX > 0) read_positions<AX>(sp[w], j * 16 + 4 * g, px[j], py[j], pz[j]);
-        }
+            x[j] = f32x4{0.f, 0.f, 0.f, 0.f};
 #pragma unroll
-        for (int b = 0; b < CB; ++b) {
-            if (b >= live) break;
-            if constexpr (!PLAIN) S.template apply<PB>(x[b]);
-            float top = NEG_INF;
+            for (int f = 0; f < NF; ++f) x[j] = mma(as_frag<T>(rk[j][f]), qf[f], x[j]);
+        }
+        if (k0 + 4 * X::KB < kz) fetch(k0 + 4 * X::KB);
+        if constexpr (!PLAIN) S.template apply<PB>(x);
+        if constexpr (AX > 0) {
 #pragma unroll
             for (int j = 0; j < PB; ++j) {
-                if constexpr (AX > 0) x[b][j] -= slope[b] * S.dist4(qpos[b], px[j], py[j], pz[j]);
-                if (tail) {
-#pragma unroll
-                    for (int i = 0; i < 4; ++i) x[b][j][i] = k0 + j * 16 + 4 * g + i < kz ? x[b][j][i] : NEG_INF;
-                }
-#pragma unroll
-                for (int i = 0; i < 4; ++i) top = fmaxf(top, x[b][j][i]);
+                f32x4 px = {}, py = {}, pz = {};
+                read_positions<AX>(sp[w], j * 16 + 4 * g, px, py, pz);
+                x[j] -= slope * S.dist4(qpos, px, py, pz);
             }
-            top = group_max(top);
-            if constexpr (PLAIN) top = top == NEG_INF ? NEG_INF : top * k;
-            if (__any(top > m[b])) {
-                const float nm = fmaxf(top, m[b]), corr = exp2_(m[b] - (nm == NEG_INF ? 0.f : nm));
-                m[b] = nm;
-                l[b] *= corr;
-#pragma unroll
-                for (int d = 0; d < DB; ++d) o[b][d] *= corr;
-            }
-            const float base = m[b] == NEG_INF ? 0.f : m[b];
-            float sum = 0.f;
+        }
+        if (k0 + X::KB > kz) {
 #pragma unroll
             for (int j = 0; j < PB; ++j)
 #pragma unroll
-                for (int i = 0; i < 4; ++i) {
-                    x[b][j][i] = exp2_(PLAIN ? x[b][j][i] * k - base : x[b][j][i] - base);
-                    sum += x[b][j][i];
-                }
-            l[b] += sum;
+                for (int i = 0; i < 4; ++i) x[j][i] = k0 + j * 16 + 4 * g + i < kz ? x[j][i] : NEG_INF;
         }
-        typename X::frag p[CB];
+        float top = NEG_INF;
 #pragma unroll
-        for (int b = 0; b < CB; ++b) p[b] = pack_p(x[b], T());
+        for (int j = 0; j < PB; ++j)
 #pragma unroll
-        for (int d = 0; d < DB; ++d) {
-            const typename X::frag a = frag_cols<DP>(sv[w], 0, d, lane, T());
+            for (int i = 0; i < 4; ++i) top = fmaxf(top, x[j][i]);
+        top = group_max(top);
+        if constexpr (PLAIN) top = top == NEG_INF ? NEG_INF : top * k;
+        if (__any(top > m)) {
+            const float nm = fmaxf(top, m), corr = exp2_(m - (nm == NEG_INF ? 0.f : nm));
+            m = nm;
+            l *= corr;
 #pragma unroll
-            for (int b = 0; b < CB; ++b)
-                if (b < live) o[b][d] = mma(a, p[b], o[b][d]);
+            for (int d = 0; d < DB; ++d) o[d] *= corr;
         }
+        const float base = m == NEG_INF ? 0.f : m;
+        float sum = 0.f;
+#pragma unroll
+        for (int j = 0; j < PB; ++j)
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+                x[j][i] = exp2_(PLAIN ? x[j][i] * k - base : x[j][i] - base);
+                sum += x[j][i];
+            }
+        l += sum;
+        const typename X::frag p = pack_p(x, T());
+#pragma unroll
+        for (int d = 0; d < DB; ++d) o[d] = mma(frag_cols<DP>(sv[w], 0, d, lane, T()), p, o[d]);
         __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "wavefront");
         __builtin_amdgcn_wave_barrier();
     }
     // the four waves' parts: statistics first, then the outputs, rescaled, through the waves' V stretches
-#pragma unroll
-    for (int b = 0; b < CB; ++b) {
-        l[b] = group_sum(l[b]);
-        if (g == 0) { sm[b][w][c] = m[b]; sl[b][w][c] = l[b]; }
-    }
+    l = group_sum(l);
+    if (g == 0) { sm[w][c] = m; sl[w][c] = l; }
     __syncthreads();
     float *so = reinterpret_cast<float *>(&sv[0][0]);                // [4 waves][16][DP]
     static_assert(4 * NC * 4 >= 4 * 16 * DP, "LDS");
+    float M = NEG_INF, sum = 0.f;
 #pragma unroll
-    for (int b = 0; b < CB; ++b) {
-        if (b >= live) break;                                        // the same for the whole workgroup
-        float M = NEG_INF, sum = 0.f;
+    for (int i = 0; i < 4; ++i) M = fmaxf(M, sm[i][c]);
+    const float base = M == NEG_INF ? 0.f : M;
 #pragma unroll
-        for (int i = 0; i < 4; ++i) M = fmaxf(M, sm[b][i][c]);
-        const float base = M == NEG_INF ? 0.f : M;
+    for (int i = 0; i < 4; ++i) sum += sl[i][c] * exp2_(sm[i][c] - base);
+    const float corr = exp2_(m - base);
 #pragma unroll
-        for (int i = 0; i < 4; ++i) sum += sl[b][i][c] * exp2_(sm[b][i][c] - base);
-        const float corr = exp2_(m[b] - base);
-        if (b) __syncthreads();
+    for (int d = 0; d < DB; ++d) *reinterpret_cast<f32x4 *>(so + (w * 16 + c) * DP + d * 16 + g * 4) = o[d] * corr;
+    __syncthreads();
+    if ((int64_t)cb * 16 + c >= n) return;
+    const int64_t item = (int64_t)row * A.a.H + head;
+    const float inv = A.splits > 1 ? 1.f : sum == 0.f ? 0.f : 1.f / sum;
 #pragma unroll
-        for (int d = 0; d < DB; ++d) *reinterpret_cast<f32x4 *>(so + (w * 16 + c) * DP + d * 16 + g * 4) = o[b][d] * corr;
-        __syncthreads();
-        if ((int64_t)(cb + b) * 16 + c >= n) continue;
-        const int64_t item = (int64_t)row[b] * A.a.H + head[b];
-        const float inv = A.splits > 1 ? 1.f : sum == 0.f ? 0.f : 1.f / sum;
+    for (int d = 0; d < DB; ++d) {                                   // every wave sums and stores its share of the columns
+        if (d % 4 != w) continue;
+        f32x4 acc = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll
-        for (int d = 0; d < DB; ++d) {                               // every wave sums and stores its share of the columns
-            if (d % 4 != w) continue;
-            f32x4 acc = {0.f, 0.f, 0.f, 0.f};
-#pragma unroll
-            for (int i = 0; i < 4; ++i) acc += *reinterpret_cast<const f32x4 *>(so + (i * 16 + c) * DP + d * 16 + g * 4);
-            if (A.splits > 1) store4(A.part + (item * A.splits + split) * A.a.D, acc, d * 16 + g * 4, A.a.D, A.a.D % 4 == 0);
-            else store4(reinterpret_cast<T *>(A.a.out) + item * A.a.D, acc * inv, d * 16 + g * 4, A.a.D, A.a.o_vec != 0);
-        }
-        if (A.splits > 1 && w == 0 && g == 0) {
-            A.stat[(item * A.splits + split) * 2] = M;
-            A.stat[(item * A.splits + split) * 2 + 1] = sum;
-        }
+        for (int i = 0; i < 4; ++i) acc += *reinterpret_cast<const f32x4 *>(so + (i * 16 + c) * DP + d * 16 + g * 4);
+        if (A.splits > 1) store4(A.part + (item * A.splits + split) * A.a.D, acc, d * 16 + g * 4, A.a.D, A.a.D % 4 == 0);
+        else store4(reinterpret_cast<T *>(A.a.out) + item * A.a.D, acc * inv, d * 16 + g * 4, A.a.D, A.a.o_vec != 0);
+    }
+    if (A.splits > 1 && w == 0 && g == 0) {
+        A.stat[(item * A.splits + split) * 2] = M;
+        A.stat[(item * A.splits + split) * 2 + 1] = sum;
     }
 }
 
@@ -252,22 +220,17 @@ template <typename T, int TP> __global__ __launch_bounds__(256) void scene_attn_
     if ((int64_t)blockIdx.x * IT + it < items) store4(reinterpret_cast<T *>(A.a.out) + item * D, o * inv, d, D, A.a.o_vec != 0);
 }
 
-template <typename T, int DP, int CB, bool CAP, int AX> hipError_t launch_step(const SceneStepArgs &A, hipStream_t st) {
+template <typename T, int DP, bool CAP, int AX> hipError_t launch_step(const SceneStepArgs &A, hipStream_t st) {
     const int64_t blocks = (int64_t)A.scenes * A.a.KV * A.splits * A.cblocks, items = (int64_t)A.a.nq * A.a.H;
-    hipLaunchKernelGGL((scene_attn_step_kernel<T, DP, CB, CAP, AX>), dim3((unsigned)blocks), dim3(256), 0, st, A);
+    hipLaunchKernelGGL((scene_attn_step_kernel<T, DP, CAP, AX>), dim3((unsigned)blocks), dim3(256), 0, st, A);
     if (A.splits > 8) hipLaunchKernelGGL((scene_attn_join_kernel<T, 256>), dim3((unsigned)items), dim3(256), 0, st, A);
     else if (A.splits > 1) hipLaunchKernelGGL((scene_attn_join_kernel<T, 64>), dim3((unsigned)((items + 3) / 4)), dim3(256), 0, st, A);
     return hipGetLastError();
 }
-template <typename T, int DP, int CB> hipError_t pick_step(const SceneStepArgs &A, hipStream_t st) {
+template <typename T, int DP> hipError_t pick_step(const SceneStepArgs &A, hipStream_t st) {
     const int ax = A.a.axes;
-    if (A.a.cap > 0.f) return ax == 0 ? launch_step<T, DP, CB, true, 0>(A, st) : ax == 1 ? launch_step<T, DP, CB, true, 1>(A, st) : launch_step<T, DP, CB, true, 3>(A, st);
-    return ax == 0 ? launch_step<T, DP, CB, false, 0>(A, st) : ax == 1 ? launch_step<T, DP, CB, false, 1>(A, st) : launch_step<T, DP, CB, false, 3>(A, st);
-}
-// row blocks a workgroup takes at once where there are more than one: what the registers hold
-constexpr int STEP_BLOCKS = 2;
-template <typename T, int DP> hipError_t step_rows(const SceneStepArgs &A, hipStream_t st) {
-    return A.wide ? pick_step<T, DP, STEP_BLOCKS>(A, st) : pick_step<T, DP, 1>(A, st);
+    if (A.a.cap > 0.f) return ax == 0 ? launch_step<T, DP, true, 0>(A, st) : ax == 1 ? launch_step<T, DP, true, 1>(A, st) : launch_step<T, DP, true, 3>(A, st);
+    return ax == 0 ? launch_step<T, DP, false, 0>(A, st) : ax == 1 ? launch_step<T, DP, false, 1>(A, st) : launch_step<T, DP, false, 3>(A, st);
 }
 
 }  // namespace sattn
@@ -277,21 +240,21 @@ template <typename T, int DP> hipError_t step_rows(const SceneStepArgs &A, hipSt
 extern "C" hipError_t dn_scene_attn_step_bf16(const SceneStepArgs *A, hipStream_t st) {
     using namespace sattn;
     const int D = A->a.D;
-    return D <= 32 ? step_rows<bf16, 32>(*A, st) : D <= 64 ? step_rows<bf16, 64>(*A, st) : step_rows<bf16, 128>(*A, st);
+    return D <= 32 ? pick_step<bf16, 32>(*A, st) : D <= 64 ? pick_step<bf16, 64>(*A, st) : pick_step<bf16, 128>(*A, st);
 }
 #else
 extern "C" hipError_t dn_scene_attn_step_f32(const SceneStepArgs *A, hipStream_t st) {
     using namespace sattn;
     const int D = A->a.D;
-    return D <= 16 ? step_rows<float, 16>(*A, st) : D <= 32 ? step_rows<float, 32>(*A, st) : D <= 64 ? step_rows<float, 64>(*A, st) : step_rows<float, 128>(*A, st);
+    return D <= 16 ? pick_step<float, 16>(*A, st) : D <= 32 ? pick_step<float, 32>(*A, st) : D <= 64 ? pick_step<float, 64>(*A, st) : pick_step<float, 128>(*A, st);
 }
-// rows: packed rows of the largest scene; kv_scenes: scenes x kv heads.  Splits of the keys: four workgroups to each of the chip's 256 CUs, but
-// no split below 256 keys of the cache.
-extern "C" void dn_scene_attn_step_shape(int64_t rows, int64_t kv_scenes, int room, int *cblocks, int *splits, int *wide) {
-    const int64_t blocks = (rows + 15) / 16, at_once = blocks > 1 ? sattn::STEP_BLOCKS : 1;
-    *wide = blocks > 1;
-    *cblocks = (int)((blocks + at_once - 1) / at_once);
-    const int64_t groups = kv_scenes * *cblocks, want = (1024 + groups - 1) / groups, most = ((int64_t)room + 255) / 256;
-    *splits = (int)std::max<int64_t>(1, std::min<int64_t>(std::min(want, most), 64));
+// rows: packed rows of the largest scene; kv_scenes: scenes x kv heads.  Splits of the keys: 1536 workgroups in all - two or three full rounds of what the
+// chip's 256 CUs hold at once (1024 left a third of a round at its end: 131 000 keys of 64 rows 215 us, 185 with 1536) - but none below 256 keys of the
+// cache.  Several blocks of 16 rows that share keys are workgroups of their own: one workgroup for two blocks halves the reads, which
+// come from L2 then, but its registers leave half as many waves (2000 keys of 256 scenes, 34 packed rows: 85 us, 70 in blocks of their own).
+extern "C" void dn_scene_attn_step_shape(int64_t rows, int64_t kv_scenes, int room, int *cblocks, int *splits) {
+    *cblocks = (int)((rows + 15) / 16);
+    const int64_t groups = kv_scenes * *cblocks, want = (1536 + groups - 1) / groups, most = ((int64_t)room + 255) / 256;
+    *splits = (int)std::max<int64_t>(1, std::min<int64_t>(std::min(want, most), 128));
 }
 #endif
