@@ -1664,142 +1664,24 @@ class ClipAdam:
 # ---------------------------------------------------------------------------------------------
 # attention over the rows of a scene, rotary positions (public names and argument checks: dagnet_amd.attention)
 # ---------------------------------------------------------------------------------------------
-class _Attn(C.Structure):                       # dagnet_attn
-    _fields_ = [(n, C.c_void_p) for n in ("q", "k", "v", "slopes", "q_pos", "k_pos")] + \
-               [(n, C.c_int64) for n in ("q_row", "q_head", "k_row", "k_head", "v_row", "v_head")] + \
-               [(n, C.c_int32) for n in ("nq", "nk", "n_heads", "n_kv_heads", "head_dim", "axes", "dtype", "max_keys", "mean_keys")] + \
-               [("scale", C.c_float), ("softcap", C.c_float)]
+_calls = None
+_raw_stream = getattr(torch._C, "_cuda_getCurrentRawStream", None)
 
 
-def _addr(t):
-    return None if t is None else t.data_ptr()
-
-
-def _attn_struct(q, k, v, slopes, pos, k_pos, nk, span, scale, softcap):
-    """q [nq, H, D], k and v [..., KV, D] (their row and head strides are those of the last three dimensions)."""
-    qs, ks, vs, (n, H, D) = q.stride(), k.stride(), v.stride(), q.shape
-    if slopes is None:
-        sl = qp = kp = None
-        axes = 0
-    else:
-        sl, qp, kp, axes = slopes.data_ptr(), pos.data_ptr(), k_pos.data_ptr(), pos.shape[-1]
-    return _Attn(q.data_ptr(), k.data_ptr(), v.data_ptr(), sl, qp, kp, qs[0], qs[1], ks[-3], ks[-2], vs[-3], vs[-2], n, nk, H, k.shape[-2], D, axes,
-                 q.dtype is torch.bfloat16, span[0], span[1], scale, softcap)
-
-
-_raw_stream = torch._C._cuda_getCurrentRawStream if hasattr(torch._C, "_cuda_getCurrentRawStream") else None
-_same = contextlib.nullcontext()
-
-
-def _on(index: int):
-    """The calls launch on the CURRENT device; tensors of another one make it current for the call."""
-    return _same if index == torch._C._cuda_getDevice() else torch.cuda.device(index)
-
-
-def _heads(t: torch.Tensor) -> torch.Tensor:
-    """A gradient as autograd hands it over -> unit column stride."""
-    return t if t.stride(-1) == 1 or t.shape[-1] == 1 else t.contiguous()
-
-
-def scene_attn(q, k, v, slopes, tables, scale, softcap, pos, k_pos, grad):
-    """dagnet_op_attn_fwd -> out; with ``grad`` also the call's arguments, the rows' statistics and the unrounded output (else None)."""
-    index, fp32 = q.get_device(), q.dtype is torch.float32
-    out = torch.empty_like(q, memory_format=torch.contiguous_format)
-    lse = o32 = None
-    if grad:
-        lse = q.new_empty(q.shape[0] * q.shape[1], dtype=torch.float32)
-        o32 = None if fp32 else q.new_empty(q.shape, dtype=torch.float32)
-    a = _attn_struct(q, k, v, slopes, pos, k_pos, k.shape[0], tables[5], scale, softcap)
-    lib, ref = _lib(), C.byref(a)
-    n = lib.dagnet_op_attn_fwd_workspace(ref)
-    ws = q.new_empty(n, dtype=torch.float32) if n else None          # of its own: captured calls must not share one
-    with _on(index):
-        _check(lib.dagnet_op_attn_fwd(ref, tables[0], tables[1], out.data_ptr(), _addr(lse), _addr(o32), _addr(ws), _raw_stream(index)))
-    return out, a, lse, (out if fp32 else o32) if grad else None
-
-
-class SceneAttnFn(torch.autograd.Function):
-    """Attention over the rows of a scene (include/dagnet_hip.h, dagnet_op_attn_fwd / _bwd).  ``tables``: layout.tables(device)."""
-
-    @staticmethod
-    def forward(ctx, q, k, v, slopes, tables, scale, softcap, pos, k_pos):
-        out, a, lse, o = scene_attn(q, k, v, slopes, tables, scale, softcap, pos, k_pos, True)
-        # saved: what the call's addresses point to, watched for changes in place; the output too where the backward reads it (fp32)
-        ctx.save_for_backward(q, k, v, slopes, pos, k_pos, out if o is out else None)
-        ctx.meta = (a, _lib().dagnet_op_attn_bwd_workspace(C.byref(a)), tables, lse, None if o is out else o)
-        return out
-
-    @staticmethod
-    @torch.autograd.function.once_differentiable
-    def backward(ctx, dout):
-        a, n, tables, lse, o = ctx.meta
-        q, k, v, slopes, _, _, out = ctx.saved_tensors
-        need_q, need_k, need_v, need_s = ctx.needs_input_grad[:4]
-        dout = _heads(dout)
-        index, gs = q.get_device(), dout.stride()
-        dense = torch.contiguous_format
-        dq = torch.empty_like(q, memory_format=dense) if need_q or need_s else None
-        dk, dv = (torch.empty_like(k, memory_format=dense), torch.empty_like(v, memory_format=dense)) if need_k or need_v else (None, None)
-        ds = torch.empty_like(slopes) if need_s else None
-        ws = lse.new_empty(n)
-        with _on(index):
-            _check(_lib().dagnet_op_attn_bwd(C.byref(a), *tables[:4], dout.data_ptr(), gs[0], gs[1], lse.data_ptr(), (out if o is None else o).data_ptr(),
-                                             ws.data_ptr(), _addr(dq), _addr(dk), _addr(dv), _addr(ds), _raw_stream(index)))
-        return dq if need_q else None, dk if need_k else None, dv if need_v else None, ds, None, None, None, None, None
-
-
-def scene_attn_step(q, k, v, k_len, q_ptr, max_rows, slopes, pos, k_pos, scale, softcap):
-    """dagnet_op_attn_step: k, v [S, room, KV, D]; q_ptr, k_len int32 device tensors."""
-    S, room = k.shape[:2]
-    index = q.get_device()
-    out = torch.empty_like(q, memory_format=torch.contiguous_format)
-    a = _attn_struct(q, k, v, slopes, pos, k_pos, 0, (0, 0), scale, softcap)
-    lib, ref = _lib(), C.byref(a)
-    n = lib.dagnet_op_attn_step_workspace(ref, S, room, max_rows)
-    ws = q.new_empty(n, dtype=torch.float32) if n else None
-    with _on(index):
-        _check(lib.dagnet_op_attn_step(ref, q_ptr, k_len.data_ptr(), S, room, max_rows, k.stride(0), v.stride(0), out.data_ptr(), _addr(ws),
-                                       _raw_stream(index)))
-    return out
-
-
-_POS_TYPES = {torch.float32: 0, torch.int32: 1, torch.int64: 2}
-
-
-def rotary_apply(q, k, pos, tables, pairs, interleaved, inverse, qo, ko):
-    """dagnet_op_rotary: writes qo (and ko); k and ko may be None."""
-    (n, hq, D), qs, qos, index = q.shape, q.stride(), qo.stride(), q.get_device()
-    if k is None:
-        hk, kp, kop, ks, kos = 0, None, None, (0, 0), (0, 0)
-    else:
-        hk, kp, kop, ks, kos = k.shape[1], k.data_ptr(), ko.data_ptr(), k.stride(), ko.stride()
-    with _on(index):
-        _check(_lib().dagnet_op_rotary(n, hq, hk, D, q.dtype is torch.bfloat16, q.data_ptr(), qs[0], qs[1], kp, ks[0], ks[1], pos.data_ptr(),
-                                       _POS_TYPES[pos.dtype], pos.shape[1], tables[0], tables[1], pairs, interleaved, inverse, qo.data_ptr(), qos[0],
-                                       qos[1], kop, kos[0], kos[1], _raw_stream(index)))
-
-
-def rotary_new(q, k, pos, tables, pairs, interleaved, inverse=False):
-    dense = torch.contiguous_format
-    qo = torch.empty_like(q, memory_format=dense)
-    ko = None if k is None else torch.empty_like(k, memory_format=dense)
-    rotary_apply(q, k, pos, tables, pairs, interleaved, inverse, qo, ko)
-    return qo, ko
-
-
-class RotaryFn(torch.autograd.Function):
-    """(q, k or None) turned by their positions; the gradient is the same turn backwards."""
-
-    @staticmethod
-    def forward(ctx, q, k, pos, tables, pairs, interleaved):
-        ctx.save_for_backward(pos)
-        ctx.meta = (tables, pairs, interleaved, k is not None)
-        return rotary_new(q, k, pos, tables, pairs, interleaved)
-
-    @staticmethod
-    @torch.autograd.function.once_differentiable
-    def backward(ctx, gq, gk):
-        pos, = ctx.saved_tensors
-        tables, pairs, interleaved, has_k = ctx.meta
-        dq, dk = rotary_new(_heads(gq), _heads(gk) if has_k else None, pos, tables, pairs, interleaved, True)
-        return dq, dk, None, None, None, None
+def calls():
+    """The compiled callers of dagnet_op_attn_* and dagnet_op_rotary with their autograd nodes (csrc/torch_calls.cpp), bound to the loaded
+    library's entries: scene_attn, scene_attn_step, rotary."""
+    global _calls
+    if _calls is None:
+        import importlib.util
+        path = os.path.join(os.path.dirname(os.path.abspath(__file__)), "_lib", "_dagnet_torch.so")
+        if not os.path.exists(path):
+            raise DagnetHipError(f"{path} not found: build it with `make -C dagnet_amd/csrc`. There is no fallback.")
+        spec = importlib.util.spec_from_file_location("_dagnet_torch", path)
+        m = importlib.util.module_from_spec(spec)
+        spec.loader.exec_module(m)
+        lib = _lib()
+        names = ("dagnet_last_error",) + tuple(n for n in OP_EXPORTS if n.startswith("dagnet_op_attn_")) + ("dagnet_op_rotary",)
+        m.bind({n: C.cast(getattr(lib, n), C.c_void_p).value for n in names}, DagnetHipError)
+        _calls = m
+    return _calls

@@ -8,7 +8,8 @@ the graph layers (gat.py, gcn.py) by attention over a scene's agents, or over it
     out = scene_attention(q, k, v, layout, softcap=30.0, slopes=slopes, pos=pos)           # differentiable
     out = scene_attention_step(q, k_cache, v_cache, k_len, step_layout)                    # the new rows of a rollout's step
 
-The kernels are csrc/scene_attn_*.hip and csrc/rotary.hip behind dagnet_op_attn_* and dagnet_op_rotary (include/dagnet_hip.h).  fp32 and
+The kernels are csrc/scene_attn_*.hip and csrc/rotary.hip behind dagnet_op_attn_* and dagnet_op_rotary (include/dagnet_hip.h), called
+by csrc/torch_calls.cpp.  fp32 and
 bf16; there is no CPU path.
 """
 from __future__ import annotations
@@ -23,6 +24,7 @@ from . import _ops
 from ._capi import DagnetHipError
 
 _TYPES = (torch.float32, torch.bfloat16)
+_POSITIONS = (torch.float32, torch.int32, torch.int64)
 
 
 class _Tables:
@@ -230,10 +232,7 @@ def scene_attention(q, k, v, layout: SceneLayout, *, scale: Optional[float] = No
         slopes = slopes.contiguous()
         if pos is None:
             pos, k_pos = layout.places(index)
-    q, k, v, tables = _columns(q), _columns(k), _columns(v), layout.tables(index)
-    if torch.is_grad_enabled() and (q.requires_grad or k.requires_grad or v.requires_grad or (slopes is not None and slopes.requires_grad)):
-        return _ops.SceneAttnFn.apply(q, k, v, slopes, tables, scale, softcap, pos, k_pos)
-    return _ops.scene_attn(q, k, v, slopes, tables, scale, softcap, pos, k_pos, False)[0]
+    return _ops.calls().scene_attn(_columns(q), _columns(k), _columns(v), slopes, layout.tables(index), scale, softcap, pos, k_pos)
 
 
 def scene_attention_step(q, k_cache, v_cache, k_len, layout: SceneLayout, *, scale: Optional[float] = None, softcap: float = 0.0, slopes=None,
@@ -270,8 +269,8 @@ def scene_attention_step(q, k_cache, v_cache, k_len, layout: SceneLayout, *, sca
             raise DagnetHipError(f"pos has {pos.shape[-1]} axes and k_pos {k_pos.shape[-1]}")
         slopes = slopes.contiguous()
     index = _check_device("q k_cache v_cache k_len slopes pos k_pos", q, k_cache, v_cache, k_len, slopes, pos, k_pos)
-    return _ops.scene_attn_step(_columns(q), _columns(k_cache), _columns(v_cache), k_len.contiguous(), layout.tables(index)[4], layout.max_rows, slopes, pos,
-                                k_pos, scale, softcap)
+    return _ops.calls().scene_attn_step(_columns(q), _columns(k_cache), _columns(v_cache), k_len.contiguous(), layout.tables(index)[4], layout.max_rows,
+                                        slopes, pos, k_pos, scale, softcap)
 
 
 class RotaryAxes(_Tables):
@@ -315,21 +314,16 @@ def rotary(q, k, pos, axes: RotaryAxes, *, inplace: bool = False):
             raise DagnetHipError(f"q and k must both be fp32 or both bf16 (got {name} {t.dtype})")
         if t.shape[0] != q.shape[0] or t.shape[2] != axes.head_dim or t.shape[1] < 1:
             raise DagnetHipError(f"{name} must be [{q.shape[0]}, heads, {axes.head_dim}], got {tuple(t.shape)}")
-    if not isinstance(pos, torch.Tensor) or pos.dtype not in _ops._POS_TYPES or tuple(pos.shape) != (q.shape[0], axes.axes):
+    if not isinstance(pos, torch.Tensor) or pos.dtype not in _POSITIONS or tuple(pos.shape) != (q.shape[0], axes.axes):
         raise DagnetHipError(f"pos must be fp32, int32 or int64 [{q.shape[0]}, {axes.axes}]")
     if pos.requires_grad and torch.is_grad_enabled():
         raise DagnetHipError("pos: positions have no gradient here; pass pos.detach()")
-    grad = torch.is_grad_enabled() and any(t.requires_grad for _, t in both)
     if inplace:
-        if grad:
+        if torch.is_grad_enabled() and any(t.requires_grad for _, t in both):
             raise DagnetHipError("rotary(inplace=True) has no gradient: call it under torch.no_grad()")
         for name, t in both:
             if t.stride(-1) != 1 and t.shape[-1] > 1 or any(s == 0 and n > 1 for s, n in zip(t.stride(), t.shape)):
                 raise DagnetHipError(f"rotary(inplace=True): {name} must have unit column stride and rows of its own (strides {t.stride()})")
     tables = axes.tables(_check_device("q k pos", q, k, pos))
-    pos = pos.contiguous()
-    if inplace:
-        _ops.rotary_apply(q, k, pos, tables, axes.n_pairs, axes.interleaved, False, q, k)
-        return q, k
-    q, k = _columns(q), None if k is None else _columns(k)
-    return (_ops.RotaryFn.apply if grad else _ops.rotary_new)(q, k, pos, tables, axes.n_pairs, axes.interleaved)
+    q, k = (q, k) if inplace else (_columns(q), None if k is None else _columns(k))
+    return _ops.calls().rotary(q, k, pos.contiguous(), tables, axes.n_pairs, axes.interleaved, inplace)

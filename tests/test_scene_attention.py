@@ -118,13 +118,32 @@ def test_rotary_frequencies():
     assert np.allclose(t[:96].view(np.float64) * 2 * np.pi, a.freq, rtol=1e-15) and t[96:].view(np.int32).tolist() == a.axis.tolist()
 
 
+class _Attn(C.Structure):                       # dagnet_attn
+    _fields_ = [(n, C.c_void_p) for n in ("q", "k", "v", "slopes", "q_pos", "k_pos")] + \
+               [(n, C.c_int64) for n in ("q_row", "q_head", "k_row", "k_head", "v_row", "v_head")] + \
+               [(n, C.c_int32) for n in ("nq", "nk", "n_heads", "n_kv_heads", "head_dim", "axes", "dtype", "max_keys", "mean_keys")] + \
+               [("scale", C.c_float), ("softcap", C.c_float)]
+
+
+def test_the_callers_load_and_bind():
+    m = _ops.calls()
+    assert m is _ops.calls() and all(hasattr(m, n) for n in ("scene_attn", "scene_attn_step", "rotary"))
+
+
+def test_missing_callers_fail_loudly(monkeypatch):
+    monkeypatch.setattr(_ops, "_calls", None)
+    monkeypatch.setattr(_ops.os.path, "exists", lambda p: not p.endswith("_dagnet_torch.so"))
+    with pytest.raises(DagnetHipError, match="no fallback"):
+        _ops.calls()
+
+
 def test_c_entries_refuse_before_any_launch():
     """Status and message, no exception across the boundary; none of these reaches a kernel."""
     lib = _ops._lib()
     ok = dict(nq=4, nk=4, n_heads=2, n_kv_heads=1, head_dim=16, axes=0, dtype=0, scale=1.0, softcap=0.0, q=64, k=64, v=64)
 
     def rc(**kw):
-        a = _ops._Attn(**{**ok, **kw})
+        a = _Attn(**{**ok, **kw})
         return lib.dagnet_op_attn_fwd(C.byref(a), *[None] * 7)
     for kw, word in ((dict(head_dim=129), b"head_dim"), (dict(head_dim=0), b"head_dim"), (dict(n_heads=3, n_kv_heads=2), b"multiple"), (dict(dtype=2), b"dtype"),
                      (dict(axes=4), b"axes"), (dict(max_keys=-1), b"max_keys"), (dict(nq=-1), b"row counts"), (dict(softcap=float("nan")), b"softcap"), (dict(scale=float("inf")), b"scale"),
@@ -132,7 +151,7 @@ def test_c_entries_refuse_before_any_launch():
         assert rc(**kw) == -1 and word in lib.dagnet_last_error()
     assert lib.dagnet_op_attn_fwd(None, *[None] * 7) == -1
     assert rc(nq=0, q=None) == 0
-    a = _ops._Attn(**ok)
+    a = _Attn(**ok)
     assert lib.dagnet_op_attn_bwd(C.byref(a), *[None] * 5, 0, 0, *[None] * 3, 64, 64, None, None, None) == -1 and b"dk and dv" in lib.dagnet_last_error()
     assert lib.dagnet_op_attn_bwd(C.byref(a), *[None] * 5, 0, 0, *[None] * 3, 64, None, None, 64, None) == -1 and b"dslopes" in lib.dagnet_last_error()
     assert lib.dagnet_op_attn_bwd_workspace(C.byref(a)) >= 16
