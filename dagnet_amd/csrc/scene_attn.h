@@ -251,6 +251,12 @@ __device__ __forceinline__ float group_sum(float v) {
     return __uint_as_float(b[0]) + __uint_as_float(b[1]);
 }
 
+// packed row -> (row, head within its group); 32-bit division where it does (a 64-bit one is over a hundred instructions)
+__device__ __forceinline__ int row_of(int64_t r, int G) {
+    if (G == 1) return (int)r;
+    return r <= 0xffffffffll ? (int)((uint32_t)r / (uint32_t)G) : (int)(r / G);
+}
+
 // Row c of the wave (all four lane groups hold the same), as the kernels keep it per lane.
 struct RowState {
     int row, head, lo, hi;
@@ -260,7 +266,7 @@ struct RowState {
 __device__ __forceinline__ RowState row_state(const SceneAttnArgs &A, int kvh, int64_t r, int64_t R) {
     RowState s;
     const int64_t rr = r < R ? r : R - 1;
-    s.row = (int)(rr / A.G);
+    s.row = row_of(rr, A.G);
     s.head = kvh * A.G + (int)(rr - (int64_t)s.row * A.G);
     s.lo = max(A.row_lo[s.row], 0);
     s.hi = min(A.row_hi[s.row], A.nk);
@@ -279,15 +285,15 @@ __device__ __forceinline__ float uniform(float v) { return __uint_as_float(__bui
 
 // Which tile a workgroup takes, heaviest first in rounds of one workgroup a CU, every other round backwards: a CU that got a heavy tile
 // in one round gets a light one in the next.  (Causal masks: tiles differ by the length of the sequence.)  n: tiles, i: 0 .. n - 1, per: rounds' length.
-__device__ __forceinline__ int64_t snake(int64_t i, int64_t n, int per) {
-    const int64_t r = i / per, in = i - r * per, len = min((int64_t)per, n - r * per);
-    return r * per + (r & 1 ? len - 1 - in : in);
+__device__ __forceinline__ int snake(uint32_t i, uint32_t n, uint32_t per) {
+    const uint32_t r = i / per, in = i - r * per, len = min(per, n - r * per);
+    return (int)(r * per + (r & 1 ? len - 1 - in : in));
 }
 constexpr int CUS = 256;
 
 // part i of n of the keys lo .. hi - 1, in whole tiles of BN
 template <int BN> __device__ __forceinline__ void key_part(int &lo, int &hi, int i, int n) {
-    const int64_t per = ((max(hi - lo, 0) + (int64_t)n * BN - 1) / ((int64_t)n * BN)) * BN, at = lo + per * i;
+    const int64_t per = (int64_t)(((uint32_t)max(hi - lo, 0) + (uint32_t)(n * BN) - 1) / (uint32_t)(n * BN)) * BN, at = lo + per * i;
     lo = (int)min(at, (int64_t)hi);
     hi = (int)min(at + per, (int64_t)hi);
 }
@@ -321,7 +327,8 @@ template <int AX, int N> __device__ __forceinline__ void read_positions(const fl
 // coordinates) are compiled in: the kernels are bound by vector instructions per score, not by the products.
 // Capped: with s = raw^2 the rational tanh_near() and both factors become raw (k + s (n1 + s n2)) / (1 + s (d1 + s d2)), eight instructions.
 // Scores of a trained model lie well inside the cap, so a wave seldom takes the form for |raw| >= edge.
-template <bool CAP, int AX> struct Score {
+// FINE (fp32): quotient and root to half an ulp - a score of 30 off by one more ulp is 2e-6 in its probability.
+template <bool CAP, int AX, bool FINE> struct Score {
     float k, arg, cap2, inv2, edge, n1, n2, d1, d2;
     __device__ __forceinline__ Score(const SceneAttnArgs &A) : k(uniform(A.scale * LOG2E)) {
         if constexpr (CAP) {
@@ -357,7 +364,9 @@ template <bool CAP, int AX> struct Score {
 #pragma unroll
                 for (int i = 0; i < 4; ++i) {
                     const float s = x[n][i] * x[n][i];
-                    x[n][i] = x[n][i] * fmaf(s, fmaf(s, n2, n1), k) * rcp_(fmaf(s, fmaf(s, d2, d1), 1.f));
+                    const float num = x[n][i] * fmaf(s, fmaf(s, n2, n1), k), den = fmaf(s, fmaf(s, d2, d1), 1.f), r = rcp_(den);
+                    x[n][i] = num * r;
+                    if constexpr (FINE) x[n][i] = fmaf(fmaf(-den, x[n][i], num), r, x[n][i]);
                 }
         }
     }
@@ -368,7 +377,10 @@ template <bool CAP, int AX> struct Score {
     }
     static __device__ __forceinline__ float dist(float x, float y, float z) {
         if constexpr (AX == 1) return fabsf(x);
-        return __builtin_amdgcn_sqrtf(x * x + y * y + z * z);
+        const float q = x * x + y * y + z * z;
+        float r = __builtin_amdgcn_sqrtf(q);
+        if constexpr (FINE) r = q > 0.f ? fmaf(fmaf(-r, r, q), 0.5f * rcp_(r), r) : r;
+        return r;
     }
     // of one row's position to four positions
     static __device__ __forceinline__ f32x4 dist4(const float *a, f32x4 px, f32x4 py, f32x4 pz) {

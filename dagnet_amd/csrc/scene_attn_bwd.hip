@@ -191,9 +191,10 @@ __global__ __launch_bounds__(256) void scene_attn_dq_kernel(const SceneAttnArgs 
     __shared__ __attribute__((aligned(16))) float sp[2][AX ? AX : 1][BN];
     const int tid = threadIdx.x, lane = tid & 63, w = tid >> 6, g = lane >> 4, c = lane & 15;
     const int kvh = (int)(blockIdx.x % A.KV), both = A.KV * A.key_parts, part = (int)(blockIdx.x / A.KV % A.key_parts);
-    const int64_t R = (int64_t)A.nq * A.G, tiles = gridDim.x / both, r0 = (tiles - 1 - snake(blockIdx.x / both, tiles, max(CUS / both, 1))) * ROWS;
-    const Score<CAP, AX> S(A);
-    const int qa = (int)(r0 / A.G), qb = (int)((min(r0 + ROWS, R) - 1) / A.G);
+    const int tiles = gridDim.x / both;
+    const int64_t R = (int64_t)A.nq * A.G, r0 = (int64_t)(tiles - 1 - snake(blockIdx.x / both, tiles, max(CUS / both, 1))) * ROWS;
+    const Score<CAP, AX, sizeof(T) == 4> S(A);
+    const int qa = row_of(r0, A.G), qb = row_of(min(r0 + ROWS, R) - 1, A.G);
     int tlo = uniform(max(A.row_lo[qa], 0)), thi = uniform(min(A.row_hi[qb], A.nk));
     if (A.key_parts > 1) key_part<BN>(tlo, thi, part, A.key_parts);
     const T *K = reinterpret_cast<const T *>(A.k) + kvh * A.k_hs, *V = reinterpret_cast<const T *>(A.v) + kvh * A.v_hs;
@@ -379,11 +380,11 @@ __global__ __launch_bounds__(256, DP <= 32 ? 4 : DP <= 96 ? 3 : 2) void scene_at
     const int kvh = (int)(blockIdx.x % A.KV), part = (int)(blockIdx.x / A.KV % A.parts);
     const int64_t R = (int64_t)A.nq * A.G;
     const int both = A.KV * A.parts, k0 = (int)snake(blockIdx.x / both, gridDim.x / both, max(CUS / both, 1)) * KEYS, kw = k0 + w * 16 * MB;
-    const Score<CAP, AX> S(A);
+    const Score<CAP, AX, sizeof(T) == 4> S(A);
     // the packed rows that see the workgroup's keys (this part of them)
     int64_t ra = (int64_t)max(A.key_lo[k0], 0) * A.G, rb = (int64_t)min(A.key_hi[min(k0 + KEYS - 1, A.nk - 1)], A.nq) * A.G;
     if (A.parts > 1) {
-        const int64_t per = ((rb - ra + A.parts - 1) / A.parts + BM - 1) / BM * BM;
+        const int64_t n = max(rb - ra, (int64_t)0) + A.parts - 1, per = ((n <= 0xffffffffll ? (int64_t)((uint32_t)n / (uint32_t)A.parts) : n / A.parts) + BM - 1) / BM * BM;
         ra += per * part;
         rb = min(rb, ra + per);
     }
@@ -395,7 +396,7 @@ __global__ __launch_bounds__(256, DP <= 32 ? 4 : DP <= 96 ? 3 : 2) void scene_at
     tg.offsets([&](int r) { return (uint32_t)((r / A.G * A.do_rs + r % A.G * A.do_hs) * sizeof(T)); }, A.D);
     auto issue = [&](int64_t rbase, int buf) {              // rows behind the last one: the last one again, masked below
         auto at = [&](int r, int64_t rs, int64_t hs) {
-            const int64_t rr = min(rbase + r, rb - 1), row = A.G == 1 ? rr : rr / A.G;
+            const int64_t rr = min(rbase + r, rb - 1), row = row_of(rr, A.G);
             return row * rs + (kvh * A.G + (rr - row * A.G)) * hs;
         };
         const T *Q = reinterpret_cast<const T *>(A.q), *G = reinterpret_cast<const T *>(A.dout);
@@ -406,7 +407,7 @@ __global__ __launch_bounds__(256, DP <= 32 ? 4 : DP <= 96 ? 3 : 2) void scene_at
             tq.any(sq[buf], [&](int r) { return Q + at(r, A.q_rs, A.q_hs); }, A.D, A.q_vec);
             tg.any(sg[buf], [&](int r) { return G + at(r, A.do_rs, A.do_hs); }, A.D, A.do_vec);
         }
-        const int64_t rr = min(rbase + lane, rb - 1), row = A.G == 1 ? rr : rr / A.G;
+        const int64_t rr = min(rbase + lane, rb - 1), row = row_of(rr, A.G);
         if (w == 0) {
             stage_values<BM>(srow[buf][0], A.lse + kvh * R + rr);
             stage_values<BM>(srow[buf][1], A.delta + kvh * R + rr);

@@ -53,14 +53,15 @@ __global__ __launch_bounds__(256, MB == 2 ? 2 : 3) void scene_attn_fwd_kernel(co
     __shared__ __attribute__((aligned(16))) float sp[2][AX ? AX : 1][BN];
     const int tid = threadIdx.x, lane = tid & 63, w = tid >> 6, g = lane >> 4, c = lane & 15;
     const int kvh = (int)(blockIdx.x % A.KV), both = A.KV * A.key_parts, part = (int)(blockIdx.x / A.KV % A.key_parts);
-    const int64_t R = (int64_t)A.nq * A.G, tiles = gridDim.x / both, r0 = (tiles - 1 - snake(blockIdx.x / both, tiles, max(CUS / both, 1))) * ROWS;
-    const Score<CAP, AX> S(A);
+    const int tiles = gridDim.x / both;
+    const int64_t R = (int64_t)A.nq * A.G, r0 = (int64_t)(tiles - 1 - snake(blockIdx.x / both, tiles, max(CUS / both, 1))) * ROWS;
+    const Score<CAP, AX, sizeof(T) == 4> S(A);
     constexpr bool PLAIN = !CAP && AX == 0;                 // scores stay raw until the exponent: 2^(raw k - base) in one fma
     const bool flip = PLAIN && A.scale < 0.f;               // their maximum then needs k >= 0: the sign goes to q
     const float k = flip ? -S.k : S.k;
 
     // the keys of the workgroup's rows; the first two tiles are on their way before anything else is read
-    const int qa = (int)(r0 / A.G), qb = (int)((min(r0 + ROWS, R) - 1) / A.G);
+    const int qa = row_of(r0, A.G), qb = row_of(min(r0 + ROWS, R) - 1, A.G);
     int tlo = uniform(max(A.row_lo[qa], 0)), thi = uniform(min(A.row_hi[qb], A.nk));
     if (A.key_parts > 1) key_part<BN>(tlo, thi, part, A.key_parts);
     const T *K = reinterpret_cast<const T *>(A.k) + kvh * A.k_hs, *V = reinterpret_cast<const T *>(A.v) + kvh * A.v_hs;

@@ -33,7 +33,7 @@ template <typename T, int DP, bool CAP, int AX> __global__ __launch_bounds__(256
     const int len = min(max(A.k_len[sc], 0), A.room);
     const int per = (int)((((int64_t)len + A.splits - 1) / A.splits + 4 * X::KB - 1) / (4 * X::KB)) * (4 * X::KB);   // whole rounds of the four waves
     const int ka = (int)min((int64_t)split * per, (int64_t)len), kz = (int)min((int64_t)ka + per, (int64_t)len);
-    const Score<CAP, AX> S(A.a);
+    const Score<CAP, AX, sizeof(T) == 4> S(A.a);
     const bool flip = PLAIN && A.a.scale < 0.f;
     const float k = flip ? -S.k : S.k;
     const T *K = reinterpret_cast<const T *>(A.a.k) + sc * A.k_ss + kvh * A.a.k_hs, *V = reinterpret_cast<const T *>(A.a.v) + sc * A.v_ss + kvh * A.a.v_hs;
