@@ -38,19 +38,19 @@ template <typename T> __global__ __launch_bounds__(256) void scene_attn_delta_ke
     if (i < n && part == 0) A.delta[(int64_t)kvh * A.nq * A.G + row * A.G + (head - kvh * A.G)] = s;
 }
 
-// dslopes[h] = sum over the rows of what the dq kernel left per packed row; one workgroup per head, fp64, fixed order, eight loads a thread in
+// dslopes[h] = sum over the rows of what the dq kernel left per packed row; one workgroup per head, fp64, fixed order, 16 loads a thread in
 // flight (a workgroup alone is bound by their latency)
 static __global__ __launch_bounds__(1024) void scene_attn_dslope_kernel(int nq, int G, const float *__restrict__ part, float *__restrict__ out) {
     __shared__ double sh[16];
     const int h = blockIdx.x, kvh = h / G, g = h - kvh * G;
     const float *p = part + (int64_t)kvh * nq * G + g;
     double s = 0.0;
-    for (int64_t i = threadIdx.x; i < nq; i += 8192) {
-        float v[8];
+    for (int64_t i = threadIdx.x; i < nq; i += 16384) {
+        float v[16];
 #pragma unroll
-        for (int u = 0; u < 8; ++u) v[u] = i + u * 1024 < nq ? p[(i + u * 1024) * G] : 0.f;
+        for (int u = 0; u < 16; ++u) v[u] = p[min(i + u * 1024, (int64_t)nq - 1) * G];
 #pragma unroll
-        for (int u = 0; u < 8; ++u) s += v[u];
+        for (int u = 0; u < 16; ++u) s += i + u * 1024 < nq ? v[u] : 0.f;
     }
 #pragma unroll
     for (int o = 32; o > 0; o >>= 1) s += __shfl_xor(s, o);
@@ -658,9 +658,11 @@ template <typename T> hipError_t run_bwd(const SceneAttnArgs &A, float *dslopes,
 extern "C" hipError_t dn_scene_attn_bwd_bf16(const SceneAttnArgs *A, float *dslopes, hipStream_t st) { return sattn::run_bwd<sattn::bf16>(*A, dslopes, st); }
 #else
 extern "C" hipError_t dn_scene_attn_bwd_f32(const SceneAttnArgs *A, float *dslopes, hipStream_t st) { return sattn::run_bwd<float>(*A, dslopes, st); }
-// Parts of the rows in the dk / dv kernel: as many as give the chip four workgroups a CU, but none below 512 packed rows.
+// Parts of the rows in the dk / dv kernel: as many as give the chip four workgroups a CU, but none below 256 packed rows.  The whole backward of 1000
+// fp32 rows and keys, 4 heads of 72 to one: 199 us with at least 512, 134 with 256, 122 with 128; of 512 bf16 rows, 8 heads of 32: 54, 35 and 32.  Below
+// 256 the fp32 sums that parts leave (two for every element of k and v) are more than what the tile itself reads.
 extern "C" int dn_scene_attn_bwd_parts(int64_t nq, int64_t nk, int KV, int G) {
-    const int64_t groups = (nk + 63) / 64 * KV, want = groups ? 1024 / groups : 1, most = nq * G / 512;
+    const int64_t groups = (nk + 63) / 64 * KV, want = groups ? 1024 / groups : 1, most = nq * G / 256;
     return (int)(want < 1 || most < 1 ? 1 : want < most ? (want < 16 ? want : 16) : (most < 16 ? most : 16));
 }
 #endif

@@ -327,11 +327,13 @@ extern "C" hipError_t dn_scene_attn_fwd_f32(const SceneAttnArgs *A, hipStream_t 
     return D <= 16 ? pick_fwd<float, 16, 64, 1>(*A, st) : D <= 32 ? pick_fwd<float, 32, 64, 1>(*A, st) : D <= 48 ? pick_fwd<float, 48, 32, 1>(*A, st)
          : D <= 64 ? pick_fwd<float, 64, 32, 1>(*A, st) : D <= 96 ? pick_fwd<float, 96, 32, 1>(*A, st) : pick_fwd<float, 128, 32, 1>(*A, st);
 }
-// Parts of the keys of a row tile, forward and dq, where there are few tiles: none below 256 of the keys that a row sees (most), and as many as give the
+// Parts of the keys of a row tile, forward and dq, where there are few tiles: none below 128 of the keys that a row sees (most), and as many as give the
 // chip's CUs three workgroups each (what their registers and LDS hold) - four where rows see unlike numbers of keys (mean far below most): then the
-// longest tile is what the rest waits for.  4096 causal rows of 8 heads: 102 us in one part, 66 + 8 to join in two; seeing all keys: 92 and 121.
+// longest tile is what the rest waits for.  4096 causal bf16 rows of 8 heads: 102 us in one part, 66 + 8 to join in two; seeing all keys: 92 and 121.
+// The least part, 1000 fp32 rows and keys, 4 heads of 72 to one: 42 us with 256 keys, 37 with 128 (512 keys, 25 and 18), 33 with 64; in bf16 18.4,
+// 18.8 and 18.3 (512 keys of 8 heads of 32: 11.8, 10.7 and 13.0: the join's share grows).
 extern "C" int dn_scene_attn_key_parts(int64_t nq, int KV, int G, int64_t most, int64_t mean) {
-    const int64_t tiles = (nq * G + 63) / 64 * KV, want = tiles ? (3 * mean < 2 * most ? 1024 : 768) / tiles : 1, parts = want < most / 256 ? want : most / 256;
+    const int64_t tiles = (nq * G + 63) / 64 * KV, want = tiles ? (3 * mean < 2 * most ? 1024 : 768) / tiles : 1, parts = want < most / 128 ? want : most / 128;
     return (int)(parts < 1 ? 1 : parts < 8 ? parts : 8);
 }
 #endif
