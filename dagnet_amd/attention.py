@@ -28,10 +28,14 @@ _POSITIONS = (torch.float32, torch.int32, torch.int64)
 
 
 class _Tables:
-    """Small host tables that are uploaded once per device (before a graph capture: a capturing stream refuses the copy)."""
+    """Small host tables that are uploaded once per device (before a graph capture: a capturing stream refuses the copy).  A captured
+    graph replays with their addresses: keep the object as long as the graph."""
 
     def __init__(self):
         self._dev = {}
+
+    def __getstate__(self):               # a copy (deepcopy, pickle) uploads its own: the addresses are this object's
+        return {**self.__dict__, "_dev": {}}
 
     def _host(self) -> torch.Tensor:      # pragma: no cover - overridden
         raise NotImplementedError
@@ -175,8 +179,8 @@ def _check_device(names, *tensors) -> int:
 def _numbers(scale, softcap, D):
     scale = 1.0 / math.sqrt(D) if scale is None else float(scale)
     softcap = float(softcap or 0.0)
-    if not math.isfinite(scale) or not math.isfinite(softcap) or softcap < 0.0:
-        raise DagnetHipError(f"scale and softcap must be finite and softcap not negative (got {scale}, {softcap})")
+    if not abs(scale) <= 1e15 or not (softcap == 0.0 or 1e-15 <= softcap <= 1e15):
+        raise DagnetHipError(f"softcap must be 0 or 1e-15 .. 1e15 and scale within 1e15 (got scale {scale}, softcap {softcap})")
     return scale, softcap
 
 
@@ -301,6 +305,37 @@ class RotaryAxes(_Tables):
         return t.data_ptr(), t.data_ptr() + 8 * self.n_pairs                  # turns per unit (fp64), axis
 
 
+def _apart(a, b) -> bool:
+    """No element of the views a and b of one storage is in both, by what their strides show: one lies behind the other, or they share
+    strides and their columns differ (a fused projection's q and k, by rows or by heads)."""
+    def end(t):
+        return t.storage_offset() + sum((n - 1) * s for n, s in zip(t.shape, t.stride())) + 1
+
+    if not a.numel() or not b.numel() or end(a) <= b.storage_offset() or end(b) <= a.storage_offset():
+        return True
+    step, cols_a, cols_b = 0, 1, 1                     # elements that repeat every step; what stands in a step
+    dims = sorted([(s, n, 0) for s, n in zip(a.stride(), a.shape) if n > 1] + [(s, n, 1) for s, n in zip(b.stride(), b.shape) if n > 1])
+    for i, (s, n, which) in enumerate(dims):
+        step = 0
+        for s2, _, _ in dims[i:]:
+            step = math.gcd(step, s2)
+        gap = (b.storage_offset() - a.storage_offset()) % step if step else 0
+        if step and gap >= cols_a and gap + cols_b <= step:
+            return True
+        cols_a, cols_b = (cols_a + (n - 1) * s, cols_b) if which == 0 else (cols_a, cols_b + (n - 1) * s)
+    return False
+
+
+def _own_elements(t) -> bool:
+    """Every index has an element of its own, by what the strides show."""
+    reach = 1
+    for s, n in sorted((s, n) for s, n in zip(t.stride(), t.shape) if n > 1):
+        if s < reach:
+            return False
+        reach += (n - 1) * s
+    return True
+
+
 def rotary(q, k, pos, axes: RotaryAxes, *, inplace: bool = False):
     """Turns the column pairs of every head of q [n, heads, head_dim] and k [n, key heads, head_dim] (or None) by their row's positions
     pos [n, number of axes] (fp32, int32 or int64) -> (q, k).  Angles are computed in fp64, so positions may lie far from zero.
@@ -322,8 +357,13 @@ def rotary(q, k, pos, axes: RotaryAxes, *, inplace: bool = False):
         if torch.is_grad_enabled() and any(t.requires_grad for _, t in both):
             raise DagnetHipError("rotary(inplace=True) has no gradient: call it under torch.no_grad()")
         for name, t in both:
-            if t.stride(-1) != 1 and t.shape[-1] > 1 or any(s == 0 and n > 1 for s, n in zip(t.stride(), t.shape)):
-                raise DagnetHipError(f"rotary(inplace=True): {name} must have unit column stride and rows of its own (strides {t.stride()})")
+            if t.stride(-1) != 1 and t.shape[-1] > 1 or not _own_elements(t):
+                raise DagnetHipError(f"rotary(inplace=True): {name} must have unit column stride and elements of its own (strides {t.stride()})")
+        store = [t.untyped_storage().data_ptr() for _, t in both]
+        if k is not None and store[0] == store[1] and not _apart(q, k):
+            raise DagnetHipError("rotary(inplace=True): q and k overlap")
+        if pos.untyped_storage().data_ptr() in store:
+            pos = pos.clone()                          # read before anything is overwritten
     tables = axes.tables(_check_device("q k pos", q, k, pos))
     q, k = (q, k) if inplace else (_columns(q), None if k is None else _columns(k))
     return _ops.calls().rotary(q, k, pos.contiguous(), tables, axes.n_pairs, axes.interleaved, inplace)

@@ -2173,6 +2173,9 @@ extern "C" hipError_t dn_scene_attn_step_bf16(const SceneStepArgs *, hipStream_t
 extern "C" void dn_scene_attn_step_shape(int64_t, int64_t, int, int *, int *);
 extern "C" hipError_t dn_rotary(const RotaryArgs *, int, int, hipStream_t);
 
+// workgroups of 256 threads in a launch: the runtime counts its threads in 32 bits (parts and joins multiply small counts only)
+constexpr int64_t ATTN_BLOCKS = 0xffffff;
+
 // bytes per load that a matrix of rows allows
 static int attn_vec(const void *p, int64_t rs, int64_t hs, int D, int size) {
     for (int b = 16; b > size && b >= 8; b /= 2)
@@ -2188,7 +2191,9 @@ static int attn_args(const dagnet_attn *a, SceneAttnArgs *A) {
     OP_NEED(a->nq >= 0 && a->nk >= 0 && a->nq <= 0x7fff0000 && a->nk <= 0x7fff0000, "row counts must be 0 .. 2^31 - 65536");
     OP_NEED(a->max_keys >= 0 && a->mean_keys >= 0, "max_keys and mean_keys must not be negative");
     OP_NEED(a->axes >= 0 && a->axes <= 3, "axes must be 0 .. 3");
-    OP_NEED(a->softcap >= 0.f && a->softcap < INFINITY && a->scale == a->scale && fabsf(a->scale) < INFINITY, "scale and softcap must be finite, softcap not negative");
+    // beyond these bounds scale / softcap and their products leave fp32's range
+    OP_NEED(fabsf(a->scale) <= 1e15f && (a->softcap == 0.f || (a->softcap >= 1e-15f && a->softcap <= 1e15f)),
+            "softcap must be 0 or 1e-15 .. 1e15 and scale within 1e15");
     OP_NEED(a->nq == 0 || a->q, "null q");
     OP_NEED(a->nq == 0 || !a->axes || (a->slopes && a->q_pos), "axes > 0 needs slopes and positions");
     *A = SceneAttnArgs{};
@@ -2203,8 +2208,7 @@ static int attn_args(const dagnet_attn *a, SceneAttnArgs *A) {
     A->v_vec = attn_vec(a->v, a->v_row, a->v_head, a->head_dim, size);
     A->o_vec = a->head_dim % 4 == 0;
     const int64_t tiles = ((int64_t)a->nq * A->G + 63) / 64;
-    OP_NEED(tiles * A->KV <= 0x7fffffffLL && ((int64_t)a->nk + 63) / 64 * A->KV <= 0x7fffffffLL && ((int64_t)a->nq * A->H + 3) / 4 <= 0x7fffffffLL,
-            "too many rows for one launch");
+    OP_NEED(tiles * A->KV <= ATTN_BLOCKS && ((int64_t)a->nk + 63) / 64 * A->KV <= ATTN_BLOCKS, "too many rows for one launch");
     return DAGNET_OK;
 }
 // 4 values at once need a base of that alignment
@@ -2270,7 +2274,6 @@ extern "C" int dagnet_op_attn_bwd(const dagnet_attn *a, const int32_t *row_lo, c
         next = A.stat + up4(items * A.key_parts * 3);
     }
     if (A.parts > 1) A.part2 = next;
-    OP_NEED(((int64_t)a->nk + 63) / 64 * A.KV * A.parts <= 0x7fffffffLL && ((int64_t)a->nk * A.KV + 3) / 4 <= 0x7fffffffLL, "too many keys for one launch");
     if (!attn_base(dq, size) || !attn_base(dk, size) || !attn_base(dv, size)) A.o_vec = 0;
     HIP_TRY(a->dtype ? dn_scene_attn_bwd_bf16(&A, dslopes, OP_ST) : dn_scene_attn_bwd_f32(&A, dslopes, OP_ST));
     return DAGNET_OK;
@@ -2296,7 +2299,7 @@ extern "C" int dagnet_op_attn_step(const dagnet_attn *a, const int32_t *q_ptr, c
     OP_NEED(max_rows >= 1 && q_ptr && k_len && out && (room == 0 || (a->k && a->v && (!a->axes || a->k_pos))), "bad argument");
     A.q_ptr = q_ptr; A.k_len = k_len; A.scenes = scenes; A.room = room; A.k_ss = k_scene; A.v_ss = v_scene;
     step_shape(a, scenes, room, max_rows, &A.cblocks, &A.splits);
-    OP_NEED((int64_t)scenes * a->n_kv_heads * A.cblocks * A.splits <= 0x7fffffffLL, "too many rows for one launch");
+    OP_NEED((int64_t)scenes * a->n_kv_heads <= ATTN_BLOCKS && (int64_t)scenes * a->n_kv_heads * A.cblocks * A.splits <= ATTN_BLOCKS, "too many rows for one launch");
     OP_NEED(A.splits == 1 || workspace, "workspace is NULL");
     const int size = a->dtype ? 2 : 4;
     A.a.out = out;
@@ -2314,6 +2317,7 @@ extern "C" int dagnet_op_rotary(int64_t n, int32_t hq, int32_t hk, int32_t head_
                                 const double *turns, const int32_t *axis, int32_t pairs, int32_t interleaved, int32_t inverse, void *qo,
                                 int64_t qo_row, int64_t qo_head, void *ko, int64_t ko_row, int64_t ko_head, void *stream) {
     OP_NEED(n >= 0 && hq >= 1 && hk >= 0 && (int64_t)hq + hk <= 65536 && head_dim >= 2 && head_dim <= 1024, "bad shape");
+    OP_NEED(n <= 16 * ATTN_BLOCKS, "too many rows for one launch");
     OP_NEED(dtype == 0 || dtype == 1, "dtype must be 0 (fp32) or 1 (bf16)");
     OP_NEED(pos_type >= 0 && pos_type <= 2 && axes >= 1, "bad positions");
     OP_NEED(pairs >= 1 && 2 * pairs <= head_dim, "pairs must be 1 .. head_dim / 2");

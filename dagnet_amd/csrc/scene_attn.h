@@ -39,7 +39,6 @@ struct SceneAttnArgs {
 namespace sattn {
 
 typedef __bf16 bf16;
-typedef __bf16 bf16x4 __attribute__((ext_vector_type(4)));
 typedef __bf16 bf16x8 __attribute__((ext_vector_type(8)));
 typedef float f32x2 __attribute__((ext_vector_type(2)));
 typedef float f32x4 __attribute__((ext_vector_type(4)));
@@ -335,7 +334,7 @@ template <bool CAP, int AX, bool FINE> struct Score {
             arg = uniform(A.scale / A.cap);
             cap2 = uniform(A.cap * LOG2E);
             inv2 = uniform(1.f / cap2);
-            edge = uniform(1.f / fabsf(arg));
+            edge = uniform(fabsf(arg) > 1e-8f && fabsf(arg) < 1e8f ? 1.f / fabsf(arg) : 0.f);      // else arg^4 leaves fp32's range
             const float a2 = arg * arg;
             n1 = uniform(k * a2 * (105.f / 945.f));
             n2 = uniform(k * a2 * a2 * (1.f / 945.f));
@@ -379,7 +378,7 @@ template <bool CAP, int AX, bool FINE> struct Score {
         if constexpr (AX == 1) return fabsf(x);
         const float q = x * x + y * y + z * z;
         float r = __builtin_amdgcn_sqrtf(q);
-        if constexpr (FINE) r = q > 0.f ? fmaf(fmaf(-r, r, q), 0.5f * rcp_(r), r) : r;
+        if constexpr (FINE) r = q > 0.f && q < __builtin_inff() ? fmaf(fmaf(-r, r, q), 0.5f * rcp_(r), r) : r;
         return r;
     }
     // of one row's position to four positions
@@ -391,7 +390,7 @@ template <bool CAP, int AX, bool FINE> struct Score {
     }
 };
 
-// the same with everything read at run time (the slow forms and the step kernel's launch-time choices)
+// the same with everything read at run time (the slow forms)
 __device__ __forceinline__ float score2(const SceneAttnArgs &A, float raw, float inv_cap, float slope2, const float *qpos, const float *kpos) {
     float x = raw * A.scale;
     if (A.cap > 0.f) x = A.cap * tanh_(x * inv_cap);

@@ -143,6 +143,7 @@ template <typename T> __device__ void dq_slow(const SceneAttnArgs &A, int kvh, c
         a0 += e.dz * k0;
         a1 += e.dz * k1;
         sl.add(e);
+        if (e.dz != e.dz) break;                             // every sum is NaN already
     }
     T *out = reinterpret_cast<T *>(A.dq) + ((int64_t)s.row * A.H + s.head) * A.D;
     if (h0) out[lane] = (T)(a0 * A.scale);
@@ -171,6 +172,7 @@ template <typename T> __device__ void dkv_slow(const SceneAttnArgs &A, int kvh, 
         a1 += e.dz * q1;
         b0 += e.p * g0;
         b1 += e.p * g1;
+        if (e.p != e.p) break;                               // every sum is NaN already
     }
     const int64_t at = (key * A.KV + kvh) * A.D;
     T *dk = reinterpret_cast<T *>(A.dk) + at, *dv = reinterpret_cast<T *>(A.dv) + at;
@@ -179,13 +181,13 @@ template <typename T> __device__ void dkv_slow(const SceneAttnArgs &A, int kvh, 
 }
 
 // ---------------------------------------------------------------------------------------------------------------------
-// dq and dslope: 64 MB packed rows a workgroup, 16 MB a wave (columns); K and V tiles in LDS
+// dq and dslope: 64 packed rows a workgroup, 16 a wave (columns); K and V tiles in LDS
 // ---------------------------------------------------------------------------------------------------------------------
-template <typename T, int DP, int BN, int MB, bool CAP, int AX>
+template <typename T, int DP, int BN, bool CAP, int AX>
 __global__ __launch_bounds__(256) void scene_attn_dq_kernel(const SceneAttnArgs A) {
     using X = Tr<T>;
     using L = Tile<T, DP>;
-    constexpr int NF = DP / X::KD, DB = DP / 16, PB = X::KB / 16, NC = BN * L::NCH, ROWS = 64 * MB;
+    constexpr int NF = DP / X::KD, DB = DP / 16, PB = X::KB / 16, NC = BN * L::NCH, ROWS = 64;
     static_assert(BN % X::KB == 0, "tile");
     __shared__ u32x4 sk[2][NC], sv[2][NC];
     __shared__ __attribute__((aligned(16))) float sp[2][AX ? AX : 1][BN];
@@ -216,170 +218,148 @@ __global__ __launch_bounds__(256) void scene_attn_dq_kernel(const SceneAttnArgs 
     if (tlo + BN < thi) issue(tlo + BN, 1);
     clear_positions<AX>(sp[0], A.axes);
     clear_positions<AX>(sp[1], A.axes);
-    RowState s[MB];
-    float lse[MB], delta[MB];
-    typename X::frag qf[MB][NF], gf[MB][NF];
+    const int64_t r = r0 + w * 16 + c;
+    const RowState s = row_state(A, kvh, r, R);
+    typename X::frag qf[NF], gf[NF];
+    const float lse = A.lse[kvh * R + min(r, R - 1)];
+    const T *Q = reinterpret_cast<const T *>(A.q) + s.row * A.q_rs + s.head * A.q_hs;
+    const T *G = reinterpret_cast<const T *>(A.dout) + s.row * A.do_rs + s.head * A.do_hs;
 #pragma unroll
-    for (int b = 0; b < MB; ++b) {
-        const int64_t r = r0 + (w * MB + b) * 16 + c;
-        s[b] = row_state(A, kvh, r, R);
-        lse[b] = A.lse[kvh * R + min(r, R - 1)];
-        const T *Q = reinterpret_cast<const T *>(A.q) + s[b].row * A.q_rs + s[b].head * A.q_hs;
-        const T *G = reinterpret_cast<const T *>(A.dout) + s[b].row * A.do_rs + s[b].head * A.do_hs;
-#pragma unroll
-        for (int f = 0; f < NF; ++f) {
-            qf[b][f] = as_frag<T>(load_chunk<T>(Q, f * X::KD + g * X::CH, A.D, A.q_vec));
-            gf[b][f] = as_frag<T>(load_chunk<T>(G, f * X::KD + g * X::CH, A.D, A.do_vec));
-        }
-        const float *o = A.o32 + ((int64_t)s[b].row * A.H + s[b].head) * A.D;
-        float sum = 0.f;
-#pragma unroll
-        for (int f = 0; f < NF; ++f) sum = delta_chunk<T>(sum, o, gf[b][f], f * X::KD + g * X::CH, A.D, A.o32_vec);
-        delta[b] = group_sum(sum);
-        if (A.dk && part == 0 && g == 0 && r < R) A.delta[kvh * R + r] = delta[b];
+    for (int f = 0; f < NF; ++f) {
+        qf[f] = as_frag<T>(load_chunk<T>(Q, f * X::KD + g * X::CH, A.D, A.q_vec));
+        gf[f] = as_frag<T>(load_chunk<T>(G, f * X::KD + g * X::CH, A.D, A.do_vec));
     }
-    const int wlo = uniform(__shfl(s[0].lo, 0)), whi = uniform(__shfl(s[MB - 1].hi, 15));
-    const int alo = uniform(__shfl(s[MB - 1].lo, 15)), ahi = uniform(__shfl(s[0].hi, 0));
-    f32x4 acc[MB][DB];
-    Slope sl[MB];
+    const float *o = A.o32 + ((int64_t)s.row * A.H + s.head) * A.D;
+    float sum = 0.f;
 #pragma unroll
-    for (int b = 0; b < MB; ++b)
+    for (int f = 0; f < NF; ++f) sum = delta_chunk<T>(sum, o, gf[f], f * X::KD + g * X::CH, A.D, A.o32_vec);
+    const float delta = group_sum(sum);
+    if (part == 0 && g == 0 && r < R) A.delta[kvh * R + r] = delta;
+    const int wlo = uniform(__shfl(s.lo, 0)), whi = uniform(__shfl(s.hi, 15));
+    const int alo = uniform(__shfl(s.lo, 15)), ahi = uniform(__shfl(s.hi, 0));
+    f32x4 acc[DB];
+    Slope sl;
 #pragma unroll
-        for (int d = 0; d < DB; ++d) acc[b][d] = f32x4{0.f, 0.f, 0.f, 0.f};
+    for (int d = 0; d < DB; ++d) acc[d] = f32x4{0.f, 0.f, 0.f, 0.f};
 
     int buf = 0;
     for (int kb = tlo; kb < thi; kb += BN, buf ^= 1) {
         landed();
         __syncthreads();
         if (kb > tlo && kb + BN < thi) issue(kb + BN, buf ^ 1);
-        TileSlope ts[MB];
+        TileSlope ts;
 #pragma unroll
         for (int j = 0; j < BN / X::KB; ++j) {
             const int k0 = kb + j * X::KB, at = j * X::KB;
             if (k0 >= whi || k0 + X::KB <= wlo) continue;
-            f32x4 x[MB][PB], e[MB][PB];
+            f32x4 x[PB], e[PB];
 #pragma unroll
             for (int n = 0; n < PB; ++n) {
-#pragma unroll
-                for (int b = 0; b < MB; ++b) x[b][n] = e[b][n] = f32x4{0.f, 0.f, 0.f, 0.f};
+                x[n] = e[n] = f32x4{0.f, 0.f, 0.f, 0.f};
 #pragma unroll
                 for (int f = 0; f < NF; ++f) {
                     const typename X::frag ka = frag_rows<T, DP>(sk[buf], at + n * 16, f, lane);
                     const typename X::frag va = frag_rows<T, DP>(sv[buf], at + n * 16, f, lane);
-#pragma unroll
-                    for (int b = 0; b < MB; ++b) {
-                        x[b][n] = mma(ka, qf[b][f], x[b][n]);
-                        e[b][n] = mma(va, gf[b][f], e[b][n]);
-                    }
+                    x[n] = mma(ka, qf[f], x[n]);
+                    e[n] = mma(va, gf[f], e[n]);
                 }
             }
-#pragma unroll
-            for (int b = 0; b < MB; ++b) S.template apply<PB>(x[b]);
+            S.template apply<PB>(x);
 #pragma unroll
             for (int n = 0; n < PB; ++n) {
                 f32x4 px = {}, py = {}, pz = {};
                 if constexpr (AX > 0) read_positions<AX>(sp[buf], at + n * 16 + 4 * g, px, py, pz);
+                f32x4 p, ds, dist, t = x[n];
+                p = t - lse;
+                if constexpr (AX > 0) {
+                    dist = S.dist4(s.pos, px, py, pz);
+                    p -= s.slope * dist;
+                }
 #pragma unroll
-                for (int b = 0; b < MB; ++b) {
-                    f32x4 p, ds, dist, t = x[b][n];
-                    p = t - lse[b];
-                    if constexpr (AX > 0) {
-                        dist = S.dist4(s[b].pos, px, py, pz);
-                        p -= s[b].slope * dist;
-                    }
+                for (int i = 0; i < 4; ++i) {
+                    p[i] = exp2_(p[i]);
+                    ds[i] = e[n][i] - delta;
+                }
+                if (k0 + n * 16 < alo || k0 + n * 16 + 16 > ahi) {       // a masked place is 0, not 0 * inf
 #pragma unroll
                     for (int i = 0; i < 4; ++i) {
-                        p[i] = exp2_(p[i]);
-                        ds[i] = e[b][n][i] - delta[b];
+                        const int key = k0 + n * 16 + 4 * g + i;
+                        const bool seen = key >= s.lo && key < s.hi;
+                        p[i] = seen ? p[i] : 0.f;
+                        ds[i] = seen ? ds[i] : 0.f;
+                        if constexpr (CAP) t[i] = seen ? t[i] : 0.f;
                     }
-                    if (k0 + n * 16 < alo || k0 + n * 16 + 16 > ahi) {       // a masked place is 0, not 0 * inf
-#pragma unroll
-                        for (int i = 0; i < 4; ++i) {
-                            const int key = k0 + n * 16 + 4 * g + i;
-                            const bool seen = key >= s[b].lo && key < s[b].hi;
-                            p[i] = seen ? p[i] : 0.f;
-                            ds[i] = seen ? ds[i] : 0.f;
-                            if constexpr (CAP) t[i] = seen ? t[i] : 0.f;
-                        }
-                    }
-                    ds *= p;
-                    if constexpr (AX > 0)
-                        if (A.dsl) ts[b].add(p, ds, dist);
-                    e[b][n] = CAP ? ds * S.slope_of(t) : ds;
                 }
+                ds *= p;
+                if constexpr (AX > 0)
+                    if (A.dsl) ts.add(p, ds, dist);
+                e[n] = CAP ? ds * S.slope_of(t) : ds;
             }
-            typename X::frag z[MB];
-#pragma unroll
-            for (int b = 0; b < MB; ++b) z[b] = pack_p(e[b], T());
+            const typename X::frag z = pack_p(e, T());
 #pragma unroll
             for (int d = 0; d < DB; ++d) {
                 const typename X::frag a = frag_cols<DP>(sk[buf], at, d, lane, T());
-#pragma unroll
-                for (int b = 0; b < MB; ++b) acc[b][d] = mma(a, z[b], acc[b][d]);
+                acc[d] = mma(a, z, acc[d]);
             }
         }
         if constexpr (AX > 0)
             if (A.dsl) {
-#pragma unroll
-                for (int b = 0; b < MB; ++b) ts[b].into(sl[b]);
+                ts.into(sl);
             }
     }
-#pragma unroll
-    for (int b = 0; b < MB; ++b) {
-        const int64_t r = r0 + (w * MB + b) * 16 + c, item = (int64_t)s[b].row * A.H + s[b].head;
-        if constexpr (AX > 0) sl[b].over_groups();
-        if (A.key_parts > 1) {
-            if (r < R) {
-#pragma unroll
-                for (int d = 0; d < DB; ++d) store4(A.part + (item * A.key_parts + part) * A.D, acc[b][d] * A.scale, d * 16 + g * 4, A.D, A.D % 4 == 0);
-                if (AX > 0 && g == 0) {
-                    float *st = A.stat + (item * A.key_parts + part) * 3;
-                    st[0] = (float)sl[b].ds; st[1] = (float)sl[b].dsd; st[2] = (float)sl[b].pd;
-                }
-            }
-            continue;
-        }
-        const float dslope = AX > 0 ? sl[b].row() : 0.f;
-        bool fine = finite_(dslope);
-#pragma unroll
-        for (int d = 0; d < DB; ++d)
-#pragma unroll
-            for (int i = 0; i < 4; ++i) {
-                acc[b][d][i] *= A.scale;
-                fine = fine && finite_(acc[b][d][i]);
-            }
+    const int64_t item = (int64_t)s.row * A.H + s.head;
+    if constexpr (AX > 0) sl.over_groups();
+    if (A.key_parts > 1) {
         if (r < R) {
-            T *out = reinterpret_cast<T *>(A.dq) + item * A.D;
 #pragma unroll
-            for (int d = 0; d < DB; ++d) store4(out, acc[b][d], d * 16 + g * 4, A.D, A.o_vec != 0);
-            if (AX > 0 && A.dsl && g == 0) A.dsl[kvh * R + r] = dslope;
+            for (int d = 0; d < DB; ++d) store4(A.part + (item * A.key_parts + part) * A.D, acc[d] * A.scale, d * 16 + g * 4, A.D, A.D % 4 == 0);
+            if (AX > 0 && g == 0) {
+                float *st = A.stat + (item * A.key_parts + part) * 3;
+                st[0] = (float)sl.ds; st[1] = (float)sl.dsd; st[2] = (float)sl.pd;
+            }
         }
-        uint64_t bad = __ballot(!fine && r < R);
-        while (bad) {
-            const int src = __builtin_ctzll(bad) & 15;
-            bad &= ~(0x0001000100010001ull << src);
-            const int64_t rr = r - c + src;
-            dq_slow<T>(A, kvh, row_state(A, kvh, rr, R), rr, R);
+        return;
+    }
+    const float dslope = AX > 0 ? sl.row() : 0.f;
+    bool fine = finite_(dslope);
+#pragma unroll
+    for (int d = 0; d < DB; ++d)
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            acc[d][i] *= A.scale;
+            fine = fine && finite_(acc[d][i]);
         }
+    if (r < R) {
+        T *out = reinterpret_cast<T *>(A.dq) + item * A.D;
+#pragma unroll
+        for (int d = 0; d < DB; ++d) store4(out, acc[d], d * 16 + g * 4, A.D, A.o_vec != 0);
+        if (AX > 0 && A.dsl && g == 0) A.dsl[kvh * R + r] = dslope;
+    }
+    uint64_t bad = __ballot(!fine && r < R);
+    while (bad) {
+        const int src = __builtin_ctzll(bad) & 15;
+        bad &= ~(0x0001000100010001ull << src);
+        const int64_t rr = r - c + src;
+        dq_slow<T>(A, kvh, row_state(A, kvh, rr, R), rr, R);
     }
 }
 
 // ---------------------------------------------------------------------------------------------------------------------
-// dk and dv: 64 MB keys a workgroup, 16 MB a wave (columns); tiles of BM packed rows (q, do and what belongs to a row) in LDS.
+// dk and dv: 64 keys a workgroup, 16 a wave (columns); tiles of BM packed rows (q, do and what belongs to a row) in LDS.
 // parts > 1: a workgroup takes one part of the rows that see its keys and leaves fp32 sums; scene_attn_dkv_join_kernel adds them.
 // ---------------------------------------------------------------------------------------------------------------------
-template <typename T, int DP, int BM, int MB, bool CAP, int AX>
+template <typename T, int DP, int BM, bool CAP, int AX>
 __global__ __launch_bounds__(256, DP <= 32 ? 4 : DP <= 96 ? 3 : 2) void scene_attn_dkv_kernel(const SceneAttnArgs A) {
     using X = Tr<T>;
     using L = Tile<T, DP>;
-    constexpr int NF = DP / X::KD, DB = DP / 16, PB = X::KB / 16, NC = BM * L::NCH, KEYS = 64 * MB, NV = 5 + AX;
+    constexpr int NF = DP / X::KD, DB = DP / 16, PB = X::KB / 16, NC = BM * L::NCH, KEYS = 64, NV = 5 + AX;
     static_assert(BM % X::KB == 0 && BM <= 64, "tile");
     __shared__ u32x4 sq[2][NC], sg[2][NC];
     __shared__ __attribute__((aligned(16))) float srow[2][NV][BM];      // lse, delta, lo, hi, slope, position
     const int tid = threadIdx.x, lane = tid & 63, w = tid >> 6, g = lane >> 4, c = lane & 15;
     const int kvh = (int)(blockIdx.x % A.KV), part = (int)(blockIdx.x / A.KV % A.parts);
     const int64_t R = (int64_t)A.nq * A.G;
-    const int both = A.KV * A.parts, k0 = (int)snake(blockIdx.x / both, gridDim.x / both, max(CUS / both, 1)) * KEYS, kw = k0 + w * 16 * MB;
+    const int both = A.KV * A.parts, k0 = (int)snake(blockIdx.x / both, gridDim.x / both, max(CUS / both, 1)) * KEYS, kw = k0 + w * 16;
     const Score<CAP, AX, sizeof(T) == 4> S(A);
     // the packed rows that see the workgroup's keys (this part of them)
     int64_t ra = (int64_t)max(A.key_lo[k0], 0) * A.G, rb = (int64_t)min(A.key_hi[min(k0 + KEYS - 1, A.nk - 1)], A.nq) * A.G;
@@ -427,27 +407,22 @@ __global__ __launch_bounds__(256, DP <= 32 ? 4 : DP <= 96 ? 3 : 2) void scene_at
     if (AX > 1 && A.axes < 3)
         for (int i = tid; i < 2 * BM; i += 256) srow[i / BM][NV - 1][i % BM] = 0.f;
 
-    typename X::frag kf[MB][NF], vf[MB][NF];
-    float kpos[MB][3];
+    typename X::frag kf[NF], vf[NF];
+    float kpos[3];
+    const int kk = min(kw + c, A.nk - 1);
+    const T *K = reinterpret_cast<const T *>(A.k) + (int64_t)kk * A.k_rs + kvh * A.k_hs, *V = reinterpret_cast<const T *>(A.v) + (int64_t)kk * A.v_rs + kvh * A.v_hs;
 #pragma unroll
-    for (int b = 0; b < MB; ++b) {
-        const int kk = min(kw + b * 16 + c, A.nk - 1);
-        const T *K = reinterpret_cast<const T *>(A.k) + (int64_t)kk * A.k_rs + kvh * A.k_hs, *V = reinterpret_cast<const T *>(A.v) + (int64_t)kk * A.v_rs + kvh * A.v_hs;
-#pragma unroll
-        for (int f = 0; f < NF; ++f) {
-            kf[b][f] = as_frag<T>(load_chunk<T>(K, f * X::KD + g * X::CH, A.D, A.k_vec));
-            vf[b][f] = as_frag<T>(load_chunk<T>(V, f * X::KD + g * X::CH, A.D, A.v_vec));
-        }
-#pragma unroll
-        for (int a = 0; a < 3; ++a) kpos[b][a] = a < AX && a < A.axes ? A.kpos[(int64_t)kk * A.axes + a] : 0.f;
+    for (int f = 0; f < NF; ++f) {
+        kf[f] = as_frag<T>(load_chunk<T>(K, f * X::KD + g * X::CH, A.D, A.k_vec));
+        vf[f] = as_frag<T>(load_chunk<T>(V, f * X::KD + g * X::CH, A.D, A.v_vec));
     }
+#pragma unroll
+    for (int a = 0; a < 3; ++a) kpos[a] = a < AX && a < A.axes ? A.kpos[(int64_t)kk * A.axes + a] : 0.f;
     // the rows that see a key of this wave
-    const int64_t wa = (int64_t)max(A.key_lo[min(kw, A.nk - 1)], 0) * A.G, wb = (int64_t)min(A.key_hi[min(kw + 16 * MB - 1, A.nk - 1)], A.nq) * A.G;
-    f32x4 dk[MB][DB], dv[MB][DB];
+    const int64_t wa = (int64_t)max(A.key_lo[min(kw, A.nk - 1)], 0) * A.G, wb = (int64_t)min(A.key_hi[min(kw + 15, A.nk - 1)], A.nq) * A.G;
+    f32x4 dk[DB], dv[DB];
 #pragma unroll
-    for (int b = 0; b < MB; ++b)
-#pragma unroll
-        for (int d = 0; d < DB; ++d) dk[b][d] = dv[b][d] = f32x4{0.f, 0.f, 0.f, 0.f};
+    for (int d = 0; d < DB; ++d) dk[d] = dv[d] = f32x4{0.f, 0.f, 0.f, 0.f};
 
     int buf = 0;
     for (int64_t rbase = ra; rbase < rb; rbase += BM, buf ^= 1) {
@@ -461,25 +436,20 @@ __global__ __launch_bounds__(256, DP <= 32 ? 4 : DP <= 96 ? 3 : 2) void scene_at
             if (r0 >= wb || r0 + X::KB <= wa || r0 >= rb) continue;
             // bounds never decrease: the last row has the latest lo, the first the earliest hi
             const int lo_last = uniform(__float_as_int(srow[buf][2][at + X::KB - 1])), hi_first = uniform(__float_as_int(srow[buf][3][at]));
-            const bool masked = kw < lo_last || kw + 16 * MB > hi_first || r0 + X::KB > rb;
-            f32x4 p[MB][PB], z[MB][PB];
+            const bool masked = kw < lo_last || kw + 16 > hi_first || r0 + X::KB > rb;
+            f32x4 p[PB], z[PB];
 #pragma unroll
             for (int n = 0; n < PB; ++n) {
-#pragma unroll
-                for (int b = 0; b < MB; ++b) p[b][n] = z[b][n] = f32x4{0.f, 0.f, 0.f, 0.f};
+                p[n] = z[n] = f32x4{0.f, 0.f, 0.f, 0.f};
 #pragma unroll
                 for (int f = 0; f < NF; ++f) {
                     const typename X::frag qa = frag_rows<T, DP>(sq[buf], at + n * 16, f, lane);
                     const typename X::frag ga = frag_rows<T, DP>(sg[buf], at + n * 16, f, lane);
-#pragma unroll
-                    for (int b = 0; b < MB; ++b) {
-                        p[b][n] = mma(qa, kf[b][f], p[b][n]);
-                        z[b][n] = mma(ga, vf[b][f], z[b][n]);
-                    }
+                    p[n] = mma(qa, kf[f], p[n]);
+                    z[n] = mma(ga, vf[f], z[n]);
                 }
             }
-#pragma unroll
-            for (int b = 0; b < MB; ++b) S.template apply<PB>(p[b]);
+            S.template apply<PB>(p);
 #pragma unroll
             for (int n = 0; n < PB; ++n) {
                 auto col = [&](int v) { return *reinterpret_cast<const f32x4 *>(&srow[buf][v][at + n * 16 + 4 * g]); };
@@ -493,83 +463,69 @@ __global__ __launch_bounds__(256, DP <= 32 ? 4 : DP <= 96 ? 3 : 2) void scene_at
                     py = col(6);
                     pz = col(NV - 1);
                 }
+                f32x4 t = p[n];
+                p[n] = t - lse;
+                if constexpr (AX > 0) p[n] -= slope * S.dist4(kpos, px, py, pz);
+                z[n] -= delta;
 #pragma unroll
-                for (int b = 0; b < MB; ++b) {
-                    f32x4 t = p[b][n];
-                    p[b][n] = t - lse;
-                    if constexpr (AX > 0) p[b][n] -= slope * S.dist4(kpos[b], px, py, pz);
-                    z[b][n] -= delta;
+                for (int i = 0; i < 4; ++i) p[n][i] = exp2_(p[n][i]);
+                if (masked) {                           // a masked place is 0, not 0 * inf
+                    const f32x4 lo = col(2), hi = col(3);
+                    const int key = kw + c;
 #pragma unroll
-                    for (int i = 0; i < 4; ++i) p[b][n][i] = exp2_(p[b][n][i]);
-                    if (masked) {                           // a masked place is 0, not 0 * inf
-                        const f32x4 lo = col(2), hi = col(3);
-                        const int key = kw + b * 16 + c;
-#pragma unroll
-                        for (int i = 0; i < 4; ++i) {
-                            const bool seen = key >= __float_as_int(lo[i]) && key < __float_as_int(hi[i]) && r0 + n * 16 + 4 * g + i < rb;
-                            p[b][n][i] = seen ? p[b][n][i] : 0.f;
-                            z[b][n][i] = seen ? z[b][n][i] : 0.f;
-                            if constexpr (CAP) t[i] = seen ? t[i] : 0.f;
-                        }
+                    for (int i = 0; i < 4; ++i) {
+                        const bool seen = key >= __float_as_int(lo[i]) && key < __float_as_int(hi[i]) && r0 + n * 16 + 4 * g + i < rb;
+                        p[n][i] = seen ? p[n][i] : 0.f;
+                        z[n][i] = seen ? z[n][i] : 0.f;
+                        if constexpr (CAP) t[i] = seen ? t[i] : 0.f;
                     }
-                    z[b][n] *= p[b][n];
-                    if constexpr (CAP) z[b][n] *= S.slope_of(t);
                 }
+                z[n] *= p[n];
+                if constexpr (CAP) z[n] *= S.slope_of(t);
             }
-            typename X::frag pf[MB], zf[MB];
-#pragma unroll
-            for (int b = 0; b < MB; ++b) {
-                pf[b] = pack_p(p[b], T());
-                zf[b] = pack_p(z[b], T());
-            }
+            const typename X::frag pf = pack_p(p, T()), zf = pack_p(z, T());
 #pragma unroll
             for (int d = 0; d < DB; ++d) {
                 const typename X::frag ga = frag_cols<DP>(sg[buf], at, d, lane, T());
                 const typename X::frag qa = frag_cols<DP>(sq[buf], at, d, lane, T());
-#pragma unroll
-                for (int b = 0; b < MB; ++b) {
-                    dv[b][d] = mma(ga, pf[b], dv[b][d]);
-                    dk[b][d] = mma(qa, zf[b], dk[b][d]);
-                }
+                dv[d] = mma(ga, pf, dv[d]);
+                dk[d] = mma(qa, zf, dk[d]);
             }
         }
     }
+    const int key = kw + c;
+    const int64_t at = ((int64_t)key * A.KV + kvh) * A.D;
+    bool fine = true;
 #pragma unroll
-    for (int b = 0; b < MB; ++b) {
-        const int key = kw + b * 16 + c;
-        const int64_t at = ((int64_t)key * A.KV + kvh) * A.D;
-        bool fine = true;
+    for (int d = 0; d < DB; ++d)
 #pragma unroll
-        for (int d = 0; d < DB; ++d)
-#pragma unroll
-            for (int i = 0; i < 4; ++i) {
-                dk[b][d][i] *= A.scale;
-                fine = fine && finite_(dk[b][d][i]) && finite_(dv[b][d][i]);
-            }
-        if (A.parts > 1) {
-            const int64_t n = (int64_t)A.nk * A.KV * A.D;
-            if (key < A.nk) {
-#pragma unroll
-                for (int d = 0; d < DB; ++d) {
-                    store4(A.part2 + 2 * part * n + at, dk[b][d], d * 16 + g * 4, A.D, A.D % 4 == 0);
-                    store4(A.part2 + (2 * part + 1) * n + at, dv[b][d], d * 16 + g * 4, A.D, A.D % 4 == 0);
-                }
-            }
-            continue;
+        for (int i = 0; i < 4; ++i) {
+            dk[d][i] *= A.scale;
+            fine = fine && finite_(dk[d][i]) && finite_(dv[d][i]);
         }
+    if (A.parts > 1) {
+        const int64_t n = (int64_t)A.nk * A.KV * A.D;
         if (key < A.nk) {
 #pragma unroll
             for (int d = 0; d < DB; ++d) {
-                store4(reinterpret_cast<T *>(A.dk) + at, dk[b][d], d * 16 + g * 4, A.D, A.o_vec != 0);
-                store4(reinterpret_cast<T *>(A.dv) + at, dv[b][d], d * 16 + g * 4, A.D, A.o_vec != 0);
+                store4(A.part2 + 2 * part * n + at, dk[d], d * 16 + g * 4, A.D, A.D % 4 == 0);
+                store4(A.part2 + (2 * part + 1) * n + at, dv[d], d * 16 + g * 4, A.D, A.D % 4 == 0);
             }
         }
-        uint64_t bad = __ballot(!fine && key < A.nk);
-        while (bad) {
-            const int src = __builtin_ctzll(bad) & 15;
-            bad &= ~(0x0001000100010001ull << src);
-            dkv_slow<T>(A, kvh, key - c + src, R);
+        return;
+    }
+    if (key < A.nk) {
+#pragma unroll
+        for (int d = 0; d < DB; ++d) {
+            store4(reinterpret_cast<T *>(A.dk) + at, dk[d], d * 16 + g * 4, A.D, A.o_vec != 0);
+            store4(reinterpret_cast<T *>(A.dv) + at, dv[d], d * 16 + g * 4, A.D, A.o_vec != 0);
         }
+    }
+    uint64_t bad = __ballot(!fine && key < A.nk);
+    while (bad) {
+        const int src = __builtin_ctzll(bad) & 15;
+        bad &= ~(0x0001000100010001ull << src);
+        dkv_slow<T>(A, kvh, key - c + src, R);
     }
 }
 
@@ -626,10 +582,10 @@ template <typename T> __global__ __launch_bounds__(256) void scene_attn_dkv_join
 
 template <typename T, int DP, int BN, bool CAP, int AX> hipError_t launch_bwd(const SceneAttnArgs &A, hipStream_t st) {
     const int64_t tiles = ((int64_t)A.nq * A.G + 63) / 64;
-    if (tiles > 0 && A.dq) hipLaunchKernelGGL((scene_attn_dq_kernel<T, DP, BN, 1, CAP, AX>), dim3((unsigned)(tiles * A.KV * A.key_parts)), dim3(256), 0, st, A);
+    if (tiles > 0 && A.dq) hipLaunchKernelGGL((scene_attn_dq_kernel<T, DP, BN, CAP, AX>), dim3((unsigned)(tiles * A.KV * A.key_parts)), dim3(256), 0, st, A);
     if (tiles > 0 && A.dq && A.key_parts > 1) hipLaunchKernelGGL((scene_attn_dq_join_kernel<T>), dim3((unsigned)(((int64_t)A.nq * A.H + 7) / 8)), dim3(256), 0, st, A);
     if (A.nk > 0 && A.dk) {
-        hipLaunchKernelGGL((scene_attn_dkv_kernel<T, DP, BN, 1, CAP, AX>), dim3((unsigned)(((int64_t)A.nk + 63) / 64 * A.KV * A.parts)), dim3(256), 0, st, A);
+        hipLaunchKernelGGL((scene_attn_dkv_kernel<T, DP, BN, CAP, AX>), dim3((unsigned)(((int64_t)A.nk + 63) / 64 * A.KV * A.parts)), dim3(256), 0, st, A);
         if (A.parts > 1) hipLaunchKernelGGL((scene_attn_dkv_join_kernel<T>), dim3((unsigned)(((int64_t)A.nk * A.KV + 7) / 8)), dim3(256), 0, st, A);
     }
     return hipGetLastError();

@@ -27,6 +27,7 @@ template <typename T> __device__ void row_slow(const SceneAttnArgs &A, int kvh, 
         o0 = o0 * corr + (h0 ? p * to_f(v[j * A.v_rs + lane]) : 0.f);
         o1 = o1 * corr + (h1 ? p * to_f(v[j * A.v_rs + lane + 64]) : 0.f);
         m = mn;
+        if (l != l) break;                                   // the whole row is NaN already
     }
     const float inv = l == 0.f ? 0.f : 1.f / l;
     const int64_t at = ((int64_t)s.row * A.H + s.head) * A.D;

@@ -3,7 +3,7 @@
 // addresses that bind() got from the loaded libdagnet_hip.so.
 //
 // Why not ctypes and a Python autograd.Function, like the other operators: a training call of a small batch spent 128 us on the host (a third of
-// it Python in autograd's own thread, on a cold core) for 35 us on the GPU; these nodes take 50.
+// it Python in autograd's own thread, on a cold core) for 35 us on the GPU; these nodes take 55.
 #include <torch/csrc/autograd/custom_function.h>
 #include <torch/csrc/autograd/functions/basic_ops.h>
 #include <torch/extension.h>
@@ -86,9 +86,11 @@ std::tuple<Tensor, Tensor, Tensor> attend(dagnet_attn &a, const Tensor &q, const
     return {out, lse, o};
 }
 
-// gradients that have none of their own: a second derivative through them raises
+// gradients that have none of their own: a second derivative through them raises (the error's node is attached to tensors that require a gradient only)
 variable_list once(variable_list grads, const char *what) {
     if (!at::GradMode::is_enabled()) return grads;
+    for (Tensor &g : grads)
+        if (g.defined()) g.set_requires_grad(true);
     return torch::autograd::DelayedError(std::string(what) + " has no second derivative", (int64_t)grads.size())(std::move(grads));
 }
 
@@ -211,6 +213,9 @@ py::tuple rotary(const Tensor &q, const std::optional<Tensor> &k_, const Tensor 
         if (!inplace && at::GradMode::is_enabled() && (q.requires_grad() || (k.defined() && k.requires_grad()))) out = Rotary::apply(q, k_, pos, x, held);
         else {
             out = {inplace ? q : dense(q), !k.defined() || inplace ? k : dense(k)};
+            if (inplace)                                    // what autograd saved of them is no longer what it was
+                for (const Tensor &t : out)
+                    if (t.defined()) t.unsafeGetTensorImpl()->bump_version();
             turn(q, k, pos, x, false, out[0], out[1]);
         }
     }

@@ -85,7 +85,10 @@ def attention(q, k, v, seen, scale, cap=0.0, slopes=None, pos=None, k_pos=None, 
             mean = (p * dist).sum(1, keepdim=True)
             tol["dslopes"][h] = (e * (dist + mean)).sum() + (edelta * (rel + n * U) * 2 * mean).sum() + U * abs(res["dslopes"][h])
         if cap:
-            ds, eds = ds * (1 - t * t), eds * (1 - t * t) + ds.abs() * (2 * t.abs() * (ex / cap + 12 * U) + 4 * U)
+            # (ds + e) (f + d) - ds f = e f + ds d + e d, f = 1 - t^2, d its error.  The last term is what is left in a row with one key, where ds
+            # is 0 but for e, under a saturated cap, where f is 0 but for d.
+            f, ef = 1 - t * t, 2 * t.abs() * (ex / cap + 12 * U) + 4 * U
+            ds, eds = ds * f, eds * f + ds.abs() * ef + eds * ef
         eds = eds + r * ds.abs()
         res["dq"][:, h] = ds @ kh * scale
         tol["dq"][:, h] = (eds @ kh.abs() + n * U * (ds.abs() @ kh.abs())) * abs(scale)

@@ -509,3 +509,136 @@ def test_mixed_devices_are_refused():
         scene_attention(t["q"], t["k"].cpu(), t["v"], SceneLayout([0, 20]))
     with pytest.raises(DagnetHipError, match="ROCm device"):
         scene_attention(t["q"], t["k"], t["v"], SceneLayout([0, 20]), slopes=t["slopes"], pos=t["pos"].cpu())
+
+
+@pytest.mark.parametrize("dt", [F32, BF16], ids=["fp32", "bf16"])
+@pytest.mark.parametrize("names", [("q",), ("slopes",), ("q", "slopes"), ("k", "v")])
+def test_rows_repaired_one_by_one_whichever_gradients_are_wanted(names, dt):
+    """A NaN in a key of another scene sends the rows of its tile through the form that takes them one by one; what that form reads has to be there
+    (memory that the calls get is filled with large values first)."""
+    ptr = [0, 20, 51]
+    t = inputs(5, 51, 51, 4, 2, 24, dt, 2)
+    t["k"][22], t["v"][22] = float("nan"), float("nan")
+    del t["k_pos"]
+    layout = SceneLayout(ptr)
+    leaves = [t[n].requires_grad_() for n in names]
+    out = scene_attention(t["q"], t["k"], t["v"], layout, softcap=8.0, slopes=t["slopes"], pos=t["pos"])
+    keep = [torch.full((n,), 1e4, device=DEV) for n in (64, 512, 4096, 1 << 16, 1 << 20) for _ in range(8)]
+    del keep
+    dout = t["dout"].clone()
+    dout[20:] = 0
+    got = dict(zip(names, torch.autograd.grad(out, leaves, dout)))
+    cut = {n: t[n].detach()[:20] for n in ("q", "k", "v", "pos")}
+    want, tol = ref.attention(cut["q"], cut["k"], cut["v"], ref.seen_matrix([0, 20], None, 0), 24 ** -0.5, 8.0, t["slopes"].detach(), cut["pos"], cut["pos"], t["dout"][:20])
+    ref.close(out[:20], want["out"], tol["out"], "out")
+    for n, g in got.items():
+        if n == "slopes":
+            assert g.isnan().all()                    # the other scene's own NaN
+        else:
+            ref.close(g[:20], want["d" + n], tol["d" + n], "d" + n)
+
+
+@pytest.mark.parametrize("dt", [F32, BF16], ids=["fp32", "bf16"])
+def test_a_cap_far_below_the_scores(dt):
+    t = inputs(9, 70, 70, 2, 1, 16, dt, 0)
+    both(t, SceneLayout([0, 70], causal=1), ref.seen_matrix([0, 70], None, 1), cap=1e-3)
+
+
+@pytest.mark.parametrize("dt", [F32, BF16], ids=["fp32", "bf16"])
+def test_a_cap_far_above_the_scores_is_none(dt):
+    """cap 1e12 moves a score x by x^3 / 3e24.  tanh near zero is a product, a quotient and the two factors: at most six roundings, 6 U |x|, which
+    is what the bounds without a cap hold for x already (2 U and 4 U of its size): twice those bounds."""
+    t = inputs(9, 70, 70, 2, 1, 16, dt, 0)
+    leaves = [t[n].requires_grad_() for n in ("q", "k", "v")]
+    out = scene_attention(*leaves, SceneLayout([0, 70], causal=1), softcap=1e12)
+    want, tol = ref.attention(*leaves, ref.seen_matrix([0, 70], None, 1), 0.25, 0.0, None, None, None, t["dout"])
+    for name, got in zip(("out", "dq", "dk", "dv"), (out,) + torch.autograd.grad(out, leaves, t["dout"])):
+        ref.close(got, want[name], 2 * tol[name], name)
+
+
+@pytest.mark.parametrize("dt", [F32, BF16], ids=["fp32", "bf16"])
+def test_a_cap_next_to_zero_gives_the_mean(dt):
+    """Scores within 1e-12 of each other: p is 1 / n to eps, for rows of zeros too (0 / cap).  n = 40 terms: sums off by at most 40 eps of the values'
+    size, the quotient, p's rounding (bf16: half a step, 2^-8) and the output's on top."""
+    t = inputs(9, 40, 40, 2, 1, 16, dt, 0)
+    t["q"][::2] = 0
+    leaves = [t[n].requires_grad_() for n in ("q", "k", "v")]
+    out = scene_attention(*leaves, SceneLayout([0, 40]), softcap=1e-12)
+    want = t["v"].detach().double().mean(0, keepdim=True).expand(40, 2, 16)
+    size = t["v"].detach().double().abs().max().item()
+    tol = size * 48 * 2 ** -23 + (size * 2 * 2 ** -8 if dt == BF16 else 0)
+    assert ((out.double() - want).abs() <= tol).all()
+    assert all(torch.isfinite(g).all() for g in torch.autograd.grad(out, leaves, t["dout"]))
+
+
+@pytest.mark.parametrize("dt", [F32, BF16], ids=["fp32", "bf16"])
+def test_positions_whose_squares_overflow(dt):
+    """The far half is infinitely far in fp32 (2e20 ** 2 > 3.4e38): its keys have p = 0, as in 64 bits (exp(-0.1 2e20))."""
+    t = inputs(3, 60, 60, 2, 2, 16, dt, 2)
+    t["slopes"] = torch.full((2,), 0.1, device=DEV)
+    near = t["pos"].clone()
+    t["pos"][30:] += 2e20
+    out = scene_attention(t["q"], t["k"], t["v"], SceneLayout([0, 60]), slopes=t["slopes"], pos=t["pos"])
+    cut = {n: t[n][:30] for n in ("q", "k", "v")}
+    want, tol = ref.attention(cut["q"], cut["k"], cut["v"], ref.seen_matrix([0, 30], None, 0), 0.25, 0.0, t["slopes"], near[:30], near[:30], t["dout"][:30])
+    ref.close(out[:30], want["out"], tol["out"], "out")
+
+
+@pytest.mark.parametrize("N", [700, 2500])
+def test_a_batch_of_nan_gives_nan(N):
+    """Every row is taken one by one then, and ends at its first key."""
+    t = inputs(2, N, N, 4, 2, 32, BF16, 0)
+    t["q"].fill_(float("nan"))
+    leaves = [t[n].requires_grad_() for n in ("q", "k", "v")]
+    out = scene_attention(*leaves, SceneLayout([0, N], causal=1))
+    assert out.isnan().all() and all(g.isnan().all() for g in torch.autograd.grad(out, leaves, t["dout"]))
+
+
+def test_in_place_rotary_is_seen_by_autograd():
+    g = torch.Generator().manual_seed(1)
+    q, k = randn(g, (9, 2, 16), F32), randn(g, (9, 2, 16), F32)
+    axes, pos = RotaryAxes(16, (8,)), torch.arange(9, device=DEV)[:, None]
+    w = torch.ones(16, device=DEV, requires_grad=True)
+    before = (q * w).sum() + (k * w).sum()
+    with torch.no_grad():
+        rotary(q, k, pos, axes, inplace=True)
+    with pytest.raises(RuntimeError, match="modified by an inplace operation"):
+        before.backward()
+
+
+def test_in_place_rotary_of_one_product_and_positions_within():
+    """q and k as parts of one tensor, the positions another part of it; what is not turned stays."""
+    g = torch.Generator().manual_seed(2)
+    x = randn(g, (33, 5, 16), F32)
+    pos = x[:, 4, :2]
+    axes = RotaryAxes(16, (4, 4))
+    was = x.clone()
+    want = rotary(was[:, :2], was[:, 2:3], was[:, 4, :2], axes)
+    rotary(x[:, :2], x[:, 2:3], pos, axes, inplace=True)
+    assert torch.equal(x[:, :2], want[0]) and torch.equal(x[:, 2:3], want[1]) and torch.equal(x[:, 3:], was[:, 3:])
+    rotary(x[:, :2], x[:, 4:], pos, axes, inplace=True)              # k holds the positions
+    twice = rotary(want[0], was[:, 4:], was[:, 4, :2], axes)
+    assert torch.equal(x[:, :2], twice[0]) and torch.equal(x[:, 4:], twice[1])
+
+
+@pytest.mark.parametrize("which", [0, 1])
+def test_one_of_the_two_turned_tensors_used(which):
+    g = torch.Generator().manual_seed(3)
+    q, k = randn(g, (17, 3, 16), F32).requires_grad_(), randn(g, (17, 1, 16), F32).requires_grad_()
+    axes, pos = RotaryAxes(16, (5, 3)), torch.rand((17, 2), generator=g).to(DEV)
+    out = rotary(q, k, pos, axes)[which]
+    got = torch.autograd.grad(out.sum(), (q, k), allow_unused=True)
+    alone = (q, k)[which].detach().requires_grad_()
+    want = torch.autograd.grad(rotary(alone, None, pos, axes)[0].sum(), alone)[0]
+    assert torch.equal(got[which], want) and (got[1 - which] is None or (got[1 - which] == 0).all())
+
+
+def test_second_derivatives_are_refused_whatever_asks_for_them():
+    t = inputs(4, 20, 20, 2, 2, 16, F32, 1)
+    for names in (("q",), ("slopes",), ("q", "k", "v", "slopes")):
+        leaves = [t[n].detach().requires_grad_() for n in names]
+        a = {**t, **dict(zip(names, leaves))}
+        out = scene_attention(a["q"], a["k"], a["v"], SceneLayout([0, 20]), slopes=a["slopes"], pos=a["pos"])
+        grads = torch.autograd.grad(out.square().sum(), leaves, create_graph=True)
+        with pytest.raises(RuntimeError, match="no second derivative"):
+            sum(x.sum() for x in grads).backward()

@@ -1,11 +1,14 @@
 """CPU: the layouts' row and key bounds against a row-by-row reading of their definition, and what the entry points refuse."""
+import copy
 import ctypes as C
+import pickle
+import random
 
 import numpy as np
 import pytest
 import torch
 
-from dagnet_amd import _capi, _ops
+from dagnet_amd import _capi, _ops, attention
 from dagnet_amd._capi import DagnetHipError
 from dagnet_amd.attention import RotaryAxes, SceneLayout, rotary, scene_attention, scene_attention_step
 from tests import scene_attn_ref as ref
@@ -165,3 +168,72 @@ def test_c_entries_refuse_before_any_launch():
     assert lib.dagnet_op_rotary(0, *r[1:]) == 0
     with pytest.raises(DagnetHipError, match="null argument"):
         _capi._check(lib.dagnet_op_attn_fwd(C.byref(a), *[None] * 7))
+
+
+@pytest.mark.parametrize("make", [lambda: SceneLayout([0, 3, 8], causal=1), lambda: RotaryAxes(16, (4, 4))])
+def test_copies_do_not_take_another_objects_addresses(make):
+    a = make()
+    a._dev[0] = ((1, 2, 3), 0)                       # as if uploaded
+    for b in (copy.deepcopy(a), copy.copy(a), pickle.loads(pickle.dumps(a))):
+        assert b._dev == {} and np.array_equal(b._host().numpy(), a._host().numpy())
+    assert a._dev
+
+
+@pytest.mark.parametrize("kw", [dict(softcap=1e-20), dict(softcap=1e20), dict(scale=1e20), dict(softcap=1e-46)])
+def test_scales_that_leave_fp32_are_refused(kw):
+    with pytest.raises(DagnetHipError, match="1e-15 .. 1e15"):
+        scene_attention(**_args(**kw))
+
+
+def _views(kind):
+    n, H, KV, D = 6, 4, 2, 16
+    if kind == "rows":                               # columns of one product
+        x = torch.zeros(n, H + 2 * KV, D)
+        return x[:, :H], x[:, H:H + KV]
+    if kind == "heads":                              # q, k and v side by side in every head
+        x = torch.zeros(n, H, 3, D)
+        return x[:, :, 0], x[:, :, 1]
+    if kind == "behind":                             # heads first
+        x = torch.zeros(H + KV, n, D).transpose(0, 1)
+        return x[:, :H], x[:, H:]
+    x = torch.zeros(n, H, D)
+    return {"same": (x, x), "part": (x, x[:, 1:3]), "shifted": (x.view(-1)[:n * 2 * D].view(n, 2, D), x.view(-1)[D:D + n * 2 * D].view(n, 2, D)),
+            "windows": (x.view(-1).as_strided((n, 4, D), (16, 16, 1)), None)}[kind]
+
+
+@pytest.mark.parametrize("kind,match", [("rows", "no CPU path"), ("heads", "no CPU path"), ("behind", "no CPU path"), ("same", "overlap"), ("part", "overlap"),
+                                        ("shifted", "overlap"), ("windows", "of its own")])
+def test_in_place_rotary_refuses_elements_that_are_turned_twice(kind, match):
+    q, k = _views(kind)
+    with pytest.raises(DagnetHipError, match=match):
+        rotary(**_rot(q=q, k=k), inplace=True)
+
+
+def test_what_the_strides_show_is_what_is():
+    """Against the sets of elements: views that are called apart share none."""
+    r = random.Random(3)
+    x = torch.zeros(400)
+    apart = 0
+    for _ in range(2000):
+        v = []
+        for _ in range(2):
+            shape = (r.randint(1, 4), r.randint(1, 3), r.choice((2, 4)))
+            v.append(torch.as_strided(x, shape, (r.choice((4, 8, 16, 24)), r.choice((4, 8, 48)), 1), r.randint(0, 40)))
+        sets = [(t.storage_offset() + (torch.arange(t.shape[0])[:, None, None] * t.stride(0) + torch.arange(t.shape[1])[:, None] * t.stride(1)
+                                       + torch.arange(t.shape[2]))).flatten().tolist() for t in v]
+        if attention._apart(*v):
+            apart += 1
+            assert not set(sets[0]) & set(sets[1])
+        for t, s in zip(v, sets):
+            assert not attention._own_elements(t) or len(set(s)) == len(s)
+    assert apart > 500
+
+
+def test_launches_that_cannot_be_counted_are_refused():
+    lib = _ops._lib()
+    a = _Attn(nq=2 ** 30, nk=4, n_heads=8, n_kv_heads=8, head_dim=16, axes=0, dtype=0, scale=1.0, softcap=0.0, q=64, k=64, v=64)
+    assert lib.dagnet_op_attn_fwd(C.byref(a), *[64] * 3, None, None, None, None) == -1 and b"too many rows" in lib.dagnet_last_error()
+    a.nq, a.nk = 4, 2 ** 30
+    assert lib.dagnet_op_attn_fwd(C.byref(a), *[64] * 3, None, None, None, None) == -1 and b"too many rows" in lib.dagnet_last_error()
+    assert lib.dagnet_op_rotary(16 * 0xffffff + 1, 1, 0, 16, 0, 64, 16, 16, None, 0, 0, 64, 0, 1, 64, 64, 4, 0, 0, 64, 16, 16, None, 0, 0, None) == -1
+    assert b"too many rows" in lib.dagnet_last_error()
