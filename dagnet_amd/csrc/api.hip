@@ -2167,6 +2167,7 @@ extern "C" hipError_t dn_scene_attn_fwd_bf16(const SceneAttnArgs *, hipStream_t)
 extern "C" hipError_t dn_scene_attn_bwd_f32(const SceneAttnArgs *, float *, hipStream_t);
 extern "C" hipError_t dn_scene_attn_bwd_bf16(const SceneAttnArgs *, float *, hipStream_t);
 extern "C" int dn_scene_attn_bwd_parts(int64_t, int64_t, int, int);
+extern "C" int dn_scene_attn_uneven(int64_t, int64_t);
 extern "C" int dn_scene_attn_key_parts(int64_t, int, int, int64_t, int64_t);
 extern "C" hipError_t dn_scene_attn_step_f32(const SceneStepArgs *, hipStream_t);
 extern "C" hipError_t dn_scene_attn_step_bf16(const SceneStepArgs *, hipStream_t);
@@ -2202,6 +2203,7 @@ static int attn_args(const dagnet_attn *a, SceneAttnArgs *A) {
     A->q_rs = a->q_row; A->q_hs = a->q_head; A->k_rs = a->k_row; A->k_hs = a->k_head; A->v_rs = a->v_row; A->v_hs = a->v_head;
     A->nq = a->nq; A->nk = a->nk; A->H = a->n_heads; A->KV = a->n_kv_heads; A->G = a->n_heads / a->n_kv_heads; A->D = a->head_dim;
     A->axes = a->axes; A->scale = a->scale; A->cap = a->softcap;
+    A->uneven = dn_scene_attn_uneven(a->max_keys, a->mean_keys);
     const int size = a->dtype ? 2 : 4;
     A->q_vec = attn_vec(a->q, a->q_row, a->q_head, a->head_dim, size);
     A->k_vec = attn_vec(a->k, a->k_row, a->k_head, a->head_dim, size);

@@ -41,8 +41,7 @@ template <typename T> __device__ void row_slow(const SceneAttnArgs &A, int kvh, 
     if (A.lse && lane == 0) A.lse[kvh * R + r] = l == 0.f ? 0.f : m + log2_(l);
 }
 
-// MB: 16-row blocks per wave.  One (64 rows a workgroup) where the rows would not fill the chip otherwise, two (128 rows) where they do: every K and
-// V fragment read from LDS then serves two products.  EXACT (bf16, for a backward pass): what rounding p left over goes through the second
+// MB: 16-row blocks per wave, one or two (rows_fwd() chooses): with two, every K and V fragment read from LDS serves two products.  EXACT (bf16, for a backward pass): what rounding p left over goes through the second
 // product too, so that o, and delta with it, does not carry that rounding.
 template <typename T, int DP, int BN, int MB, bool CAP, int AX, bool EXACT>
 __global__ __launch_bounds__(256, MB == 2 ? 2 : 3) void scene_attn_fwd_kernel(const SceneAttnArgs A) {
@@ -303,38 +302,50 @@ template <typename T, int DP, int BN, int MB, bool CAP, int AX> hipError_t launc
     if (A.key_parts > 1) hipLaunchKernelGGL((scene_attn_fwd_join_kernel<T>), dim3((unsigned)(((int64_t)A.nq * A.H + 7) / 8)), dim3(256), 0, st, A);
     return hipGetLastError();
 }
-template <typename T, int DP, int BN, int MB> hipError_t pick_fwd(const SceneAttnArgs &A, hipStream_t st) {
-    if (A.cap > 0.f) return A.axes == 0 ? launch_fwd<T, DP, BN, MB, true, 0>(A, st) : A.axes == 1 ? launch_fwd<T, DP, BN, MB, true, 1>(A, st) : launch_fwd<T, DP, BN, MB, true, 3>(A, st);
-    return A.axes == 0 ? launch_fwd<T, DP, BN, MB, false, 0>(A, st) : A.axes == 1 ? launch_fwd<T, DP, BN, MB, false, 1>(A, st) : launch_fwd<T, DP, BN, MB, false, 3>(A, st);
+// Two blocks of 16 rows a wave read K and V from LDS half as often but leave a CU with two workgroups of 128 rows instead of three or four of 64.  Worth
+// it where the products weigh more than the scores' vector work (cap, distance), the more so the wider a head, and where the workgroups fill
+// the chip's 512 places; rows that see unlike numbers of keys need more of them, short tiles filling up behind long ones.  bf16, 8 heads to 2,
+// us with one block and with two:
+//     rows 8192, all seen, no cap: width 64 212 203, 96 364 248, 128 416 304;  causal: 126 164, 178 205, 227 258;  16384 causal: 401 361, 571 502, 812 631
+//     16384, all seen: width 32 549 538 (training 694 698);  64, one axis 896 814, cap 1184 1202;  96, cap 1486 1460, cap and an axis 1582 1617;
+//     128, cap and an axis 2136 1749, cap and three axes 2520 2618;  width 96, 544 to 704 workgroups (a second round hardly filled): 385 449, 536 572
+template <typename T, int DP, int BN, bool CAP, int AX> hipError_t rows_fwd(const SceneAttnArgs &A, hipStream_t st) {
+    if constexpr (sizeof(T) == 2 && DP >= 64 && (CAP ? 2 : 0) + (AX > 1 ? 2 : AX) < DP / 32) {
+        const int64_t groups = ((int64_t)A.nq * A.G + 127) / 128 * A.KV;
+        if (A.uneven ? groups >= 768 : groups >= 448 && !(DP == 96 && groups > 512 && groups < 768)) return launch_fwd<T, DP, BN, 2, CAP, AX>(A, st);
+    }
+    return launch_fwd<T, DP, BN, 1, CAP, AX>(A, st);
+}
+template <typename T, int DP, int BN> hipError_t pick_fwd(const SceneAttnArgs &A, hipStream_t st) {
+    if (A.cap > 0.f) return A.axes == 0 ? rows_fwd<T, DP, BN, true, 0>(A, st) : A.axes == 1 ? rows_fwd<T, DP, BN, true, 1>(A, st) : rows_fwd<T, DP, BN, true, 3>(A, st);
+    return A.axes == 0 ? rows_fwd<T, DP, BN, false, 0>(A, st) : A.axes == 1 ? rows_fwd<T, DP, BN, false, 1>(A, st) : rows_fwd<T, DP, BN, false, 3>(A, st);
 }
 
 }  // namespace sattn
 
 // one object file per type (the Makefile compiles this source twice)
 #ifdef SCENE_ATTN_BF16
-template <int DP, int BN> static hipError_t fwd_rows(const SceneAttnArgs &A, hipStream_t st) {
-    using namespace sattn;
-    const int64_t tiles = ((int64_t)A.nq * A.G + 127) / 128;
-    return tiles * A.KV >= 1536 ? pick_fwd<bf16, DP, BN, 2>(A, st) : pick_fwd<bf16, DP, BN, 1>(A, st);
-}
 extern "C" hipError_t dn_scene_attn_fwd_bf16(const SceneAttnArgs *A, hipStream_t st) {
+    using namespace sattn;
     const int D = A->D;
-    return D <= 32 ? fwd_rows<32, 64>(*A, st) : D <= 64 ? fwd_rows<64, 64>(*A, st) : D <= 96 ? fwd_rows<96, 64>(*A, st) : fwd_rows<128, 64>(*A, st);
+    return D <= 32 ? pick_fwd<bf16, 32, 64>(*A, st) : D <= 64 ? pick_fwd<bf16, 64, 64>(*A, st) : D <= 96 ? pick_fwd<bf16, 96, 64>(*A, st) : pick_fwd<bf16, 128, 64>(*A, st);
 }
 #else
 extern "C" hipError_t dn_scene_attn_fwd_f32(const SceneAttnArgs *A, hipStream_t st) {
     using namespace sattn;
     const int D = A->D;
-    return D <= 16 ? pick_fwd<float, 16, 64, 1>(*A, st) : D <= 32 ? pick_fwd<float, 32, 64, 1>(*A, st) : D <= 48 ? pick_fwd<float, 48, 32, 1>(*A, st)
-         : D <= 64 ? pick_fwd<float, 64, 32, 1>(*A, st) : D <= 96 ? pick_fwd<float, 96, 32, 1>(*A, st) : pick_fwd<float, 128, 32, 1>(*A, st);
+    return D <= 16 ? pick_fwd<float, 16, 64>(*A, st) : D <= 32 ? pick_fwd<float, 32, 64>(*A, st) : D <= 48 ? pick_fwd<float, 48, 32>(*A, st)
+         : D <= 64 ? pick_fwd<float, 64, 32>(*A, st) : D <= 96 ? pick_fwd<float, 96, 32>(*A, st) : pick_fwd<float, 128, 32>(*A, st);
 }
+// whether rows see unlike numbers of keys
+extern "C" int dn_scene_attn_uneven(int64_t most, int64_t mean) { return 3 * mean < 2 * most; }
 // Parts of the keys of a row tile, forward and dq, where there are few tiles: none below 128 of the keys that a row sees (most), and as many as give the
 // chip's CUs three workgroups each (what their registers and LDS hold) - four where rows see unlike numbers of keys (mean far below most): then the
 // longest tile is what the rest waits for.  4096 causal bf16 rows of 8 heads: 102 us in one part, 66 + 8 to join in two; seeing all keys: 92 and 121.
 // The least part, 1000 fp32 rows and keys, 4 heads of 72 to one: 42 us with 256 keys, 37 with 128 (512 keys, 25 and 18), 33 with 64; in bf16 18.4,
 // 18.8 and 18.3 (512 keys of 8 heads of 32: 11.8, 10.7 and 13.0: the join's share grows).
 extern "C" int dn_scene_attn_key_parts(int64_t nq, int KV, int G, int64_t most, int64_t mean) {
-    const int64_t tiles = (nq * G + 63) / 64 * KV, want = tiles ? (3 * mean < 2 * most ? 1024 : 768) / tiles : 1, parts = want < most / 128 ? want : most / 128;
+    const int64_t tiles = (nq * G + 63) / 64 * KV, want = tiles ? (dn_scene_attn_uneven(most, mean) ? 1024 : 768) / tiles : 1, parts = want < most / 128 ? want : most / 128;
     return (int)(parts < 1 ? 1 : parts < 8 ? parts : 8);
 }
 #endif

@@ -642,3 +642,16 @@ def test_second_derivatives_are_refused_whatever_asks_for_them():
         grads = torch.autograd.grad(out.square().sum(), leaves, create_graph=True)
         with pytest.raises(RuntimeError, match="no second derivative"):
             sum(x.sum() for x in grads).backward()
+
+
+@pytest.mark.parametrize("H,KV,D,causal,cap,axes", [(72, 72, 64, 0, 0.0, 1), (72, 72, 72, 0, 20.0, 0), (128, 64, 128, 3, 20.0, 1), (128, 128, 33, 1, 0.0, 0)])
+def test_rows_that_fill_the_chip(H, KV, D, causal, cap, axes):
+    """bf16, enough (row, key head) tiles for two blocks of 16 rows a wave; ragged ends, a scene of one row, an empty one."""
+    ptr = [0, 300, 301, 301, 800]
+    t = inputs(D, 800, 800, H, KV, D, BF16, axes)
+    both(t, SceneLayout(ptr, causal=causal), ref.seen_matrix(ptr, None, causal), cap=cap, same=True)
+    with torch.no_grad():
+        kw = dict(slopes=t["slopes"], pos=t["pos"]) if axes else {}
+        out = scene_attention(t["q"], t["k"], t["v"], SceneLayout(ptr, causal=causal), softcap=cap, **kw)
+    want, tol = ref.attention(t["q"], t["k"], t["v"], ref.seen_matrix(ptr, None, causal), D ** -0.5, cap, t["slopes"], t["pos"], t["pos"])
+    ref.close(out, want["out"], tol["out"], "out")
