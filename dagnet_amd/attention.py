@@ -9,8 +9,7 @@ the graph layers (gat.py, gcn.py) by attention over a scene's agents, or over it
     out = scene_attention_step(q, k_cache, v_cache, k_len, step_layout)                    # the new rows of a rollout's step
 
 The kernels are csrc/scene_attn_*.hip and csrc/rotary.hip behind dagnet_op_attn_* and dagnet_op_rotary (include/dagnet_hip.h), called
-by csrc/torch_calls.cpp.  fp32 and
-bf16; there is no CPU path.
+by csrc/torch_calls.cpp.  fp32 and bf16; there is no CPU path.
 """
 from __future__ import annotations
 
@@ -206,7 +205,8 @@ def scene_attention(q, k, v, layout: SceneLayout, *, scale: Optional[float] = No
     and keys are the same); without pos the distance is that of the rows' places in their scene.
     Differentiable in q, k, v and slopes; gradients repeat bit for bit.  A row that sees nothing gives 0; what stands in keys a row does
     not see (infinities and NaN included) does not reach it.  fp32: fp32 products and sums.  bf16: fp32 scores and statistics, the
-    probabilities (and their gradients) are rounded to bf16 for the second product, the output once at the end."""
+    probabilities (and their gradients) are rounded to bf16 for the second product, the output once at the end.
+    A captured graph replays with the layout's tables: keep the layout as long as the graph."""
     if not isinstance(layout, SceneLayout):
         raise DagnetHipError("layout must be a SceneLayout")
     _matrix3(q, "q"), _matrix3(k, "k"), _matrix3(v, "v")
@@ -246,7 +246,8 @@ def scene_attention_step(q, k_cache, v_cache, k_len, layout: SceneLayout, *, sca
 
     q [nq, heads, head_dim]; k_cache, v_cache [S, room, key heads, head_dim] with any strides but the last; k_len int32 [S] ON THE DEVICE (a
     captured call follows a growing cache; values are clamped to 0 .. room); pos [nq, 1 .. 3] and k_pos [S, room, ..] with slopes.  Write
-    the new rows' own keys into the cache first if they are to see each other.  No gradient.  -> [nq, heads, head_dim]."""
+    the new rows' own keys into the cache first if they are to see each other.  What stands behind k_len does not matter; an infinity or NaN in
+    a key that is seen makes its rows not finite.  No gradient.  -> [nq, heads, head_dim]."""
     if not isinstance(layout, SceneLayout):
         raise DagnetHipError("layout must be a SceneLayout")
     if layout.masked or not layout.same_rows:
@@ -339,7 +340,8 @@ def _own_elements(t) -> bool:
 def rotary(q, k, pos, axes: RotaryAxes, *, inplace: bool = False):
     """Turns the column pairs of every head of q [n, heads, head_dim] and k [n, key heads, head_dim] (or None) by their row's positions
     pos [n, number of axes] (fp32, int32 or int64) -> (q, k).  Angles are computed in fp64, so positions may lie far from zero.
-    fp32 or bf16, any row and head strides.  Differentiable in q and k; inplace=True overwrites them (without gradient)."""
+    fp32 or bf16, any row and head strides.  Differentiable in q and k; inplace=True overwrites them (without gradient; they must not overlap, and
+    autograd sees that they changed)."""
     if not isinstance(axes, RotaryAxes):
         raise DagnetHipError("axes must be RotaryAxes")
     both = (("q", q),) if k is None else (("q", q), ("k", k))

@@ -7,6 +7,11 @@
 // delta is taken from the unrounded output.  What is left of its error (in bf16 the forward's p was rounded for its second product) moves
 // every ds of a row by p_ij e_i.  dslope, a sum over all scores of which most cancels, does not forgive that, but a row's ds have to
 // add up to nothing, so e_i = - sum_j ds_ij is known and what it did to dslope is taken back: three sums per row instead of one.
+//
+// Bound by vector instructions like the forward (the scores once per kernel, then ds).  Measured: 4093 causal bf16 rows of 8 heads of 96 to 2, dq 81 us
+// (6 D operations a pair: 476 TFLOP/s), dk and dv 118 us (8 D: 436), joins 9 us each; 32 scenes of 500 bf16 rows, 8 heads of 64, cap and three axes, 85 and
+// 93 us; 4096 fp32 scenes of ten rows, 4 heads of 16, 32 us each.  One block of 16 rows (or keys) a wave: two of 128 columns would keep 192 registers of sums
+// and operands before the first score.
 #include "scene_attn.h"
 
 namespace sattn {

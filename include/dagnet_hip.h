@@ -409,13 +409,13 @@ int dagnet_op_adam(int64_t n, float *p, float *g, float *m, float *v, const doub
  * softcap 0: no cap; axes 0: no distance term (slopes, q_pos, k_pos unused), else 1 - 3 coordinates.  Query head h reads kv head
  * h / (n_heads / n_kv_heads).  A row that sees nothing gives 0 and has no gradient; what stands in keys that a row does not see never
  * reaches it, infinities and NaN included.  dtype: 0 fp32, 1 bf16 (q, k, v, out and their gradients; everything else fp32); statistics
- * and sums are fp32.  head_dim 1 - 128.  Strides are in elements, columns have stride 1; out, dq, dk, dv are contiguous. */
+ * and sums are fp32.  head_dim 1 - 128, |scale| at most 1e15, softcap 0 or 1e-15 - 1e15.  Strides are in elements, columns have stride 1; out, dq, dk, dv are contiguous. */
 typedef struct {
     const void *q, *k, *v;               /* [nq][n_heads][head_dim], [nk][n_kv_heads][head_dim] twice */
     const float *slopes, *q_pos, *k_pos; /* [n_heads], [nq][axes], [nk][axes] */
     int64_t q_row, q_head, k_row, k_head, v_row, v_head;
     int32_t nq, nk, n_heads, n_kv_heads, head_dim, axes, dtype;
-    int32_t max_keys, mean_keys;         /* of what the rows see: whether a row's keys are split over workgroups (0, 0: never); no effect on results
+    int32_t max_keys, mean_keys;         /* of what the rows see: whether a row's keys are split over workgroups (0, 0: never), and tiles; no effect on results
                                           * but for the order of sums */
     float scale, softcap;
 } dagnet_attn;
