@@ -46,8 +46,9 @@ template <typename T> __device__ void row_slow(const SceneAttnArgs &A, int kvh, 
     if (A.lse && lane == 0) A.lse[kvh * R + r] = l == 0.f ? 0.f : m + log2_(l);
 }
 
-// MB: 16-row blocks per wave, one or two (rows_fwd() chooses): with two, every K and V fragment read from LDS serves two products.  EXACT (bf16, for a backward pass): what rounding p left over goes through the second
-// product too, so that o, and delta with it, does not carry that rounding.
+// MB: 16-row blocks per wave, one or two (rows_fwd() chooses): with two, every K and V fragment read from LDS serves two products.  EXACT
+// (bf16, for a backward pass with distances): what rounding p left over goes through the second product too, so that o, and delta with it, does not
+// carry that rounding into dslope.  dq and dk need it as little as the rounding of ds itself (the error of 4093 causal rows stays 0.24 %).
 template <typename T, int DP, int BN, int MB, bool CAP, int AX, bool EXACT>
 __global__ __launch_bounds__(256, MB == 2 ? 2 : 3) void scene_attn_fwd_kernel(const SceneAttnArgs A) {
     using X = Tr<T>;
@@ -302,7 +303,8 @@ template <typename T> __global__ __launch_bounds__(256) void scene_attn_fwd_join
 template <typename T, int DP, int BN, int MB, bool CAP, int AX> hipError_t launch_fwd(const SceneAttnArgs &A, hipStream_t st) {
     const int64_t tiles = ((int64_t)A.nq * A.G + 64 * MB - 1) / (64 * MB);
     const dim3 grid((unsigned)(tiles * A.KV * A.key_parts));
-    if (sizeof(T) == 2 && A.o32) hipLaunchKernelGGL((scene_attn_fwd_kernel<T, DP, BN, MB, CAP, AX, sizeof(T) == 2>), grid, dim3(256), 0, st, A);
+    constexpr bool EXACT = sizeof(T) == 2 && AX > 0;
+    if (EXACT && A.o32) hipLaunchKernelGGL((scene_attn_fwd_kernel<T, DP, BN, MB, CAP, AX, EXACT>), grid, dim3(256), 0, st, A);
     else hipLaunchKernelGGL((scene_attn_fwd_kernel<T, DP, BN, MB, CAP, AX, false>), grid, dim3(256), 0, st, A);
     if (A.key_parts > 1) hipLaunchKernelGGL((scene_attn_fwd_join_kernel<T>), dim3((unsigned)(((int64_t)A.nq * A.H + 7) / 8)), dim3(256), 0, st, A);
     return hipGetLastError();
@@ -312,7 +314,7 @@ template <typename T, int DP, int BN, int MB, bool CAP, int AX> hipError_t launc
 // the chip's 512 places; rows that see unlike numbers of keys need more of them, short tiles filling up behind long ones.  bf16, 8 heads to 2,
 // us with one block and with two:
 //     rows 8192, all seen, no cap: width 64 212 203, 96 364 248, 128 416 304;  causal: 126 164, 178 205, 227 258;  16384 causal: 401 361, 571 502, 812 631
-//     16384, all seen: width 32 549 538 (training 694 698);  64, one axis 896 814, cap 1184 1202;  96, cap 1486 1460, cap and an axis 1582 1617;
+//     16384, all seen: width 32 549 538;  64, one axis 896 814, cap 1184 1202;  96, cap 1486 1460, cap and an axis 1582 1617;
 //     128, cap and an axis 2136 1749, cap and three axes 2520 2618;  width 96, 544 to 704 workgroups (a second round hardly filled): 385 449, 536 572
 template <typename T, int DP, int BN, bool CAP, int AX> hipError_t rows_fwd(const SceneAttnArgs &A, hipStream_t st) {
     if constexpr (sizeof(T) == 2 && DP >= 64 && (CAP ? 2 : 0) + (AX > 1 ? 2 : AX) < DP / 32) {
