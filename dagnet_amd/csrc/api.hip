@@ -2166,7 +2166,7 @@ extern "C" hipError_t dn_scene_attn_fwd_f32(const SceneAttnArgs *, hipStream_t);
 extern "C" hipError_t dn_scene_attn_fwd_bf16(const SceneAttnArgs *, hipStream_t);
 extern "C" hipError_t dn_scene_attn_bwd_f32(const SceneAttnArgs *, float *, hipStream_t);
 extern "C" hipError_t dn_scene_attn_bwd_bf16(const SceneAttnArgs *, float *, hipStream_t);
-extern "C" int dn_scene_attn_bwd_parts(int64_t, int64_t, int, int);
+extern "C" int dn_scene_attn_bwd_parts(int64_t, int, int, int64_t);
 extern "C" int dn_scene_attn_uneven(int64_t, int64_t);
 extern "C" int dn_scene_attn_key_parts(int64_t, int, int, int64_t, int64_t);
 extern "C" hipError_t dn_scene_attn_step_f32(const SceneStepArgs *, hipStream_t);
@@ -2218,7 +2218,10 @@ static bool attn_base(const void *p, int size) { return reinterpret_cast<uintptr
 
 static bool attn_counts(const dagnet_attn *a) { return a && a->nq >= 0 && a->nk >= 0 && a->n_kv_heads >= 1 && a->n_heads >= a->n_kv_heads && a->head_dim >= 1; }
 static int key_parts(const dagnet_attn *a) { return dn_scene_attn_key_parts(a->nq, a->n_kv_heads, a->n_heads / a->n_kv_heads, a->max_keys, a->mean_keys); }
-static int row_parts(const dagnet_attn *a) { return dn_scene_attn_bwd_parts(a->nq, a->nk, a->n_kv_heads, a->n_heads / a->n_kv_heads); }
+static int row_parts(const dagnet_attn *a) {
+    const int64_t seen = a->max_keys && a->nk ? (int64_t)a->nq * a->max_keys / a->nk : a->nq;
+    return dn_scene_attn_bwd_parts(a->nk, a->n_kv_heads, a->n_heads / a->n_kv_heads, seen);
+}
 static int64_t up4(int64_t n) { return (n + 3) / 4 * 4; }        // floats to a multiple of 16 bytes
 
 extern "C" int64_t dagnet_op_attn_fwd_workspace(const dagnet_attn *a) {

@@ -619,11 +619,19 @@ template <typename T> hipError_t run_bwd(const SceneAttnArgs &A, float *dslopes,
 extern "C" hipError_t dn_scene_attn_bwd_bf16(const SceneAttnArgs *A, float *dslopes, hipStream_t st) { return sattn::run_bwd<sattn::bf16>(*A, dslopes, st); }
 #else
 extern "C" hipError_t dn_scene_attn_bwd_f32(const SceneAttnArgs *A, float *dslopes, hipStream_t st) { return sattn::run_bwd<float>(*A, dslopes, st); }
-// Parts of the rows in the dk / dv kernel: as many as give the chip four workgroups a CU, but none below 256 packed rows.  The whole backward of 1000
-// fp32 rows and keys, 4 heads of 72 to one: 199 us with at least 512, 134 with 256, 122 with 128; of 512 bf16 rows, 8 heads of 32: 54, 35 and 32.  Below
-// 256 the fp32 sums that parts leave (two for every element of k and v) are more than what the tile itself reads.
-extern "C" int dn_scene_attn_bwd_parts(int64_t nq, int64_t nk, int KV, int G) {
-    const int64_t groups = (nk + 63) / 64 * KV, want = groups ? 1024 / groups : 1, most = nq * G / 256;
-    return (int)(want < 1 || most < 1 ? 1 : want < most ? (want < 16 ? want : 16) : (most < 16 ? most : 16));
+// Parts of the rows in the dk / dv kernel.  seen: rows that see a key, where most do (the longest tile is what the rest waits for); 64 keys see about 64 more.
+// - As many as give the chip nine workgroups a CU (places for two or three at once: unlike tiles level out, and no round is left half empty), beyond 8 parts only
+//   what gives four: the join reads two fp32 sums a part.  bf16, 8 heads to 2, dk and dv with four and with nine: 16384 causal rows of 96, 1499 us and
+//   1218, of 64 960 and 781, all seen 2927 and 2391; 24000 causal, 4423 and 2646; 4093 causal (8 and 16 parts), 112 + 10 to join and 110 + 16.
+// - None below 128 packed rows of those.  fp32, 2400 causal rows in two scenes, one head of 100: the whole backward and forward 151 us with at least 256, 126 with
+//   128; 1000 rows, 4 heads of 72 to one, backward alone: 199 us with 512, 134 with 256, 122 with 128.  48 scenes of 60 - 340 rows, 4 heads of 32 to 2: 52 + 7
+//   to join with 256, 53 + 10 with 128: there the chip is full already.
+extern "C" int dn_scene_attn_bwd_parts(int64_t nk, int KV, int G, int64_t seen) {
+    const int64_t groups = (nk + 63) / 64 * KV;
+    if (!groups) return 1;
+    const int64_t four = 1024 / groups, nine = 2304 / groups, most = (seen + 64) * G / 128;
+    int64_t parts = four > 8 ? four : nine < 8 ? nine : 8;
+    parts = parts < most ? parts : most;
+    return (int)(parts < 1 ? 1 : parts < 16 ? parts : 16);
 }
 #endif
