@@ -7,7 +7,7 @@
 #include <torch/csrc/autograd/custom_function.h>
 #include <torch/csrc/autograd/functions/basic_ops.h>
 #include <torch/extension.h>
-#include <c10/hip/HIPGuard.h>
+#include <c10/core/DeviceGuard.h>
 #include <c10/hip/HIPStream.h>
 
 #include "../../include/dagnet_hip.h"
@@ -38,7 +38,8 @@ void check(int rc) {
     if (rc) throw Refused(std::string("libdagnet_hip: ") + E.last_error() + " (status " + std::to_string(rc) + ")");
 }
 
-void *stream_of(const Tensor &t) { return c10::hip::getCurrentHIPStream(t.get_device()).stream(); }
+// host tensors (no stream) reach only entries that a test has bound: dagnet_amd/attention.py refuses them
+void *stream_of(const Tensor &t) { return t.is_cuda() ? c10::hip::getCurrentHIPStream(t.get_device()).stream() : nullptr; }
 template <typename T> T *ptr(const Tensor &t) { return t.defined() ? static_cast<T *>(t.data_ptr()) : nullptr; }
 Tensor floats(const Tensor &like, int64_t n) { return at::empty({n}, like.options().dtype(at::kFloat)); }
 Tensor dense(const Tensor &like) { return at::empty_like(like, like.options(), at::MemoryFormat::Contiguous); }
@@ -47,12 +48,36 @@ Tensor columns(const Tensor &t) { return t.stride(-1) == 1 || t.size(-1) == 1 ? 
 
 Tensor given(const std::optional<Tensor> &t) { return t ? *t : Tensor(); }
 
+// What a node saved comes back from autograd as whatever the saved-tensor hooks made of it: activation checkpointing computes it again, offloading
+// copies it back.  Addresses and strides are therefore taken from what comes back and never kept from the forward call, and a tensor of another
+// shape, type or device than the saved one is refused before a kernel reads it.
+void unpacked(const Tensor &t, at::IntArrayRef sizes, at::ScalarType type, const at::Device &device, const char *what) {
+    if (t.defined() && t.sizes() == sizes && t.scalar_type() == type && t.device() == device) return;
+    throw Refused(std::string("a saved-tensor hook returned ") + what + " with another shape, type or device than was saved");
+}
+// small plain values of a call, kept with its node
+template <typename V> void keep(AutogradContext *ctx, const char *name, const V &v) {
+    ctx->saved_data[name] = std::string(reinterpret_cast<const char *>(&v), sizeof(V));
+}
+template <typename V> V kept(AutogradContext *ctx, const char *name) {
+    V v;
+    memcpy(&v, ctx->saved_data[name].toStringRef().data(), sizeof(V));
+    return v;
+}
+
 // addresses of a layout's tables on the device, and how many keys its rows see
 struct Tables {
     int64_t row_lo, row_hi, key_lo, key_hi, ptr;
     int32_t max_keys, mean_keys;
 };
 template <typename T> const T *at_address(int64_t a) { return reinterpret_cast<const T *>(a); }
+
+// what the backward pass needs of the forward call beside its tensors; axes 0: no distance
+struct Call {
+    Tables t;
+    double scale, softcap;
+    int64_t nk, kv, axes;
+};
 
 // q [nq, H, D], k and v [..., KV, D]: their row and head strides are those of the last three dimensions
 dagnet_attn arguments(const Tensor &q, const Tensor &k, const Tensor &v, const Tensor &slopes, const Tensor &pos, const Tensor &k_pos, int64_t nk, double scale,
@@ -73,7 +98,7 @@ dagnet_attn arguments(const Tensor &q, const Tensor &k, const Tensor &v, const T
 
 // -> out, and with grad the rows' statistics and the unrounded output (bf16; fp32: out itself)
 std::tuple<Tensor, Tensor, Tensor> attend(dagnet_attn &a, const Tensor &q, const Tables &t, bool grad) {
-    const c10::hip::HIPGuard guard(q.get_device());
+    const c10::DeviceGuard guard(q.device());
     Tensor out = dense(q), lse, o;
     if (grad) {
         lse = floats(q, q.size(0) * q.size(1));
@@ -102,21 +127,38 @@ struct SceneAttn : torch::autograd::Function<SceneAttn> {
         a.max_keys = t.max_keys;
         a.mean_keys = t.mean_keys;
         auto [out, lse, o] = attend(a, q, t, true);
-        ctx->save_for_backward({q, k, v, slopes, pos, k_pos, lse, o, held});
-        ctx->saved_data["args"] = std::string(reinterpret_cast<const char *>(&a), sizeof(a));
-        ctx->saved_data["tables"] = std::string(reinterpret_cast<const char *>(&t), sizeof(t));
+        ctx->save_for_backward({q, k, v, slopes, pos, k_pos, lse, o});
+        ctx->saved_data["held"] = held;                     // no saved variable: a hook would put a copy in its place, and the addresses are held's own
+        keep(ctx, "call", Call{t, scale, softcap, k.size(0), k.size(1), a.axes});
         return out;
     }
     static variable_list backward(AutogradContext *ctx, const variable_list &grads) {
-        dagnet_attn a;
-        Tables t;
-        memcpy(&a, ctx->saved_data["args"].toStringRef().data(), sizeof(a));
-        memcpy(&t, ctx->saved_data["tables"].toStringRef().data(), sizeof(t));
+        const Call call = kept<Call>(ctx, "call");
+        const Tables &t = call.t;
         const variable_list saved = ctx->get_saved_variables();
-        const Tensor &q = saved[0], &k = saved[1], &v = saved[2], &slopes = saved[3], &lse = saved[6], &o = saved[7];
         const Tensor dout = columns(grads[0]);
+        const int64_t rows = dout.size(0), heads = dout.size(1), D = dout.size(2);
+        const at::ScalarType type = dout.scalar_type();
+        unpacked(saved[0], {rows, heads, D}, type, dout.device(), "q");
+        unpacked(saved[1], {call.nk, call.kv, D}, type, dout.device(), "k");
+        unpacked(saved[2], {call.nk, call.kv, D}, type, dout.device(), "v");
+        Tensor slopes, pos, k_pos;
+        if (call.axes) {
+            unpacked(saved[3], {heads}, at::kFloat, dout.device(), "slopes");
+            unpacked(saved[4], {rows, call.axes}, at::kFloat, dout.device(), "pos");
+            unpacked(saved[5], {call.nk, call.axes}, at::kFloat, dout.device(), "k_pos");
+            slopes = saved[3].contiguous();
+            pos = saved[4].contiguous();
+            k_pos = saved[5].contiguous();
+        }
+        unpacked(saved[6], {rows * heads}, at::kFloat, dout.device(), "the rows' statistics");
+        unpacked(saved[7], {rows, heads, D}, at::kFloat, dout.device(), "the output");
+        const Tensor q = columns(saved[0]), k = columns(saved[1]), v = columns(saved[2]), lse = saved[6].contiguous(), o = saved[7].contiguous();
+        dagnet_attn a = arguments(q, k, v, slopes, pos, k_pos, call.nk, call.scale, call.softcap);
+        a.max_keys = t.max_keys;
+        a.mean_keys = t.mean_keys;
         const bool nq = ctx->needs_input_grad(0), nk = ctx->needs_input_grad(1), nv = ctx->needs_input_grad(2), ns = slopes.defined() && ctx->needs_input_grad(3);
-        const c10::hip::HIPGuard guard(q.get_device());
+        const c10::DeviceGuard guard(q.device());
         Tensor dq, dk, dv, ds;
         if (nq || ns) dq = dense(q);
         if (nk || nv) {
@@ -158,7 +200,7 @@ Tensor scene_attn_step(const Tensor &q, const Tensor &k, const Tensor &v, const 
                        const std::optional<Tensor> &pos_, const std::optional<Tensor> &k_pos_, double scale, double softcap) {
     py::gil_scoped_release release;
     dagnet_attn a = arguments(q, k, v, given(slopes_), given(pos_), given(k_pos_), 0, scale, softcap);
-    const c10::hip::HIPGuard guard(q.get_device());
+    const c10::DeviceGuard guard(q.device());
     const int32_t scenes = (int32_t)k.size(0), room = (int32_t)k.size(1);
     Tensor out = dense(q);
     const int64_t n = E.step_workspace(&a, scenes, room, (int32_t)max_rows);
@@ -176,7 +218,7 @@ struct Axes {
 };
 
 void turn(const Tensor &q, const Tensor &k, const Tensor &pos, const Axes &x, bool inverse, const Tensor &qo, const Tensor &ko) {
-    const c10::hip::HIPGuard guard(q.get_device());
+    const c10::DeviceGuard guard(q.device());
     const bool two = k.defined();
     const int type = pos.scalar_type() == at::kFloat ? 0 : pos.scalar_type() == at::kInt ? 1 : 2;
     check(E.rotary(q.size(0), (int32_t)q.size(1), two ? (int32_t)k.size(1) : 0, (int32_t)q.size(2), q.scalar_type() == at::kBFloat16, q.data_ptr(), q.stride(0),
@@ -190,14 +232,18 @@ struct Rotary : torch::autograd::Function<Rotary> {
         const Tensor k = given(k_);
         const Tensor qo = dense(q), ko = k.defined() ? dense(k) : Tensor();
         turn(q, k, pos, x, false, qo, ko);
-        ctx->save_for_backward({pos, held});
-        ctx->saved_data["axes"] = std::string(reinterpret_cast<const char *>(&x), sizeof(x));
+        ctx->save_for_backward({pos});
+        ctx->saved_data["held"] = held;                     // as in SceneAttn
+        keep(ctx, "axes", x);
+        keep(ctx, "pos", std::array<int64_t, 2>{pos.size(1), (int64_t)pos.scalar_type()});
         return k.defined() ? variable_list{qo, ko} : variable_list{qo};
     }
     static variable_list backward(AutogradContext *ctx, const variable_list &grads) {
-        Axes x;
-        memcpy(&x, ctx->saved_data["axes"].toStringRef().data(), sizeof(x));
-        const Tensor pos = ctx->get_saved_variables()[0], gq = columns(grads[0]), gk = grads.size() > 1 ? columns(grads[1]) : Tensor();
+        const Axes x = kept<Axes>(ctx, "axes");
+        const auto was = kept<std::array<int64_t, 2>>(ctx, "pos");
+        const Tensor gq = columns(grads[0]), gk = grads.size() > 1 ? columns(grads[1]) : Tensor(), back = ctx->get_saved_variables()[0];
+        unpacked(back, {gq.size(0), was[0]}, (at::ScalarType)was[1], gq.device(), "pos");
+        const Tensor pos = back.contiguous();
         const Tensor dq = dense(gq), dk = gk.defined() ? dense(gk) : Tensor();
         turn(gq, gk, pos, x, true, dq, dk);
         return once({dq, dk, Tensor(), Tensor(), Tensor()}, "rotary");

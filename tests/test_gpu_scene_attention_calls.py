@@ -1,0 +1,47 @@
+"""GPU: attention and rotary calls as programs around them make them - under activation checkpointing and saved-tensor hooks, on empty batches, with a
+scale of nothing, split over many workgroups beside spoilt rows, straight from the C entries."""
+import gc
+
+import pytest
+import torch
+from torch.utils.checkpoint import checkpoint
+
+from dagnet_amd.attention import RotaryAxes, SceneLayout, rotary, scene_attention, scene_attention_step
+from tests import scene_attn_ref as ref
+from tests.test_gpu_scene_attention import BF16, DEV, F32, both, inputs, randn, step_inputs, step_want
+
+pytestmark = pytest.mark.gpu
+
+
+def _block(q, k, v, slopes, pos, w):
+    """A layer's call: projections whose memory nobody else holds, tables that only this call has."""
+    axes = RotaryAxes(q.shape[2], (4, 4))
+    layout = SceneLayout([0, 37, 90], causal=3)
+    a, b = rotary(q * w, k * w, pos * 2.0, axes)
+    return scene_attention(a, b, v + w, layout, softcap=10.0, slopes=slopes * 0.5, pos=pos * 1.0)
+
+
+class _Copies(torch.autograd.graph.saved_tensors_hooks):
+    def __init__(self):
+        super().__init__(lambda t: t.detach().clone(), lambda t: t.clone())
+
+
+@pytest.mark.parametrize("dt", [F32, BF16], ids=["fp32", "bf16"])
+@pytest.mark.parametrize("how", ["checkpoint", "on_host", "copies"])
+def test_gradients_under_hooks_equal_the_direct_ones(how, dt):
+    t = inputs(13, 90, 90, 4, 2, 16, dt, 2)
+    w = torch.tensor(1.25, device=DEV, dtype=dt)
+    leaves = [t[n].requires_grad_() for n in ("q", "k", "v", "slopes")]
+    args = (*leaves, t["pos"], w)
+    want = torch.autograd.grad(_block(*args), leaves, t["dout"])
+    if how == "checkpoint":
+        out = checkpoint(_block, *args, use_reentrant=False)
+    else:
+        with torch.autograd.graph.save_on_cpu() if how == "on_host" else _Copies():
+            out = _block(*args)
+    gc.collect()
+    junk = [torch.full((n,), 3, dtype=torch.int32, device=DEV) for n in (64, 400, 1440, 2880, 5760) for _ in range(24)]     # takes what was freed
+    got = torch.autograd.grad(out, leaves, t["dout"])
+    del junk
+    for a, b in zip(got, want):
+        assert torch.equal(a, b)
