@@ -390,6 +390,10 @@ template <bool CAP, int AX, bool FINE> struct Score {
     }
 };
 
+// Without cap and distance the kernels mask raw products with -inf and apply the factor later.  -inf times 0 is NaN, so a scale that is 0 (or a
+// denormal, which a product may flush) takes the form that applies the factor first: one axis of no length.
+inline bool factor_last(const SceneAttnArgs &A) { return A.axes == 0 && __builtin_fabsf(A.scale) >= 0x1p-126f; }
+
 // the same with everything read at run time (the slow forms)
 __device__ __forceinline__ float score2(const SceneAttnArgs &A, float raw, float inv_cap, float slope2, const float *qpos, const float *kpos) {
     float x = raw * A.scale;

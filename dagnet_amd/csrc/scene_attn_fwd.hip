@@ -325,7 +325,7 @@ template <typename T, int DP, int BN, bool CAP, int AX> hipError_t rows_fwd(cons
 }
 template <typename T, int DP, int BN> hipError_t pick_fwd(const SceneAttnArgs &A, hipStream_t st) {
     if (A.cap > 0.f) return A.axes == 0 ? rows_fwd<T, DP, BN, true, 0>(A, st) : A.axes == 1 ? rows_fwd<T, DP, BN, true, 1>(A, st) : rows_fwd<T, DP, BN, true, 3>(A, st);
-    return A.axes == 0 ? rows_fwd<T, DP, BN, false, 0>(A, st) : A.axes == 1 ? rows_fwd<T, DP, BN, false, 1>(A, st) : rows_fwd<T, DP, BN, false, 3>(A, st);
+    return factor_last(A) ? rows_fwd<T, DP, BN, false, 0>(A, st) : A.axes <= 1 ? rows_fwd<T, DP, BN, false, 1>(A, st) : rows_fwd<T, DP, BN, false, 3>(A, st);
 }
 
 }  // namespace sattn

@@ -67,7 +67,7 @@ template <typename T, int DP, bool CAP, int AX> __global__ __launch_bounds__(256
 
     const int64_t pr = min((int64_t)cb * 16 + c, n - 1);
     const int row = q0 + (int)(pr / A.a.G), head = kvh * A.a.G + (int)(pr % A.a.G);
-    const float slope = AX ? A.a.slopes[head] * LOG2E : 0.f;
+    const float slope = AX && A.a.axes ? A.a.slopes[head] * LOG2E : 0.f;
     float qpos[3];
 #pragma unroll
     for (int a = 0; a < 3; ++a) qpos[a] = a < AX && a < A.a.axes ? A.a.qpos[(int64_t)row * A.a.axes + a] : 0.f;
@@ -233,7 +233,7 @@ template <typename T, int DP, bool CAP, int AX> hipError_t launch_step(const Sce
 template <typename T, int DP> hipError_t pick_step(const SceneStepArgs &A, hipStream_t st) {
     const int ax = A.a.axes;
     if (A.a.cap > 0.f) return ax == 0 ? launch_step<T, DP, true, 0>(A, st) : ax == 1 ? launch_step<T, DP, true, 1>(A, st) : launch_step<T, DP, true, 3>(A, st);
-    return ax == 0 ? launch_step<T, DP, false, 0>(A, st) : ax == 1 ? launch_step<T, DP, false, 1>(A, st) : launch_step<T, DP, false, 3>(A, st);
+    return factor_last(A.a) ? launch_step<T, DP, false, 0>(A, st) : ax <= 1 ? launch_step<T, DP, false, 1>(A, st) : launch_step<T, DP, false, 3>(A, st);
 }
 
 }  // namespace sattn

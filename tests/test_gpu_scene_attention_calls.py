@@ -45,3 +45,23 @@ def test_gradients_under_hooks_equal_the_direct_ones(how, dt):
     del junk
     for a, b in zip(got, want):
         assert torch.equal(a, b)
+
+
+@pytest.mark.parametrize("dt", [F32, BF16], ids=["fp32", "bf16"])
+@pytest.mark.parametrize("scale", [0.0, -0.0, 1e-50, 1e-40])
+@pytest.mark.parametrize("rows,lens,room", [([1], [1], 1), ([3, 2], [37, 90], 100), ([10, 1, 4], [1001, 0, 700], 1111)])
+def test_a_step_with_a_scale_of_nothing_gives_the_mean(rows, lens, room, scale, dt):
+    """Scores are 0 (1e-50 is 0 in fp32, 1e-40 a denormal): all kept keys weigh the same, one split of the keys or several."""
+    t = step_inputs(room, rows, lens, room, 4, 2, 24, dt, 0)
+    got = scene_attention_step(t["q"], t["k"], t["v"], t["k_len"], SceneLayout(t["ptr"]), scale=scale)
+    want, tol = step_want(t, lens, 0.0, scale)
+    ref.close(got, want["out"], tol["out"], "step")
+
+
+@pytest.mark.parametrize("dt", [F32, BF16], ids=["fp32", "bf16"])
+@pytest.mark.parametrize("cap", [0.0, 5.0])
+@pytest.mark.parametrize("scale", [0.0, 1e-40])
+@pytest.mark.parametrize("ptr,causal", [([0, 5, 70], 1), ([0, 1, 300], 0), ([0, 700], 1)])
+def test_a_scale_of_nothing_forward_and_backward(ptr, causal, scale, cap, dt):
+    t = inputs(3, ptr[-1], ptr[-1], 4, 2, 24, dt, 0)
+    both(t, SceneLayout(ptr, causal=causal), ref.seen_matrix(ptr, None, causal), scale=scale, cap=cap)
