@@ -2258,7 +2258,7 @@ extern "C" int dagnet_op_attn_bwd(const dagnet_attn *a, const int32_t *row_lo, c
     SceneAttnArgs A;
     if (int rc = attn_args(a, &A)) return rc;
     OP_NEED((dk == nullptr) == (dv == nullptr), "dk and dv go together");
-    OP_NEED(!dslopes || (dq && a->axes), "dslopes needs dq and a distance term");
+    OP_NEED(!dslopes || ((dq || a->nq == 0) && a->axes), "dslopes needs dq and a distance term");      // without rows dq is an empty tensor, whose address is null
     const int size = a->dtype ? 2 : 4;
     OP_NEED(a->nq == 0 || (row_lo && row_hi && dout && lse && o && workspace), "null argument");
     OP_NEED(a->nk == 0 || (a->k && a->v && (!dk || (key_lo && key_hi)) && (!a->axes || a->k_pos)), "null argument");

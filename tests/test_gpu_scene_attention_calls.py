@@ -65,3 +65,18 @@ def test_a_step_with_a_scale_of_nothing_gives_the_mean(rows, lens, room, scale, 
 def test_a_scale_of_nothing_forward_and_backward(ptr, causal, scale, cap, dt):
     t = inputs(3, ptr[-1], ptr[-1], 4, 2, 24, dt, 0)
     both(t, SceneLayout(ptr, causal=causal), ref.seen_matrix(ptr, None, causal), scale=scale, cap=cap)
+
+
+@pytest.mark.parametrize("axes", [1, 2, 3])
+@pytest.mark.parametrize("q_ptr,k_ptr", [([0, 0], [0, 30]), ([0, 30], [0, 0]), ([0, 0], [0, 0]), ([0, 0, 7], [0, 12, 12])])
+def test_no_rows_or_no_keys_with_learned_slopes(q_ptr, k_ptr, axes):
+    t = inputs(1, q_ptr[-1], k_ptr[-1], 2, 2, 16, F32, axes)
+    out, grads = both(t, SceneLayout(q_ptr, k_ptr), torch.zeros((q_ptr[-1], k_ptr[-1]), dtype=torch.bool))
+    assert (out == 0).all() and all((g == 0).all() for g in grads) and grads[3].shape == (2,)
+
+
+def test_an_empty_batch_trains_with_the_default_positions():
+    q, k = torch.zeros((0, 2, 16), device=DEV, requires_grad=True), torch.zeros((0, 1, 16), device=DEV, requires_grad=True)
+    slopes = torch.full((2,), 0.5, device=DEV, requires_grad=True)
+    got = torch.autograd.grad(scene_attention(q, k, k, SceneLayout([0, 0, 0]), slopes=slopes).sum(), (q, k, slopes))
+    assert got[0].shape == q.shape and got[1].shape == k.shape and (got[2] == 0).all()
