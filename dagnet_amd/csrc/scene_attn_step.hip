@@ -184,7 +184,8 @@ template <typename T, int DP, bool CAP, int AX> __global__ __launch_bounds__(256
     }
 }
 
-// The splits of a (row, head) joined: TP threads, 32 of them over the columns (four each), the rest over the splits.
+// The splits of a (row, head) joined: TP threads, 32 of them over the columns (four each), the rest over the splits.  Rows that no scene owns (in front of the
+// first one's, behind the last one's) have no splits and stay as they were.
 template <typename T, int TP> __global__ __launch_bounds__(256) void scene_attn_join_kernel(const SceneStepArgs A) {
     constexpr int IT = 256 / TP, GR = TP / 32;
     __shared__ f32x4 so[256];
@@ -220,7 +221,9 @@ template <typename T, int TP> __global__ __launch_bounds__(256) void scene_attn_
         o += f * so[it * TP + i * 32 + t];
     }
     const float inv = l == 0.f ? 0.f : 1.f / l;
-    if ((int64_t)blockIdx.x * IT + it < items) store4(reinterpret_cast<T *>(A.a.out) + item * D, o * inv, d, D, A.a.o_vec != 0);
+    const int64_t row = item / A.a.H;
+    const bool owned = row >= A.q_ptr[0] && row < A.q_ptr[A.scenes];
+    if (owned && (int64_t)blockIdx.x * IT + it < items) store4(reinterpret_cast<T *>(A.a.out) + item * D, o * inv, d, D, A.a.o_vec != 0);
 }
 
 template <typename T, int DP, bool CAP, int AX> hipError_t launch_step(const SceneStepArgs &A, hipStream_t st) {

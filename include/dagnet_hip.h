@@ -434,8 +434,8 @@ int dagnet_op_attn_bwd(const dagnet_attn *a, const int32_t *row_lo, const int32_
                        void *dk, void *dv, float *dslopes, void *stream);
 /* The same attention for the new rows of a step over kept keys: scene s has the query rows q_ptr[s] .. q_ptr[s + 1] - 1 (at most max_rows
  * of them), which all see the first k_len[s] of its `room` cache rows (k_len is clamped to 0 .. room).  k, v: [scenes][room][n_kv_heads]
- * [head_dim], k_scene / v_scene elements between scenes; k_pos [scenes][room][axes] contiguous; nk of `a` is not read.  q_ptr and
- * k_len are DEVICE arrays, so a captured call follows a growing cache.  workspace: dagnet_op_attn_step_workspace() floats (0: may be
+ * [head_dim], k_scene / v_scene elements between scenes; k_pos [scenes][room][axes] contiguous; nk of `a` is not read.  Rows in front of
+ * q_ptr[0] and from q_ptr[scenes] on are left as they were in out.  q_ptr and k_len are DEVICE arrays, so a captured call follows a growing cache.  workspace: dagnet_op_attn_step_workspace() floats (0: may be
  * NULL), private to the call until it has run. */
 int64_t dagnet_op_attn_step_workspace(const dagnet_attn *a, int32_t scenes, int32_t room, int32_t max_rows);
 int dagnet_op_attn_step(const dagnet_attn *a, const int32_t *q_ptr, const int32_t *k_len, int32_t scenes, int32_t room, int32_t max_rows,

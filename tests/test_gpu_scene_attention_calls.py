@@ -1,13 +1,16 @@
 """GPU: attention and rotary calls as programs around them make them - under activation checkpointing and saved-tensor hooks, on empty batches, with a
 scale of nothing, split over many workgroups beside spoilt rows, straight from the C entries."""
+import ctypes as C
 import gc
 
 import pytest
 import torch
 from torch.utils.checkpoint import checkpoint
 
+from dagnet_amd import _ops
 from dagnet_amd.attention import RotaryAxes, SceneLayout, rotary, scene_attention, scene_attention_step
 from tests import scene_attn_ref as ref
+from tests.attn_recorder import Attn
 from tests.test_gpu_scene_attention import BF16, DEV, F32, both, inputs, randn, step_inputs, step_want
 
 pytestmark = pytest.mark.gpu
@@ -80,3 +83,34 @@ def test_an_empty_batch_trains_with_the_default_positions():
     slopes = torch.full((2,), 0.5, device=DEV, requires_grad=True)
     got = torch.autograd.grad(scene_attention(q, k, k, SceneLayout([0, 0, 0]), slopes=slopes).sum(), (q, k, slopes))
     assert got[0].shape == q.shape and got[1].shape == k.shape and (got[2] == 0).all()
+
+
+def _step_entry(t, ptr, lens, max_rows, out, dtype):
+    """dagnet_op_attn_step itself: rows of q that no scene owns can be named there only."""
+    lib = _ops._lib()
+    S, room, KV, D = t["k"].shape
+    H = t["q"].shape[1]
+    a = Attn(q=t["q"].data_ptr(), k=t["k"].data_ptr(), v=t["v"].data_ptr(), q_row=H * D, q_head=D, k_row=KV * D, k_head=D, v_row=KV * D, v_head=D, nq=t["q"].shape[0],
+             nk=0, n_heads=H, n_kv_heads=KV, head_dim=D, axes=0, dtype=dtype, scale=D ** -0.5, softcap=0.0)
+    q_ptr, k_len = (torch.tensor(x, dtype=torch.int32, device=DEV) for x in (ptr, lens))
+    ws = torch.full((max(1, lib.dagnet_op_attn_step_workspace(C.byref(a), S, room, max_rows)),), 1e3, device=DEV)
+    rc = lib.dagnet_op_attn_step(C.byref(a), q_ptr.data_ptr(), k_len.data_ptr(), S, room, max_rows, room * KV * D, room * KV * D, out.data_ptr(), ws.data_ptr(),
+                                 torch.cuda.current_stream().cuda_stream)
+    torch.cuda.synchronize()
+    return rc, ws.numel()
+
+
+@pytest.mark.parametrize("dt", [F32, BF16], ids=["fp32", "bf16"])
+@pytest.mark.parametrize("room", [90, 700, 5000])
+def test_rows_of_a_step_that_no_scene_owns_stay_as_they_were(room, dt):
+    """Rows before the first scene's and behind the last one's, with the keys in one split (90) and in several."""
+    ptr, lens = [1, 4, 4, 6], [room - 3, 5, room]
+    t = step_inputs(room, [9, 0, 0], lens, room, 4, 2, 32, dt, 0)
+    out = torch.full((9, 4, 32), 7.0, device=DEV, dtype=dt)
+    rc, ws = _step_entry(t, ptr, lens, 3, out, int(dt is BF16))
+    assert rc == 0 and (ws > 1) == (room > 256)
+    assert (out[:1] == 7.0).all() and (out[6:] == 7.0).all()
+    t["ptr"] = [0, 3, 3, 5]
+    t["q"] = t["q"][1:6]
+    want, tol = step_want(t, lens, 0.0, 32 ** -0.5)
+    ref.close(out[1:6], want["out"], tol["out"], "step")
