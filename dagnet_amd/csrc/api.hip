@@ -2284,12 +2284,16 @@ extern "C" int dagnet_op_attn_bwd(const dagnet_attn *a, const int32_t *row_lo, c
     return DAGNET_OK;
 }
 
+// scenes by key heads, and blocks of 16 packed rows of a scene, that a launch can count (and step_shape's products hold)
+static bool step_counts(const dagnet_attn *a, int32_t scenes, int32_t max_rows) {
+    return (int64_t)scenes * a->n_kv_heads <= ATTN_BLOCKS && (int64_t)max_rows * (a->n_heads / a->n_kv_heads) <= 16 * ATTN_BLOCKS;
+}
 static void step_shape(const dagnet_attn *a, int32_t scenes, int32_t room, int32_t max_rows, int *cblocks, int *splits) {
     dn_scene_attn_step_shape((int64_t)max_rows * (a->n_heads / a->n_kv_heads), (int64_t)scenes * a->n_kv_heads, room, cblocks, splits);
 }
 
 extern "C" int64_t dagnet_op_attn_step_workspace(const dagnet_attn *a, int32_t scenes, int32_t room, int32_t max_rows) {
-    if (!a || scenes < 1 || room < 1 || max_rows < 1 || a->n_kv_heads < 1 || a->n_heads < a->n_kv_heads) return 0;
+    if (!a || scenes < 1 || room < 1 || max_rows < 1 || a->n_kv_heads < 1 || a->n_heads < a->n_kv_heads || !step_counts(a, scenes, max_rows)) return 0;
     int cb, sp;
     step_shape(a, scenes, room, max_rows, &cb, &sp);
     return sp == 1 ? 0 : (int64_t)a->nq * a->n_heads * sp * (a->head_dim + 2);
@@ -2302,10 +2306,11 @@ extern "C" int dagnet_op_attn_step(const dagnet_attn *a, const int32_t *q_ptr, c
     OP_NEED(scenes >= 0 && room >= 0 && room <= 0x7fff0000 && max_rows >= 0, "bad argument");
     if (a->nq == 0 || scenes == 0) return DAGNET_OK;
     OP_NEED(max_rows >= 1 && q_ptr && k_len && out && (room == 0 || (a->k && a->v && (!a->axes || a->k_pos))), "bad argument");
+    OP_NEED(step_counts(a, scenes, max_rows), "too many rows for one launch");
     A.q_ptr = q_ptr; A.k_len = k_len; A.scenes = scenes; A.room = room; A.k_ss = k_scene; A.v_ss = v_scene;
     step_shape(a, scenes, room, max_rows, &A.cblocks, &A.splits);
-    OP_NEED((int64_t)scenes * a->n_kv_heads <= ATTN_BLOCKS && (int64_t)scenes * a->n_kv_heads * A.cblocks * A.splits <= ATTN_BLOCKS, "too many rows for one launch");
-    OP_NEED(A.splits == 1 || workspace, "workspace is NULL");
+    OP_NEED((int64_t)scenes * a->n_kv_heads * A.cblocks * A.splits <= ATTN_BLOCKS, "too many rows for one launch");
+    OP_NEED(A.splits == 1 || (workspace && attn_base(workspace, 4)), "workspace must be there and 16-byte aligned");
     const int size = a->dtype ? 2 : 4;
     A.a.out = out;
     A.a.k_vec = std::min(A.a.k_vec, attn_vec(a->k, k_scene, a->k_head, a->head_dim, size));
