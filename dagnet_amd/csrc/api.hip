@@ -2245,12 +2245,12 @@ extern "C" int dagnet_op_attn_fwd(const dagnet_attn *a, const int32_t *row_lo, c
     return DAGNET_OK;
 }
 
-// delta | dsl | parts of dq | their sums for dslope | parts of dk and dv
+// delta | dsl | parts of dq | their sums for dslope (fp64) | parts of dk and dv
 extern "C" int64_t dagnet_op_attn_bwd_workspace(const dagnet_attn *a) {
     if (!attn_counts(a)) return 0;
     const int64_t items = (int64_t)a->nq * a->n_heads, keys = (int64_t)a->nk * a->n_kv_heads * a->head_dim;
     const int kp = key_parts(a), rp = row_parts(a);
-    return up4(2 * items) + (kp > 1 ? up4(items * kp * a->head_dim) + up4(items * kp * 3) : 0) + (rp > 1 ? 2 * rp * keys : 0);
+    return up4(2 * items) + (kp > 1 ? up4(items * kp * a->head_dim) + up4(6 * items * kp) : 0) + (rp > 1 ? 2 * rp * keys : 0);
 }
 extern "C" int dagnet_op_attn_bwd(const dagnet_attn *a, const int32_t *row_lo, const int32_t *row_hi, const int32_t *key_lo,
                                   const int32_t *key_hi, const void *dout, int64_t do_row, int64_t do_head, const float *lse, const float *o,
@@ -2276,7 +2276,7 @@ extern "C" int dagnet_op_attn_bwd(const dagnet_attn *a, const int32_t *row_lo, c
     if (A.key_parts > 1) {
         A.part = next;
         A.stat = next + up4(items * A.key_parts * a->head_dim);
-        next = A.stat + up4(items * A.key_parts * 3);
+        next = A.stat + up4(6 * items * A.key_parts);
     }
     if (A.parts > 1) A.part2 = next;
     if (!attn_base(dq, size) || !attn_base(dk, size) || !attn_base(dv, size)) A.o_vec = 0;

@@ -29,7 +29,7 @@ struct SceneAttnArgs {
     int32_t nq, nk, H, KV, G, D, axes;
     float scale, cap;
     // Few tiles: their long axis is cut, the parts' sums meet in a join kernel.  key_parts: of a row tile's keys (forward: part [nq H][parts][D], stat
-    // [nq H][parts][2]; dq: part [nq H][parts][D], stat [nq H][parts][3]); parts: of a key tile's rows (part2 [parts][dk, dv][nk][KV][D])
+    // [nq H][parts][2]; dq: part [nq H][parts][D], stat fp64 [nq H][parts][3]: most of them cancels between the parts); parts: of a key tile's rows (part2 [parts][dk, dv][nk][KV][D])
     int32_t key_parts, parts, uneven;          // uneven: rows see unlike numbers of keys (the longest at least 1.5 times the mean)
     float *part, *stat, *part2;
     int32_t q_vec, k_vec, v_vec, do_vec, o32_vec;   // bytes per load that strides, base and width allow: 16, 8 or the element

@@ -319,8 +319,8 @@ __global__ __launch_bounds__(256) void scene_attn_dq_kernel(const SceneAttnArgs 
 #pragma unroll
             for (int d = 0; d < DB; ++d) store4(A.part + (item * A.key_parts + part) * A.D, acc[d] * A.scale, d * 16 + g * 4, A.D, A.D % 4 == 0);
             if (AX > 0 && g == 0) {
-                float *st = A.stat + (item * A.key_parts + part) * 3;
-                st[0] = (float)sl.ds; st[1] = (float)sl.dsd; st[2] = (float)sl.pd;
+                double *st = reinterpret_cast<double *>(A.stat) + (item * A.key_parts + part) * 3;
+                st[0] = sl.ds; st[1] = sl.dsd; st[2] = sl.pd;
             }
         }
         return;
@@ -546,7 +546,7 @@ template <typename T> __global__ __launch_bounds__(256) void scene_attn_dq_join_
     Slope s;
     if (A.dsl)
         for (int i = 0; i < P; ++i) {
-            const float *st = A.stat + (item * P + i) * 3;
+            const double *st = reinterpret_cast<const double *>(A.stat) + (item * P + i) * 3;
             s.ds += st[0];
             s.dsd += st[1];
             s.pd += st[2];

@@ -114,3 +114,20 @@ def test_rows_of_a_step_that_no_scene_owns_stay_as_they_were(room, dt):
     t["q"] = t["q"][1:6]
     want, tol = step_want(t, lens, 0.0, 32 ** -0.5)
     ref.close(out[1:6], want["out"], tol["out"], "step")
+
+
+def test_sums_of_the_slopes_gradient_keep_their_bits_between_key_parts():
+    """One row over 1024 keys in eight parts, all scores 0: p = 2^-10, the values' mean is 0, so dslope = -2^-10 sum_j v_j d_j.  With v = +-255 and whole distances
+    below 2^12 every fp32 sum of a lane's 16 pairs is exact (16 2^20 = 2^24); a part's 128 need 27 bits, and the parts cancel to fewer than 24."""
+    g = torch.Generator().manual_seed(2)
+    n = 1024
+    d = torch.randint(2 ** 11, 2 ** 12, (n,), generator=g).double() // 2 * 2 + 1
+    v = torch.where(torch.arange(n) < n // 2, 255.0, -255.0)
+    q, k = torch.zeros((1, 1, 1), device=DEV), torch.ones((n, 1, 1), device=DEV)
+    slopes = torch.zeros(1, device=DEV, requires_grad=True)
+    out = scene_attention(q, k, v.view(n, 1, 1).to(DEV), SceneLayout([0, 1], [0, n]), slopes=slopes, pos=torch.zeros((1, 1), device=DEV),
+                          k_pos=d.float().view(n, 1).to(DEV))
+    assert float(out.detach()) == 0.0
+    got, = torch.autograd.grad(out, slopes, torch.ones_like(out))
+    want = -float((v.double() * d).sum()) / n
+    assert abs(want * n) < 2 ** 24 and float(got) == want
