@@ -131,3 +131,14 @@ def test_sums_of_the_slopes_gradient_keep_their_bits_between_key_parts():
     got, = torch.autograd.grad(out, slopes, torch.ones_like(out))
     want = -float((v.double() * d).sum()) / n
     assert abs(want * n) < 2 ** 24 and float(got) == want
+
+
+@pytest.mark.parametrize("dt", [F32, BF16], ids=["fp32", "bf16"])
+@pytest.mark.parametrize("N", [700, 3000])
+def test_a_gradient_of_nan_gives_nan(N, dt):
+    """What a loss that overflowed sends back: every key is taken one by one then."""
+    t = inputs(2, N, N, 4, 2, 32, dt, 0)
+    leaves = [t[n].requires_grad_() for n in ("q", "k", "v")]
+    out = scene_attention(*leaves, SceneLayout([0, N], causal=1))
+    grads = torch.autograd.grad(out, leaves, torch.full_like(out, float("nan")))
+    assert torch.isfinite(out).all() and all(g.isnan().all() for g in grads)
