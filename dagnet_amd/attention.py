@@ -124,6 +124,7 @@ class SceneLayout(_Tables):
         keys = np.arange(self.nk)
         self._tab = np.concatenate([lo, hi, np.searchsorted(hi, keys, side="right"), np.searchsorted(lo, keys, side="right"), q, k]).astype(np.int32)
         self._at, self._k_at = at, keys - np.repeat(k[:-1], n_k)
+        self.far = bool(np.any(np.maximum(n_q, n_k) > 1 << 24))                 # a place may be no fp32 number
         if device is not None:
             self.tables(_device(device).index)
 
@@ -140,6 +141,8 @@ class SceneLayout(_Tables):
 
     def places(self, index):
         """-> fp32 [nq, 1], [nk, 1]: the places of rows and keys in their scenes, on device ``index``."""
+        if self.far:
+            raise DagnetHipError("places in a scene of more than 2^24 rows or keys are no fp32 numbers: pass pos (and k_pos)")
         t = self.tables(index)[-1][len(self._tab):].view(torch.float32)
         return t[:self.nq, None], t[self.nq:, None]
 
@@ -202,7 +205,8 @@ def scene_attention(q, k, v, layout: SceneLayout, *, scale: Optional[float] = No
     q [nq, heads, head_dim], k and v [nk, key heads, head_dim] (head h reads key head h // (heads // key heads)), fp32 or bf16 with any row
     and head strides -> [nq, heads, head_dim].  scale: default head_dim ** -0.5.  softcap 0: scores are not capped.  slopes fp32 [heads]:
     decay of a score with the Euclidean distance of the rows' positions, pos [nq, 1 .. 3] fp32 (k_pos [nk, ..]: default pos where rows
-    and keys are the same); without pos the distance is that of the rows' places in their scene.
+    and keys are the same); without pos the distance is that of the rows' places in their scene (scenes of at most 2^24 rows and keys).  Differences of
+    positions stay below 1e19: their squares leave fp32 beyond, such a key has no weight for a positive slope, and a slope of 0 and the slopes' gradient give NaN.
     Differentiable in q, k, v and slopes; gradients repeat bit for bit.  A row that sees nothing gives 0; what stands in keys a row does
     not see (infinities and NaN included) does not reach it.  fp32: fp32 products and sums.  bf16: fp32 scores and statistics, the
     probabilities (and their gradients) are rounded to bf16 for the second product, the output once at the end.
