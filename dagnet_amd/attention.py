@@ -9,7 +9,8 @@ the graph layers (gat.py, gcn.py) by attention over a scene's agents, or over it
     out = scene_attention_step(q, k_cache, v_cache, k_len, step_layout)                    # the new rows of a rollout's step
 
 The kernels are csrc/scene_attn_*.hip and csrc/rotary.hip behind dagnet_op_attn_* and dagnet_op_rotary (include/dagnet_hip.h), called
-by csrc/torch_calls.cpp.  fp32 and bf16; there is no CPU path.
+by csrc/torch_calls.cpp.  fp32 and bf16; there is no CPU path.  Calls are eager or captured into a graph: tracing, forward-mode derivatives and
+function transforms are refused.
 """
 from __future__ import annotations
 
@@ -49,6 +50,7 @@ class _Tables:
         if got is None:
             if torch.cuda.is_current_stream_capturing():
                 raise DagnetHipError(f"{type(self).__name__}: make it with device=, or call it once, before capturing a graph")
+            _ops.calls().eager()                                                 # a fake upload would be kept for later calls
             t = self._host().to(torch.device("cuda", index))
             got = self._dev[index] = (self._addresses(t) + (t,), stream)
         elif got[1] != stream:

@@ -6,8 +6,10 @@
 // it Python in autograd's own thread, on a cold core) for 35 us on the GPU; these nodes take 55.
 #include <torch/csrc/autograd/custom_function.h>
 #include <torch/csrc/autograd/functions/basic_ops.h>
+#include <torch/csrc/jit/frontend/tracer.h>
 #include <torch/extension.h>
 #include <c10/core/DeviceGuard.h>
+#include <c10/core/impl/TorchDispatchModeTLS.h>
 #include <c10/hip/HIPStream.h>
 
 #include "../../include/dagnet_hip.h"
@@ -45,6 +47,30 @@ Tensor floats(const Tensor &like, int64_t n) { return at::empty({n}, like.option
 Tensor dense(const Tensor &like) { return at::empty_like(like, like.options(), at::MemoryFormat::Contiguous); }
 // a gradient as autograd hands it over -> unit column stride
 Tensor columns(const Tensor &t) { return t.stride(-1) == 1 || t.size(-1) == 1 ? t : t.contiguous(); }
+
+// The entries write through addresses: what records, replays or replaces torch's operations does not see it.  A traced program would return the memory
+// that was allocated for the output as it found it.
+void eager() {
+    using c10::impl::TorchDispatchModeKey;
+    using Modes = c10::impl::TorchDispatchModeTLS;
+    if (torch::jit::tracer::isTracing() || (Modes::any_modes_set() && (Modes::get_mode(TorchDispatchModeKey::FAKE) || Modes::get_mode(TorchDispatchModeKey::PROXY) ||
+                                                                       Modes::get_mode(TorchDispatchModeKey::FUNCTIONAL))))
+        throw Refused("the attention and rotary calls cannot be traced (torch.jit.trace, make_fx, export, fake tensors): call them eagerly, or capture a graph");
+}
+// and what is more than its memory: its tangent would be lost, its values are elsewhere
+void plain(std::initializer_list<const Tensor *> tensors, bool gradients = false) {
+    eager();
+    using c10::DispatchKey;
+    static constexpr c10::DispatchKeySet other({DispatchKey::Python, DispatchKey::Functionalize, DispatchKey::Batched, DispatchKey::FuncTorchBatched,
+                                                DispatchKey::FuncTorchGradWrapper}), lazy({DispatchKey::Negative, DispatchKey::ZeroTensor});
+    for (const Tensor *p : tensors) {
+        if (!p || !p->defined()) continue;
+        const Tensor &t = *p;
+        if (t._fw_grad(0).defined()) throw Refused("the attention and rotary calls have no forward-mode derivative: an argument carries a tangent");
+        if (t.key_set().has_any(gradients ? other : other | lazy))
+            throw Refused("the attention and rotary calls take plain tensors: no subclass with its own dispatch, no function transform's, no lazily negated view (resolve_neg())");
+    }
+}
 
 Tensor given(const std::optional<Tensor> &t) { return t ? *t : Tensor(); }
 
@@ -133,6 +159,7 @@ struct SceneAttn : torch::autograd::Function<SceneAttn> {
         return out;
     }
     static variable_list backward(AutogradContext *ctx, const variable_list &grads) {
+        plain({&grads[0]}, true);
         const Call call = kept<Call>(ctx, "call");
         const Tables &t = call.t;
         const variable_list saved = ctx->get_saved_variables();
@@ -183,6 +210,7 @@ Tables tables_of(const py::tuple &t) {
 Tensor scene_attn(const Tensor &q, const Tensor &k, const Tensor &v, const std::optional<Tensor> &slopes_, const py::tuple &tables, double scale, double softcap,
                   const std::optional<Tensor> &pos_, const std::optional<Tensor> &k_pos_) {
     const Tensor slopes = given(slopes_), pos = given(pos_), k_pos = given(k_pos_);
+    plain({&q, &k, &v, &slopes, &pos, &k_pos});
     const Tables t = tables_of(tables);
     if (at::GradMode::is_enabled() && (q.requires_grad() || k.requires_grad() || v.requires_grad() || (slopes.defined() && slopes.requires_grad()))) {
         const Tensor held = tables[6].cast<Tensor>();       // the tables live as long as a backward pass may read them
@@ -199,7 +227,9 @@ Tensor scene_attn(const Tensor &q, const Tensor &k, const Tensor &v, const std::
 Tensor scene_attn_step(const Tensor &q, const Tensor &k, const Tensor &v, const Tensor &k_len, int64_t q_ptr, int64_t max_rows, const std::optional<Tensor> &slopes_,
                        const std::optional<Tensor> &pos_, const std::optional<Tensor> &k_pos_, double scale, double softcap) {
     py::gil_scoped_release release;
-    dagnet_attn a = arguments(q, k, v, given(slopes_), given(pos_), given(k_pos_), 0, scale, softcap);
+    const Tensor slopes = given(slopes_), pos = given(pos_), k_pos = given(k_pos_);
+    plain({&q, &k, &v, &k_len, &slopes, &pos, &k_pos});
+    dagnet_attn a = arguments(q, k, v, slopes, pos, k_pos, 0, scale, softcap);
     const c10::DeviceGuard guard(q.device());
     const int32_t scenes = (int32_t)k.size(0), room = (int32_t)k.size(1);
     Tensor out = dense(q);
@@ -239,6 +269,7 @@ struct Rotary : torch::autograd::Function<Rotary> {
         return k.defined() ? variable_list{qo, ko} : variable_list{qo};
     }
     static variable_list backward(AutogradContext *ctx, const variable_list &grads) {
+        plain({&grads[0], grads.size() > 1 ? &grads[1] : nullptr}, true);
         const Axes x = kept<Axes>(ctx, "axes");
         const auto was = kept<std::array<int64_t, 2>>(ctx, "pos");
         const Tensor gq = columns(grads[0]), gk = grads.size() > 1 ? columns(grads[1]) : Tensor(), back = ctx->get_saved_variables()[0];
@@ -253,6 +284,7 @@ struct Rotary : torch::autograd::Function<Rotary> {
 py::tuple rotary(const Tensor &q, const std::optional<Tensor> &k_, const Tensor &pos, const py::tuple &tables, int64_t pairs, bool interleaved, bool inplace) {
     const Axes x = {tables[0].cast<int64_t>(), tables[1].cast<int64_t>(), (int32_t)pairs, interleaved};
     const Tensor k = given(k_), held = tables[2].cast<Tensor>();
+    plain({&q, &k, &pos});
     variable_list out;
     {
         py::gil_scoped_release release;
@@ -292,6 +324,7 @@ void bind(const py::dict &addresses, py::object error) {
 
 PYBIND11_MODULE(_dagnet_torch, m) {
     m.def("bind", &bind);
+    m.def("eager", &eager);
     m.def("scene_attn", &scene_attn);
     m.def("scene_attn_step", &scene_attn_step);
     m.def("rotary", &rotary);
