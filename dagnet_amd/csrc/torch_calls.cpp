@@ -45,8 +45,12 @@ void *stream_of(const Tensor &t) { return t.is_cuda() ? c10::hip::getCurrentHIPS
 template <typename T> T *ptr(const Tensor &t) { return t.defined() ? static_cast<T *>(t.data_ptr()) : nullptr; }
 Tensor floats(const Tensor &like, int64_t n) { return at::empty({n}, like.options().dtype(at::kFloat)); }
 Tensor dense(const Tensor &like) { return at::empty_like(like, like.options(), at::MemoryFormat::Contiguous); }
-// a gradient as autograd hands it over -> unit column stride
-Tensor columns(const Tensor &t) { return t.stride(-1) == 1 || t.size(-1) == 1 ? t : t.contiguous(); }
+// a gradient as autograd hands it over -> memory that holds its values, unit column stride
+Tensor columns(const Tensor &t) {
+    if (t._is_zerotensor()) return at::zeros(t.sizes(), t.options());
+    if (t.is_neg()) return t.resolve_neg();
+    return t.stride(-1) == 1 || t.size(-1) == 1 ? t : t.contiguous();
+}
 
 // The entries write through addresses: what records, replays or replaces torch's operations does not see it.  A traced program would return the memory
 // that was allocated for the output as it found it.
@@ -67,7 +71,7 @@ void plain(std::initializer_list<const Tensor *> tensors, bool gradients = false
         if (!p || !p->defined()) continue;
         const Tensor &t = *p;
         if (t._fw_grad(0).defined()) throw Refused("the attention and rotary calls have no forward-mode derivative: an argument carries a tangent");
-        if (t.key_set().has_any(gradients ? other : other | lazy))
+        if (t.key_set().has_any(gradients ? other : other | lazy))       // columns() makes lazy gradients plain
             throw Refused("the attention and rotary calls take plain tensors: no subclass with its own dispatch, no function transform's, no lazily negated view (resolve_neg())");
     }
 }

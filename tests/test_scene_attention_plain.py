@@ -1,5 +1,6 @@
 """CPU: calls that torch's tracing, forward-mode differentiation and function transforms would see wrongly are refused before an entry is called (recorders
-stand for the entries, tests/attn_recorder.py)."""
+stand for the entries, tests/attn_recorder.py); gradients that come lazily are read as what they stand for."""
+import numpy as np
 import pytest
 import torch
 import torch.autograd.forward_ad as fwd
@@ -9,7 +10,7 @@ from torch.fx.experimental.proxy_tensor import make_fx
 from dagnet_amd import _ops
 from dagnet_amd._capi import DagnetHipError
 from dagnet_amd.attention import RotaryAxes, SceneLayout
-from tests.attn_recorder import host_axes, host_tables, recorded
+from tests.attn_recorder import host_axes, host_tables, recorded, rows_at
 
 N, H, KV, D = 6, 2, 1, 4
 NAMES = ("scene_attn", "scene_attn_step", "rotary", "rotary_in_place")
@@ -123,6 +124,23 @@ def test_tables_are_not_made_under_a_fake_mode(monkeypatch):
         with FakeTensorMode(), pytest.raises(DagnetHipError, match="cannot be traced"):
             x.tables(0)
         assert x._dev == {}
+
+
+@pytest.mark.parametrize("kind", ["negated", "zero", "transposed", "expanded"])
+def test_lazy_gradients_are_read_as_what_they_stand_for(kind):
+    g = torch.Generator().manual_seed(1)
+    x = torch.randn((N, H, D), generator=g)
+    dout = {"negated": torch.complex(x, x).conj().imag, "zero": torch._efficientzerotensor((N, H, D)), "transposed": x.transpose(1, 2).contiguous().transpose(1, 2),
+            "expanded": torch.tensor(2.0).expand(N, H, D)}[kind]
+    want = {"negated": -x, "zero": torch.zeros(N, H, D), "transposed": x, "expanded": torch.full((N, H, D), 2.0)}[kind].numpy()
+    got = []
+    with recorded(on_bwd=lambda d: got.append(rows_at(d["dout"], N, H, D, d["do_row"], d["do_head"])),
+                  on_rotary=lambda d: got.append(rows_at(d["q"], N, H, D, d["q_row"], d["q_head"])) if d["inverse"] else None) as m:
+        for name in ("scene_attn", "rotary"):
+            t = _tensors(name)
+            t[0].requires_grad_()
+            torch.autograd.grad(_call(m, name, t), t[0], dout)
+    assert len(got) == 2 and all(np.array_equal(a, want) for a in got)
 
 
 @pytest.mark.parametrize("name", ["scene_attn", "rotary"])
