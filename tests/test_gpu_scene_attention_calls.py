@@ -116,6 +116,31 @@ def test_rows_of_a_step_that_no_scene_owns_stay_as_they_were(room, dt):
     ref.close(out[1:6], want["out"], tol["out"], "step")
 
 
+@pytest.mark.parametrize("dt", [F32, BF16], ids=["fp32", "bf16"])
+@pytest.mark.parametrize("names", [("k", "v"), ("q", "dout"), ("dout",), ("q", "k", "v", "dout")])
+@pytest.mark.parametrize("bad", [float("nan"), float("inf")])
+def test_spoilt_rows_of_another_scene_do_not_reach_split_sums(names, bad, dt):
+    """Two scenes whose border lies inside a tile, large enough that a tile's keys and a tile's rows are split over workgroups; rows of the second one are
+    spoilt next to the border and far from it.  The first scene's results are those of the formulas, the keys beside the border among them."""
+    ptr, H, KV, D = [0, 700, 1500], 4, 2, 24
+    layout = SceneLayout(ptr)
+    t = inputs(17, 1500, 1500, H, KV, D, dt, 1)
+    lib, a = _ops._lib(), Attn(nq=1500, nk=1500, n_heads=H, n_kv_heads=KV, head_dim=D, axes=1, dtype=int(dt is BF16), max_keys=layout.span[0], mean_keys=layout.span[1])
+    more = lib.dagnet_op_attn_bwd_workspace(C.byref(a)) - 2 * 1500 * H
+    assert more >= 2 * 1500 * H * D + 2 * 2 * 1500 * KV * D              # at least two parts of the keys and of the rows
+    cut = {n: t[n][:700].clone() for n in ("q", "k", "v", "dout", "pos")}
+    for n in names:
+        for i in (700, 705, 763, 1400):
+            t[n][i] = bad
+    leaves = [t[n].requires_grad_() for n in ("q", "k", "v", "slopes")]
+    out = scene_attention(*leaves[:3], layout, softcap=8.0, slopes=t["slopes"], pos=t["pos"])
+    grads = torch.autograd.grad(out, leaves, t["dout"])
+    assert not all(torch.isfinite(x[700:]).all() for x in (out,) + grads[:3])
+    want, tol = ref.attention(cut["q"], cut["k"], cut["v"], ref.seen_matrix([0, 700]), D ** -0.5, 8.0, t["slopes"], cut["pos"], cut["pos"], cut["dout"])
+    for name, got in zip(("out", "dq", "dk", "dv"), (out,) + grads[:3]):
+        ref.close(got[:700], want[name], tol[name], name)
+
+
 def test_sums_of_the_slopes_gradient_keep_their_bits_between_key_parts():
     """One row over 1024 keys in eight parts, all scores 0: p = 2^-10, the values' mean is 0, so dslope = -2^-10 sum_j v_j d_j.  With v = +-255 and whole distances
     below 2^12 every fp32 sum of a lane's 16 pairs is exact (16 2^20 = 2^24); a part's 128 need 27 bits, and the parts cancel to fewer than 24."""
