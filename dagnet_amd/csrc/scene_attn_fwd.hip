@@ -309,17 +309,34 @@ template <typename T, int DP, int BN, int MB, bool CAP, int AX> hipError_t launc
     if (A.key_parts > 1) hipLaunchKernelGGL((scene_attn_fwd_join_kernel<T>), dim3((unsigned)(((int64_t)A.nq * A.H + 7) / 8)), dim3(256), 0, st, A);
     return hipGetLastError();
 }
-// Two blocks of 16 rows a wave read K and V from LDS half as often but leave a CU with two workgroups of 128 rows instead of three or four of 64.  Worth
-// it where the products weigh more than the scores' vector work (cap, distance), the more so the wider a head, and where the workgroups fill
-// the chip's 512 places; rows that see unlike numbers of keys need more of them, short tiles filling up behind long ones.  bf16, 8 heads to 2,
-// us with one block and with two:
-//     rows 8192, all seen, no cap: width 64 212 203, 96 364 248, 128 416 304;  causal: 126 164, 178 205, 227 258;  16384 causal: 401 361, 571 502, 812 631
-//     16384, all seen: width 32 549 538;  64, one axis 896 814, cap 1184 1202;  96, cap 1486 1460, cap and an axis 1582 1617;
-//     128, cap and an axis 2136 1749, cap and three axes 2520 2618;  width 96, 544 to 704 workgroups (a second round hardly filled): 385 449, 536 572
+// Workgroups of a kernel that a CU holds at once (its registers and LDS)
+template <void (*KERNEL)(const SceneAttnArgs)> int held() {
+    static const int n = [] {
+        int v = 0;
+        return hipOccupancyMaxActiveBlocksPerMultiprocessor(&v, KERNEL, 256, 0) == hipSuccess && v > 0 ? v : 1;
+    }();
+    return n;
+}
+// Two blocks of 16 rows a wave read K and V from LDS half as often but leave a CU with fewer workgroups, of 128 rows instead of 64.  Worth it where the
+// products weigh more than the scores' vector work (cap, distance), the more so the wider a head (the condition below), and
+// - where rows see alike numbers of keys, if a CU gets through its workgroups in fewer rounds; in as many rounds only where it holds three of them at
+//   once (with two the waits show) and has more than three of 64 rows to do.  bf16, 8 heads to 2, all seen, us with one block and with two, at (tiles of
+//   128 rows, for all heads) 320, 400, 512, 544, 672, 768, 896, 1024, 1152:
+//       width 64 (a CU holds 5 and 3): 119 133, 159 153, 214 198, 288 261, 392 325, 455 380, 599 593, 774 694, 990 893
+//       width 96 (3 and 2):            131 147, 255 187, 339 233, 369 430, 506 530, 596 607, 935 750, 1096 878, 1324 1371;  capped 187 234, 337 293, 438 382,
+//                                      511 635, 729 788, 852 906, 1203 1272, 1471 1451, 1910 2108
+//       width 128 (2 and 2):           230 182, 304 231, 391 290, 579 548, 751 671, 869 765, 1350 934, 1567 1083, 2171 1743;  capped 294 265, 404 329,
+//                                      519 416, 742 763, 993 936, 1139 1074, 1678 1401, 1984 1603, 2691 2472
+// - where they see unlike numbers, from 768 workgroups on: short tiles fill up behind long ones.  Causal, 8192 rows: width 64 126 164, 96 178 205, 128 227 258;
+//   16384: 401 361, 571 502, 812 631
+// What the condition on the width leaves out, 16384 rows, all seen: width 64, cap 1184 1202;  96, cap and an axis 1582 1617;  128, cap and three axes 2520 2618.
 template <typename T, int DP, int BN, bool CAP, int AX> hipError_t rows_fwd(const SceneAttnArgs &A, hipStream_t st) {
     if constexpr (sizeof(T) == 2 && DP >= 64 && (CAP ? 2 : 0) + (AX > 1 ? 2 : AX) < DP / 32) {
-        const int64_t groups = ((int64_t)A.nq * A.G + 127) / 128 * A.KV;
-        if (A.uneven ? groups >= 768 : groups >= 448 && !(DP == 96 && groups > 512 && groups < 768)) return launch_fwd<T, DP, BN, 2, CAP, AX>(A, st);
+        const int64_t R = (int64_t)A.nq * A.G, two = (R + 127) / 128 * A.KV, one = (R + 63) / 64 * A.KV;
+        const int h1 = A.o32 ? held<scene_attn_fwd_kernel<T, DP, BN, 1, CAP, AX, true>>() : held<scene_attn_fwd_kernel<T, DP, BN, 1, CAP, AX, false>>();
+        const int h2 = A.o32 ? held<scene_attn_fwd_kernel<T, DP, BN, 2, CAP, AX, true>>() : held<scene_attn_fwd_kernel<T, DP, BN, 2, CAP, AX, false>>();
+        const int64_t n1 = (one + CUS - 1) / CUS, n2 = (two + CUS - 1) / CUS, rounds1 = (n1 + h1 - 1) / h1, rounds2 = (n2 + h2 - 1) / h2;
+        if (A.uneven ? two >= 768 : rounds2 < rounds1 || (rounds2 == rounds1 && h2 >= 3 && n1 > 3)) return launch_fwd<T, DP, BN, 2, CAP, AX>(A, st);
     }
     return launch_fwd<T, DP, BN, 1, CAP, AX>(A, st);
 }
