@@ -13,6 +13,13 @@ namespace tops {
 
 enum { ACT_NONE = 0, ACT_LRELU = 1, ACT_TANH = 2, ACT_RELU = 3 };
 
+// a b + c d with both products rounded: which of the two a compiler would fuse into the sum depends on what it vectorises, and a tiny batch's BatchNorm
+// amplifies the difference
+__device__ __forceinline__ float sum_of_products(float a, float b, float c, float d) {
+#pragma clang fp contract(off)
+    return a * b + c * d;
+}
+
 __device__ __forceinline__ int64_t gid() { return (int64_t)blockIdx.x * blockDim.x + threadIdx.x; }
 
 // ---------------------------------------------------------------------------------------------
@@ -150,7 +157,7 @@ __global__ void gru_fwd_kernel(int64_t M, int R, const float *__restrict__ gi, c
     const float *a = gi + m * 3 * R, *b = gh + m * 3 * R;
     const float r = sigm(a[f] + b[f]), z = sigm(a[R + f] + b[R + f]);
     const float n = tanhf(a[2 * R + f] + r * b[2 * R + f]);
-    hn[i] = (1.0f - z) * n + z * h[i];
+    hn[i] = sum_of_products(1.0f - z, n, z, h[i]);
     float *g = gates + m * 3 * R;
     g[f] = r; g[R + f] = z; g[2 * R + f] = n;
 }
@@ -416,6 +423,7 @@ __global__ __launch_bounds__(256) void bn_moments_kernel(int64_t M, int N, int r
             for (int r = 1; r < 16; ++r) {
                 const float nb = scnt[r];
                 if (nb > 0.f) {
+#pragma clang fp contract(off)                          // every product rounded before it is added (as in sum_of_products)
                     const float nn = n + nb, d = smean[r][l] - mu;
                     mu += d * (nb / nn);
                     q += sm2[r][l] + d * d * (n * nb / nn);
