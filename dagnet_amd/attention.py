@@ -296,7 +296,10 @@ class RotaryAxes(_Tables):
         self.axes, self.n_pairs = len(self.pairs), sum(self.pairs)
         if self.axes < 1 or min(self.pairs) < 0 or self.n_pairs < 1 or 2 * self.n_pairs > self.head_dim or self.head_dim > 1024:
             raise DagnetHipError(f"pairs {self.pairs}: together 1 .. {self.head_dim // 2} column pairs of a head of {self.head_dim} (at most 1024)")
-        th = np.broadcast_to(np.asarray(theta, dtype=np.float64), (self.axes,))
+        th = np.asarray(theta, dtype=np.float64)
+        if th.shape not in ((), (self.axes,)):
+            raise DagnetHipError(f"theta must be one number or one per axis ({self.axes}), got shape {th.shape}")
+        th = np.broadcast_to(th, (self.axes,))
         if not np.all(np.isfinite(th)) or np.any(th <= 0):
             raise DagnetHipError(f"theta must be positive and finite, got {theta}")
         self.freq = np.concatenate([t ** (-np.arange(n, dtype=np.float64) / n) if n else np.zeros(0) for t, n in zip(th, self.pairs)])

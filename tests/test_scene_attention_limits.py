@@ -2,7 +2,7 @@
 import pytest
 
 from dagnet_amd._capi import DagnetHipError
-from dagnet_amd.attention import SceneLayout
+from dagnet_amd.attention import RotaryAxes, SceneLayout
 
 
 @pytest.mark.parametrize("q,k", [([0, 1], [0, 2 ** 24 + 1]), ([0, 3, 2 ** 24 + 4], [0, 5, 6])])
@@ -15,3 +15,10 @@ def test_places_that_are_no_fp32_numbers(q, k):
 def test_the_last_place_that_is():
     lay = SceneLayout([0, 1], [0, 2 ** 24])
     assert not lay.far and lay._at.max() == 2 ** 24 - 1 == lay._k_at.max()
+
+
+@pytest.mark.parametrize("theta", [(100.0, 10.0, 5.0), (100.0,), [[100.0, 10.0]], ()])
+def test_theta_of_another_number_of_axes(theta):
+    with pytest.raises(DagnetHipError, match="one per axis"):
+        RotaryAxes(16, (4, 4), theta=theta)
+    assert RotaryAxes(16, (8,), theta=100.0).freq[0] == RotaryAxes(16, (8,), theta=[100.0]).freq[0] == 1.0
