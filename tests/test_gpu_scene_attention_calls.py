@@ -167,3 +167,39 @@ def test_a_gradient_of_nan_gives_nan(N, dt):
     out = scene_attention(*leaves, SceneLayout([0, N], causal=1))
     grads = torch.autograd.grad(out, leaves, torch.full_like(out, float("nan")))
     assert torch.isfinite(out).all() and all(g.isnan().all() for g in grads)
+
+
+@pytest.mark.parametrize("dt", [F32, BF16], ids=["fp32", "bf16"])
+@pytest.mark.parametrize("axes", [0, 2])
+def test_a_step_without_keys_or_rows(axes, dt):
+    """A cache without room, one whose scenes keep nothing yet, and a step that brings no rows."""
+    kw = lambda t: dict(slopes=t["slopes"], pos=t["pos"], k_pos=t["k_pos"]) if axes else {}  # noqa: E731
+    for lens, room in (([0, 0], 0), ([0, 0], 700)):
+        t = step_inputs(1, [3, 2], lens, room, 4, 2, 24, dt, axes)
+        got = scene_attention_step(t["q"], t["k"], t["v"], t["k_len"], SceneLayout(t["ptr"]), softcap=5.0, **kw(t))
+        assert got.shape == (5, 4, 24) and (got == 0).all()
+    t = step_inputs(1, [0, 0], [5, 9], 20, 4, 2, 24, dt, axes)
+    assert scene_attention_step(t["q"], t["k"], t["v"], t["k_len"], SceneLayout(t["ptr"]), **kw(t)).shape == (0, 4, 24)
+
+
+@pytest.mark.parametrize("dt", [F32, BF16], ids=["fp32", "bf16"])
+def test_keys_and_values_that_are_one_tensor_or_broadcast(dt):
+    """k and v the same leaf (both gradients meet in it), and k with one head or one row spread over all (strides 0): the spread ones' gradients add up."""
+    ptr = [0, 30, 75]
+    t = inputs(6, 75, 75, 4, 2, 16, dt, 0)
+    layout, seen = SceneLayout(ptr, causal=1), ref.seen_matrix(ptr, None, 1)
+    want, tol = ref.attention(t["q"], t["k"], t["k"], seen, 0.25, 0.0, None, None, None, t["dout"])
+    q, k = t["q"].requires_grad_(), t["k"].requires_grad_()
+    dq, dk = torch.autograd.grad(scene_attention(q, k, k, layout), (q, k), t["dout"])
+    ref.close(dq, want["dq"], tol["dq"], "dq")
+    both_ = want["dk"] + want["dv"]
+    ref.close(dk, both_, tol["dk"] + tol["dv"] + (ref.ROUND[dt] + ref.U) * both_.abs(), "dk + dv")
+    for narrow in (t["k"].detach()[:, :1], t["k"].detach()[:1]):
+        leaf = narrow.clone().requires_grad_()
+        got, = torch.autograd.grad(scene_attention(q, leaf.expand(75, 2, 16), t["v"], layout), leaf, t["dout"])
+        want, tol = ref.attention(t["q"], narrow.expand(75, 2, 16), t["v"], seen, 0.25, 0.0, None, None, None, t["dout"])
+        d = 1 if narrow.shape[1] == 1 else 0
+        n = narrow.expand(75, 2, 16).shape[d]
+        # torch adds the n gradients in fp32 (bf16: rounded once more at the end)
+        ref.close(got, want["dk"].sum(d, keepdim=True), tol["dk"].sum(d, keepdim=True) + n * ref.U * want["dk"].abs().sum(d, keepdim=True)
+                  + 2 * ref.ROUND[dt] * want["dk"].sum(d, keepdim=True).abs(), "spread")
