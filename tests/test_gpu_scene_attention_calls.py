@@ -203,3 +203,37 @@ def test_keys_and_values_that_are_one_tensor_or_broadcast(dt):
         # torch adds the n gradients in fp32 (bf16: rounded once more at the end)
         ref.close(got, want["dk"].sum(d, keepdim=True), tol["dk"].sum(d, keepdim=True) + n * ref.U * want["dk"].abs().sum(d, keepdim=True)
                   + 2 * ref.ROUND[dt] * want["dk"].sum(d, keepdim=True).abs(), "spread")
+
+
+@pytest.mark.parametrize("dt", [F32, BF16], ids=["fp32", "bf16"])
+def test_offsets_beyond_32_bits(dt):
+    """Rows 2^31 + 64 elements apart (the fourth one begins beyond 2^32 elements), and scenes of a cache 2^32 + 64 apart: the bits of the packed call."""
+    n, H, KV, D, far = 4, 4, 2, 16, 2 ** 31 + 64
+    t = inputs(4, n, n, H, KV, D, dt, 0)
+    big = torch.empty(3 * far + 4096, dtype=dt, device=DEV)
+    views, at = {}, 0
+    for name, heads in (("q", H), ("k", KV), ("v", KV), ("dout", H)):
+        views[name] = big.as_strided((n, heads, D), (far, D, 1), at)
+        views[name].copy_(t[name])
+        at += heads * D
+    assert big.numel() > 2 ** 32
+
+    def run(x):
+        leaves = [x[m].detach().requires_grad_() for m in ("q", "k", "v")]
+        out = scene_attention(*leaves, SceneLayout([0, n], causal=1))
+        return (out,) + torch.autograd.grad(out, leaves, x["dout"])
+    for a, b in zip(run(views), run(t)):
+        assert torch.equal(a, b)
+    axes, pos = RotaryAxes(D, (4, 4)), torch.rand((n, 2), device=DEV) * 50
+    want = rotary(t["q"], t["k"], pos, axes)
+    for a, b in zip(rotary(views["q"], views["k"], pos, axes), want):
+        assert torch.equal(a, b)
+    rotary(views["q"], views["k"], pos, axes, inplace=True)
+    assert torch.equal(views["q"], want[0]) and torch.equal(views["k"], want[1])
+    s = step_inputs(9, [2, 1], [700, 650], 700, H, KV, D, dt, 0)
+    for name in ("k", "v"):
+        c = big.as_strided((2, 700, KV, D), (2 ** 32 + 64, 2 * KV * D, D, 1), 0 if name == "k" else KV * D)
+        c.copy_(s[name])
+        views["c" + name] = c
+    layout = SceneLayout(s["ptr"])
+    assert torch.equal(scene_attention_step(s["q"], views["ck"], views["cv"], s["k_len"], layout), scene_attention_step(s["q"], s["k"], s["v"], s["k_len"], layout))
