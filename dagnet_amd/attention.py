@@ -211,7 +211,8 @@ def scene_attention(q, k, v, layout: SceneLayout, *, scale: Optional[float] = No
     positions stay below 1e19: their squares leave fp32 beyond, such a key has no weight for a positive slope, and a slope of 0 and the slopes' gradient give NaN.
     Differentiable in q, k, v and slopes; gradients repeat bit for bit.  A row that sees nothing gives 0; what stands in keys a row does
     not see (infinities and NaN included) does not reach it.  fp32: fp32 products and sums.  bf16: fp32 scores and statistics, the
-    probabilities (and their gradients) are rounded to bf16 for the second product, the output once at the end.
+    probabilities (and their gradients) are rounded to bf16 for the second product, the output once at the end; where gradients are wanted the forward takes the
+    probabilities as two bf16 terms (its output may differ in the last bit from a call without).
     A captured graph replays with the layout's tables: keep the layout as long as the graph."""
     if not isinstance(layout, SceneLayout):
         raise DagnetHipError("layout must be a SceneLayout")
@@ -253,7 +254,7 @@ def scene_attention_step(q, k_cache, v_cache, k_len, layout: SceneLayout, *, sca
     q [nq, heads, head_dim]; k_cache, v_cache [S, room, key heads, head_dim] with any strides but the last; k_len int32 [S] ON THE DEVICE (a
     captured call follows a growing cache; values are clamped to 0 .. room); pos [nq, 1 .. 3] and k_pos [S, room, ..] with slopes.  Write
     the new rows' own keys into the cache first if they are to see each other.  What stands behind k_len does not matter; an infinity or NaN in
-    a key that is seen makes its rows not finite.  No gradient.  -> [nq, heads, head_dim]."""
+    a key that is seen may make its rows not finite.  Roundings as in scene_attention without gradients.  No gradient.  -> [nq, heads, head_dim]."""
     if not isinstance(layout, SceneLayout):
         raise DagnetHipError("layout must be a SceneLayout")
     if layout.masked or not layout.same_rows:

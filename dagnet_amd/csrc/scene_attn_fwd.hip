@@ -4,10 +4,12 @@
 // tile's loads going straight into the other copy while the current one is worked on.  A wave skips 16-key blocks that none of its rows sees, so a tile that holds
 // several small scenes costs each wave its own scenes only.
 //
-// Bound by: vector instructions, 24 to 36 a score with a cap and distances (three of them at a quarter of the rate: exponential, quotient, root), 12
-// without, beside 4 D / 1024 matrix clocks.  Measured, bf16, all keys seen: 16384 rows of 8 heads of 96 to 2, 0.89 ms (926 TFLOP/s, a plain 8192^3 product
-// reaches 1195); capped 1.46 ms; 128 wide 1.10 ms (1001 TFLOP/s).  Small scenes are bound by one workgroup's chain of loads: 4096 fp32 scenes of ten rows, 4
-// heads of 16, 24 us (42 MB, 1.7 TB/s); four times the workgroups a CU (tiles of 32 keys) changed nothing there.
+// Bound by vector instructions, by counters (masked places and filled-up tiles among them): bf16 with cap, three axes and the exact second product 40 a
+// visible score (32 scenes of 500 rows; issuing in 72 % of the CUs' busy clocks), with cap and one axis 22 (long causal rows of 128; 75 %), without either and with
+// the exact product 15 (4093 causal rows of 96; 59 %, LDS reads 45 %).  Three of them run at a quarter of the rate: exponential, quotient, root.
+// Measured, bf16, all keys seen: 16384 rows of 8 heads of 96 to 2, 0.87 ms (945 TFLOP/s, a plain 8192^3 product reaches 1195); capped 1.44 ms; 128 wide 1.08 ms
+// (1015 TFLOP/s).  Small scenes are bound by one workgroup's chain of loads: 4096 fp32 scenes of ten rows, 4 heads of 16, 25 us (42 MB, 1.7 TB/s); four times
+// the workgroups a CU (tiles of 32 keys) changed nothing there.
 #include "scene_attn.h"
 
 namespace sattn {

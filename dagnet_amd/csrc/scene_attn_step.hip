@@ -7,7 +7,8 @@
 // outputs, maxima and sums meet in scene_attn_join_kernel.
 //
 // Bound by the cache's bytes: bf16, 4 sequences of 60 000 to 131 071 keys, 4 key heads of 128, one row each: 184 us for 887 MB, 4.8 TB/s - what a large copy
-// reaches.  256 scenes of ten rows over 400 to 2000 keys (8 heads of 64 to 2, cap, three axes): 70 us for 139 MB; there the blocks' vector work counts.
+// reaches.  256 scenes of ten rows over 280 to 2000 keys (8 heads of 64 to 2, cap, three axes): 72 us for 139 MB; there the blocks' vector work counts
+// (58 instructions a score, issuing in 59 % of the busy clocks).
 #include "scene_attn.h"
 #include "scene_attn_step.h"
 #include <algorithm>
@@ -257,7 +258,7 @@ extern "C" hipError_t dn_scene_attn_step_f32(const SceneStepArgs *A, hipStream_t
 // rows: packed rows of the largest scene; kv_scenes: scenes x kv heads.  Splits of the keys: 1536 workgroups in all - two or three full rounds of what the
 // chip's 256 CUs hold at once (1024 left a third of a round at its end: 131 000 keys of 64 rows 215 us, 185 with 1536) - but none below 256 keys of the
 // cache.  Several blocks of 16 rows that share keys are workgroups of their own: one workgroup for two blocks halves the reads, which
-// come from L2 then, but its registers leave half as many waves (2000 keys of 256 scenes, 34 packed rows: 85 us, 70 in blocks of their own).
+// come from L2 then, but its registers leave half as many waves (2000 keys of 256 scenes, 34 packed rows: 85 us, 72 in blocks of their own).
 extern "C" void dn_scene_attn_step_shape(int64_t rows, int64_t kv_scenes, int room, int *cblocks, int *splits) {
     *cblocks = (int)((rows + 15) / 16);
     const int64_t groups = kv_scenes * *cblocks, want = (1536 + groups - 1) / groups, most = ((int64_t)room + 255) / 256;
