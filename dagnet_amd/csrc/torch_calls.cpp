@@ -45,7 +45,7 @@ void *stream_of(const Tensor &t) { return t.is_cuda() ? c10::hip::getCurrentHIPS
 template <typename T> T *ptr(const Tensor &t) { return t.defined() ? static_cast<T *>(t.data_ptr()) : nullptr; }
 Tensor floats(const Tensor &like, int64_t n) { return at::empty({n}, like.options().dtype(at::kFloat)); }
 Tensor dense(const Tensor &like) { return at::empty_like(like, like.options(), at::MemoryFormat::Contiguous); }
-// a gradient as autograd hands it over -> memory that holds its values, unit column stride
+// a gradient, or what a hook returned, as autograd hands it over -> memory that holds its values, unit column stride
 Tensor columns(const Tensor &t) {
     if (t._is_zerotensor()) return at::zeros(t.sizes(), t.options());
     if (t.is_neg()) return t.resolve_neg();
@@ -178,13 +178,13 @@ struct SceneAttn : torch::autograd::Function<SceneAttn> {
             unpacked(saved[3], {heads}, at::kFloat, dout.device(), "slopes");
             unpacked(saved[4], {rows, call.axes}, at::kFloat, dout.device(), "pos");
             unpacked(saved[5], {call.nk, call.axes}, at::kFloat, dout.device(), "k_pos");
-            slopes = saved[3].contiguous();
-            pos = saved[4].contiguous();
-            k_pos = saved[5].contiguous();
+            slopes = columns(saved[3]).contiguous();
+            pos = columns(saved[4]).contiguous();
+            k_pos = columns(saved[5]).contiguous();
         }
         unpacked(saved[6], {rows * heads}, at::kFloat, dout.device(), "the rows' statistics");
         unpacked(saved[7], {rows, heads, D}, at::kFloat, dout.device(), "the output");
-        const Tensor q = columns(saved[0]), k = columns(saved[1]), v = columns(saved[2]), lse = saved[6].contiguous(), o = saved[7].contiguous();
+        const Tensor q = columns(saved[0]), k = columns(saved[1]), v = columns(saved[2]), lse = columns(saved[6]).contiguous(), o = columns(saved[7]).contiguous();
         dagnet_attn a = arguments(q, k, v, slopes, pos, k_pos, call.nk, call.scale, call.softcap);
         a.max_keys = t.max_keys;
         a.mean_keys = t.mean_keys;
@@ -278,7 +278,7 @@ struct Rotary : torch::autograd::Function<Rotary> {
         const auto was = kept<std::array<int64_t, 2>>(ctx, "pos");
         const Tensor gq = columns(grads[0]), gk = grads.size() > 1 ? columns(grads[1]) : Tensor(), back = ctx->get_saved_variables()[0];
         unpacked(back, {gq.size(0), was[0]}, (at::ScalarType)was[1], gq.device(), "pos");
-        const Tensor pos = back.contiguous();
+        const Tensor pos = columns(back).contiguous();
         const Tensor dq = dense(gq), dk = gk.defined() ? dense(gk) : Tensor();
         turn(gq, gk, pos, x, true, dq, dk);
         return once({dq, dk, Tensor(), Tensor(), Tensor()}, "rotary");

@@ -50,33 +50,36 @@ def _expect(got, leaves, pos, layout):
 class _Moved:
     """Hooks that keep what they pack as copies at other places, with other strides, and spoil what was saved once the forward has gone."""
 
-    def __init__(self, dense=True):
-        self.spoil, self.out, self.dense = [], [], dense
+    def __init__(self, form="dense"):
+        self.spoil, self.out, self.form = [], [], form
 
     def pack(self, t):
         self.spoil.append(t)
         return t.detach().clone()
 
     def unpack(self, t):
-        if self.dense:
+        if self.form == "dense":
             t = t.clone()
-        else:                                                          # the same values, every second element of a row
+        elif self.form == "strided":                                   # the same values, every second element of a row
             t = torch.stack([t, t], -1)[..., 0]
+        else:                                                          # the same values, their signs in memory the other way round
+            t = torch._neg_view(-t)
+            assert t.is_neg()
         self.out.append(t)
         return t
 
 
-@pytest.mark.parametrize("dense", [True, False])
-def test_the_backward_reads_what_the_hooks_return(dense):
+@pytest.mark.parametrize("form", ["dense", "strided", "negated"])
+def test_the_backward_reads_what_the_hooks_return(form):
     leaves, pos = _inputs()
     layout = SceneLayout([0, 4, N], causal=1)
-    got, hooks = [], _Moved(dense)
+    got, hooks = [], _Moved(form)
 
     def on_bwd(d):
         got.append(_read(d))
         assert np.array_equal(floats_at(d["lse"], N * H), np.arange(N * H)) and (floats_at(d["o"], N * H * D) == 0.25).all()
         inside = [range(t.untyped_storage().data_ptr(), t.untyped_storage().data_ptr() + t.untyped_storage().nbytes()) for t in hooks.out]
-        if dense:                                                      # and not what was saved
+        if form == "dense":                                            # and not what was saved
             for n in ("q", "k", "v", "slopes", "q_pos", "k_pos"):
                 assert any(getattr(d["a"], n) in r for r in inside), n
     with recorded(on_fwd=_fill, on_bwd=on_bwd) as m:

@@ -109,7 +109,7 @@ def test_lazily_negated_views_are_refused(entries, name):
     m, called = entries
     for i in range(len(_tensors(name))):
         t = _tensors(name)
-        t[i] = torch.complex(t[i], t[i]).conj().imag
+        t[i] = torch._neg_view(t[i])
         assert t[i].is_neg()
         with pytest.raises(DagnetHipError, match="resolve_neg"):
             _call(m, name, t)
@@ -130,7 +130,7 @@ def test_tables_are_not_made_under_a_fake_mode(monkeypatch):
 def test_lazy_gradients_are_read_as_what_they_stand_for(kind):
     g = torch.Generator().manual_seed(1)
     x = torch.randn((N, H, D), generator=g)
-    dout = {"negated": torch.complex(x, x).conj().imag, "zero": torch._efficientzerotensor((N, H, D)), "transposed": x.transpose(1, 2).contiguous().transpose(1, 2),
+    dout = {"negated": torch._neg_view(x), "zero": torch._efficientzerotensor((N, H, D)), "transposed": x.transpose(1, 2).contiguous().transpose(1, 2),
             "expanded": torch.tensor(2.0).expand(N, H, D)}[kind]
     want = {"negated": -x, "zero": torch.zeros(N, H, D), "transposed": x, "expanded": torch.full((N, H, D), 2.0)}[kind].numpy()
     got = []
